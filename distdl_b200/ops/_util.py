@@ -14,6 +14,16 @@ def stream_ptr(t: torch.Tensor = None) -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """``_native.call(name, *args, stream)`` on the device of ``t`` and its current stream, whichever device is current."""
+    device = t.get_device()
+    if device == torch._C._cuda_getDevice():
+        _native.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            _native.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+
+
 # the process environment as os.environ keeps it (bytes on POSIX): a look-up per launch that sees every
 # change made through os.environ, without the encoding and the exception of os.environ.get
 _environ = getattr(os.environ, "_data", None)

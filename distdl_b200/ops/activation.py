@@ -117,7 +117,7 @@ def rope_table_ranges(ranges, head_dim: int, theta: float, device) -> torch.Tens
 
 
 def rope_(qkv: torch.Tensor, seq: int, nheads: int, theta: float = 500000.0, offset: int = 0,
-          ranges=None, layout=None) -> torch.Tensor:
+          ranges=None, layout=None, *, rotary=None, positions=None) -> torch.Tensor:
     """Applies rotary position embedding (rotate-half convention) to the first
     ``nheads`` heads of ``qkv`` [tokens, heads_total, head_dim]; position of a
     token is ``offset`` plus its index modulo ``seq`` (``offset`` > 0 for a worker that holds a
@@ -127,7 +127,16 @@ def rope_(qkv: torch.Tensor, seq: int, nheads: int, theta: float = 500000.0, off
     ``layout = (tokens, heads_total, head_dim)``: ``qkv`` is the projection's own output in
     whatever shape it has (say ``[batch, seq, heads_total * head_dim]``) and is only READ in that
     layout.  Prefer this form: rotating a reshaped VIEW in place makes autograd copy the whole
-    gradient twice in the backward pass."""
+    gradient twice in the backward pass.
+
+    ``rotary`` (an :class:`~distdl_b200.ops.Rotary`, in the place of ``theta``): other pairings, a part of the head, long
+    contexts.  ``positions`` (int64 or int32, on the device of ``qkv``): a position per token, or per place in a sequence.
+    With either of them bf16, fp16 and fp32 heads are turned in place, at any strides with unit stride inside a head;
+    :func:`~distdl_b200.ops.rope` leaves its input alone."""
+    if rotary is not None or positions is not None:
+        from .rotary import Rotary, rope_in_place
+        return rope_in_place(qkv, seq, nheads, Rotary(theta=theta) if rotary is None else rotary, offset, ranges, positions,
+                             layout)
     if layout is not None:
         if use_native(qkv) and qkv.dtype == torch.bfloat16 and layout[2] % 16 == 0 and qkv.is_contiguous():
             tokens, ht, hd = (int(v) for v in layout)

@@ -1,0 +1,452 @@
+"""Rotary positions in their usual variants, and the norm of every query and key head with the rotation in the same pass
+(kernels in ``csrc/heads.cu``).  New relative to the reference, which has no attention code."""
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from .. import _native
+from ._util import call_on, main_grad_now, ptr, use_native
+
+_v, _i, _l, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+_native.declare("dd_rotate_heads", [_v, _l, _l, _v, _l, _l, _l, _i, _i, _i, _i, _i, _v, _f, _f, _v, _i, _l, _l, _i, _v])
+_native.declare("dd_norm_heads_fwd", [_v, _l, _l, _v, _l, _l, _v, _v, _i, _f, _l, _i, _i, _i, _i, _i, _i, _v, _f, _v, _i, _l,
+                                      _l, _i, _v])
+_native.declare("dd_norm_heads_bwd", [_v, _l, _l, _v, _l, _l, _v, _l, _l, _v, _v, _i, _f, _v, _v, _i, _v, _l, _i, _i, _i, _i,
+                                      _i, _i, _v, _f, _v, _i, _l, _l, _i, _v])
+_native.declare("dd_heads_parts", [])
+
+_DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_SCALINGS = (None, "linear", "ntk", "yarn", "bands")
+
+
+@dataclass(frozen=True)
+class Rotary:
+    """How positions turn the pairs of a head's components: pair ``i`` at position ``p`` by the angle ``p * f_i``,
+    ``f_i = theta^(-2 i / dim)``.
+
+    ``dim``: the leading components that turn (an even number; None: the whole head).  ``interleaved``: neighbours
+    ``(2 i, 2 i + 1)`` are a pair, instead of ``(i, i + dim / 2)``.  ``scaling`` stretches the frequencies for contexts
+    ``factor`` times longer than the ``original`` one:
+
+    * ``"linear"``: ``f_i / factor``;
+    * ``"ntk"``: ``theta * factor^(dim / (dim - 2))`` in the place of ``theta``;
+    * ``"bands"``: with ``n_i = original f_i / (2 pi)`` turns over the original context, pairs with ``n_i > high`` stay, those
+      with ``n_i < low`` get ``f_i / factor``, between them a weighted mean;
+    * ``"yarn"``: the same from the pair that turns ``fast`` times (stays) to the one that turns ``slow`` times, along the
+      pairs' numbers, and all results times ``magnitude`` (None: ``0.1 ln(factor) + 1``).
+
+    ``magnitude`` (1 where it is None, but for ``"yarn"``) multiplies what is turned; components behind ``dim`` stay as
+    they are."""
+    theta: float = 500000.0
+    dim: Optional[int] = None
+    interleaved: bool = False
+    scaling: Optional[str] = None
+    factor: float = 1.0
+    original: Optional[int] = None
+    low: float = 1.0
+    high: float = 4.0
+    fast: float = 32.0
+    slow: float = 1.0
+    magnitude: Optional[float] = None
+
+    def __post_init__(self):
+        if not (math.isfinite(self.theta) and self.theta > 1.0):
+            raise ValueError(f"theta must be finite and above 1, not {self.theta}")
+        if self.dim is not None and (self.dim < 0 or self.dim % 2):
+            raise ValueError(f"dim must be even, not {self.dim}")
+        if self.scaling not in _SCALINGS:
+            raise ValueError(f"scaling must be one of {_SCALINGS}, not {self.scaling!r}")
+        if self.scaling is not None and not (math.isfinite(self.factor) and self.factor >= 1.0):
+            raise ValueError(f"factor must be finite and at least 1, not {self.factor}")
+        if self.scaling in ("yarn", "bands") and (self.original is None or self.original < 1):
+            raise ValueError(f"scaling {self.scaling!r} needs the original context length")
+        if self.scaling == "bands" and not 0 <= self.low < self.high:
+            raise ValueError(f"bands need 0 <= low < high, not {self.low} and {self.high}")
+        if self.scaling == "yarn" and not 0 < self.slow < self.fast:
+            raise ValueError(f"yarn needs 0 < slow < fast, not {self.slow} and {self.fast}")
+        if self.magnitude is not None and not math.isfinite(self.magnitude):
+            raise ValueError("magnitude must be finite")
+
+    def rotated(self, head_dim: int) -> int:
+        """The leading components of a head that turn."""
+        dim = head_dim - head_dim % 2 if self.dim is None else self.dim
+        if self.dim is None and head_dim % 2:
+            raise ValueError(f"heads of {head_dim} components: say how many of them turn (dim)")
+        if dim > head_dim:
+            raise ValueError(f"{dim} components are to turn, the heads have {head_dim}")
+        if self.scaling == "ntk" and dim == 2:
+            raise ValueError("scaling 'ntk' needs more than one pair")
+        return dim
+
+    @property
+    def scale(self) -> float:
+        """What multiplies the turned components."""
+        if self.magnitude is not None:
+            return float(self.magnitude)
+        return 0.1 * math.log(self.factor) + 1.0 if self.scaling == "yarn" else 1.0
+
+    def frequencies(self, head_dim: int) -> tuple:
+        """``f_i`` of the pairs of a head, in radians per position (64 bits)."""
+        return _frequencies(self, self.rotated(head_dim))
+
+
+@functools.lru_cache(maxsize=256)
+def _frequencies(rotary: Rotary, dim: int) -> tuple:
+    theta, factor = float(rotary.theta), float(rotary.factor)
+    if rotary.scaling == "ntk" and dim:
+        theta *= factor ** (dim / (dim - 2))
+    out = []
+    for i in range(dim // 2):
+        f = theta ** (-2.0 * i / dim)
+        if rotary.scaling == "linear":
+            f /= factor
+        elif rotary.scaling == "bands":
+            keep = (rotary.original * f / (2 * math.pi) - rotary.low) / (rotary.high - rotary.low)
+            keep = min(1.0, max(0.0, keep))
+            f = keep * f + (1.0 - keep) * f / factor
+        elif rotary.scaling == "yarn":
+            first, last = (dim * math.log(rotary.original / (2 * math.pi * turns)) / (2 * math.log(theta))
+                           for turns in (rotary.fast, rotary.slow))
+            first, last = max(math.floor(first), 0), min(math.ceil(last), dim - 1)
+            slowed = min(1.0, max(0.0, (i - first) / max(last - first, 1e-3)))
+            f = (1.0 - slowed) * f + slowed * f / factor
+        out.append(f)
+    return tuple(out)
+
+
+@functools.lru_cache(maxsize=256)
+def _turns(rotary: Rotary, head_dim: int):
+    """(components that turn, frequencies in turns per position as a C array, its address)."""
+    dim = rotary.rotated(head_dim)
+    arr = (ctypes.c_double * max(1, dim // 2))(*(f / (2 * math.pi) for f in _frequencies(rotary, dim)))
+    return dim, arr, ctypes.addressof(arr)
+
+
+_range_positions = {}
+
+
+def _positions_of_ranges(ranges, device) -> torch.Tensor:
+    """Positions of a local sequence made of several ranges ``((start, length), ...)``, kept per device."""
+    key = (tuple((int(a), int(n)) for a, n in ranges), str(device))
+    p = _range_positions.get(key)
+    if p is None:
+        p = torch.cat([torch.arange(a, a + n, dtype=torch.int64) for a, n in key[0]]).to(device)
+        _range_positions[key] = p
+    return p
+
+
+def _where(qkv, rotary, seq, offset, ranges, positions):
+    """The arguments that say how ``qkv [tokens, heads, head_dim]`` is turned: (rotary, positions or None, seq, offset)."""
+    if rotary is None:
+        return None, None, 1, 0
+    if not isinstance(rotary, Rotary):
+        raise TypeError(f"rotary must be an ops.Rotary, not {type(rotary).__name__}")
+    if ranges is not None:
+        if positions is not None or offset:
+            raise ValueError("give positions, ranges or an offset, not several of them")
+        positions = _positions_of_ranges(ranges, qkv.device)
+        if positions.numel() != seq:
+            raise ValueError(f"the ranges hold {positions.numel()} positions, a sequence has {seq} tokens")
+    if positions is None:
+        if seq < 1:
+            raise ValueError(f"a sequence has at least one token, not {seq}")
+        return rotary, None, int(seq), int(offset)
+    if offset:
+        raise ValueError("give positions or an offset, not both")
+    if positions.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"positions must be int64 or int32, not {positions.dtype}")
+    if positions.device != qkv.device:
+        raise ValueError(f"positions are on {positions.device}, the heads on {qkv.device}")
+    n, tokens = positions.numel(), qkv.shape[0]
+    if n != tokens and n != seq or (n == 0 and tokens) or (n and tokens % n):
+        raise ValueError(f"{n} positions for {tokens} tokens in sequences of {seq}: one per token, or one per place in a "
+                         f"sequence")
+    positions = positions.reshape(-1)
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    return rotary, positions, max(1, n), 0
+
+
+def _angles(qkv, rotary, positions, seq, offset):
+    """(cos, sin) [tokens, 1, dim / 2] times the magnitude, fp32 from 64 bits (plain path)."""
+    f = torch.tensor(rotary.frequencies(qkv.shape[2]), dtype=torch.float64, device=qkv.device)
+    at = torch.arange(qkv.shape[0], device=qkv.device) % seq
+    at = at + offset if positions is None else positions[at]
+    angle = (at.double().unsqueeze(1) * f).unsqueeze(1)
+    wide = torch.float64 if qkv.dtype == torch.float64 else torch.float32
+    return (rotary.scale * angle.cos()).to(wide), (rotary.scale * angle.sin()).to(wide)
+
+
+def _rotated(x, cos, sin, dim, interleaved):
+    if interleaved:
+        a, b = x[..., 0:dim:2], x[..., 1:dim:2]
+        turned = torch.stack([a * cos - b * sin, b * cos + a * sin], dim=-1).flatten(-2)
+    else:
+        a, b = x[..., :dim // 2], x[..., dim // 2:dim]
+        turned = torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1)
+    return torch.cat([turned, x[..., dim:]], dim=-1)
+
+
+def _wide(x):
+    return x if x.dtype == torch.float64 else x.float()
+
+
+def _plain_rope(qkv, nheads, where):
+    rotary, positions, seq, offset = where
+    cos, sin = _angles(qkv, rotary, positions, seq, offset)
+    y = _rotated(_wide(qkv[:, :nheads]), cos, sin, rotary.rotated(qkv.shape[2]), rotary.interleaved)
+    return torch.cat([y.to(qkv.dtype), qkv[:, nheads:]], dim=1)
+
+
+def _native_ok(qkv):
+    return use_native(qkv) and qkv.dtype in _DTYPE and 1 <= qkv.shape[2] <= 512
+
+
+def _unit(t):
+    """``t`` with its components next to one another."""
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def _heads(t):
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def _turn_args(where, head_dim):
+    rotary, positions, seq, offset = where
+    if rotary is None:
+        return (0, 0, 0, 1.0), (0, 0, 0, 1)
+    dim, _arr, address = _turns(rotary, head_dim)
+    wide = positions is not None and positions.dtype == torch.int64
+    return (dim, int(rotary.interleaved), address, rotary.scale), (ptr(positions), int(wide), offset, seq)
+
+
+def _rotate(src, dst, nheads, where, sign):
+    tokens, heads, hd = src.shape
+    (dim, near, address, scale), place = _turn_args(where, hd)
+    call_on(src, "dd_rotate_heads", *_heads(src), *_heads(dst), tokens, heads, nheads, hd, dim, near, address, scale, sign,
+            *place, _DTYPE[src.dtype])
+
+
+class _RopeFn(torch.autograd.Function):
+    """The rotation into a new tensor; its gradient is the rotation backwards, a call of the same function."""
+
+    @staticmethod
+    def forward(ctx, qkv, nheads, rotary, positions, seq, offset, sign):
+        ctx.save_for_backward(positions)
+        ctx.cfg = (nheads, rotary, seq, offset, sign)
+        src = _unit(qkv)
+        out = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        _rotate(src, out, nheads, (rotary, positions, seq, offset), sign)
+        return out
+
+    @staticmethod
+    def backward(ctx, d):
+        nheads, rotary, seq, offset, sign = ctx.cfg
+        (positions,) = ctx.saved_tensors
+        return _RopeFn.apply(d, nheads, rotary, positions, seq, offset, -sign), None, None, None, None, None, None
+
+
+class _RopeInPlaceFn(torch.autograd.Function):
+    """The rotation in place of ``qkv``, which is read in the layout ``[tokens, heads, head_dim]``.  (The gradient is turned
+    into a new tensor: the incoming one may be the caller's own.)"""
+
+    @staticmethod
+    def forward(ctx, qkv, layout, nheads, rotary, positions, seq, offset):
+        ctx.mark_dirty(qkv)
+        ctx.save_for_backward(positions)
+        ctx.cfg = (layout, nheads, rotary, seq, offset)
+        t = qkv.view(layout)
+        _rotate(t, t, nheads, (rotary, positions, seq, offset), 1.0)
+        return qkv
+
+    @staticmethod
+    def backward(ctx, d):
+        layout, nheads, rotary, seq, offset = ctx.cfg
+        (positions,) = ctx.saved_tensors
+        g = _RopeFn.apply(d.reshape(layout), nheads, rotary, positions, seq, offset, -1.0)
+        return g.reshape(d.shape), None, None, None, None, None, None
+
+
+def _check_heads(qkv, nheads):
+    if qkv.dim() != 3 or not qkv.is_floating_point():
+        raise ValueError(f"heads come as a floating-point tensor [tokens, heads, head_dim], not {tuple(qkv.shape)} "
+                         f"{qkv.dtype}")
+    if not 0 <= nheads <= qkv.shape[1]:
+        raise ValueError(f"{nheads} heads are asked for, there are {qkv.shape[1]}")
+
+
+def _overlaps(t):
+    """Whether elements of ``t [tokens, heads, head_dim]`` may share memory (as those of an expanded tensor do)."""
+    need = 1
+    for stride, n in sorted(zip(t.stride(), t.shape)):
+        if n > 1:
+            if stride < need:
+                return True
+            need = stride * (n - 1) + need
+    return False
+
+
+def rope(qkv: torch.Tensor, seq: int, nheads: int, *, rotary: Rotary, offset: int = 0, ranges=None,
+         positions=None) -> torch.Tensor:
+    """``qkv [tokens, heads, head_dim]`` with its first ``nheads`` heads turned by their positions, the others copied; ``qkv``
+    itself stays as it is (:func:`distdl_b200.ops.rope_` turns it in place).
+
+    A token's position is ``offset`` plus its index modulo ``seq``, or comes from ``ranges = ((start, length), ...)``
+    adding up to ``seq``, or from ``positions`` (int64 or int32, on the device): one per token, or one per place in a
+    sequence of ``seq``.  bf16, fp16 and fp32 heads of up to 512 components run on the kernel, at any strides with unit
+    stride inside a head; the angles are formed in 64 bits, so that positions may be as far as 2^31.  Differentiable any
+    number of times."""
+    _check_heads(qkv, nheads)
+    if rotary is None:
+        raise ValueError("rope needs a Rotary")
+    where = _where(qkv, rotary, seq, offset, ranges, positions)
+    rotary.rotated(qkv.shape[2])
+    if _native_ok(qkv):
+        return _RopeFn.apply(qkv, nheads, *where, 1.0)
+    return _plain_rope(qkv, nheads, where)
+
+
+def rope_in_place(qkv, seq, nheads, rotary, offset=0, ranges=None, positions=None, layout=None):
+    """:func:`distdl_b200.ops.rope_` with a :class:`Rotary`."""
+    shape = tuple(qkv.shape) if layout is None else tuple(int(v) for v in layout)
+    if layout is not None and qkv.numel() != math.prod(shape):
+        raise ValueError(f"a tensor {tuple(qkv.shape)} cannot be read as {shape}")
+    try:
+        t = qkv.detach().view(shape)
+    except RuntimeError:                    # its strides do not allow it
+        t = None
+    read = qkv.detach().reshape(shape) if t is None else t
+    _check_heads(read, nheads)
+    where = _where(read, rotary, seq, offset, ranges, positions)
+    rotary.rotated(shape[2])
+    if not _native_ok(read):
+        return _plain_rope(qkv.reshape(shape), nheads, where).reshape(qkv.shape)
+    if t is None or _overlaps(t) or (t.stride(2) != 1 and shape[2] > 1):
+        raise ValueError("a tensor that is turned in place must have its heads' components next to one another in memory "
+                         "of their own: use ops.rope")
+    return _RopeInPlaceFn.apply(qkv, shape, nheads, *where)
+
+
+# ------------------------------------------------------------------------------- norm of the heads and rotation
+def _weight_ok(w, qkv):
+    return w is None or (w.dtype in (qkv.dtype, torch.float32) and w.device == qkv.device)
+
+
+def _plain_qk_norm_rope(qkv, hq, hkv, wq, wk, eps, where):
+    nh = hq + hkv
+    x = _wide(qkv[:, :nh])
+    u = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps)
+    parts = [u[:, :hq] if wq is None else u[:, :hq] * wq.to(x.dtype), u[:, hq:] if wk is None else u[:, hq:] * wk.to(x.dtype)]
+    y = torch.cat(parts, dim=1)
+    rotary, positions, seq, offset = where
+    if rotary is not None:
+        cos, sin = _angles(qkv, rotary, positions, seq, offset)
+        y = _rotated(y, cos, sin, rotary.rotated(qkv.shape[2]), rotary.interleaved)
+    return torch.cat([y.to(qkv.dtype), qkv[:, nh:]], dim=1)
+
+
+def _norm_forward(src, dst, hq, hkv, wq, wk, eps, where):
+    tokens, heads, hd = src.shape
+    (dim, near, address, scale), place = _turn_args(where, hd)
+    wide = (wq if wq is not None else wk) is not None and (wq if wq is not None else wk).dtype == torch.float32
+    call_on(src, "dd_norm_heads_fwd", *_heads(src), *_heads(dst), ptr(wq), ptr(wk), int(wide), eps, tokens, hq, hkv,
+            heads - hq - hkv, hd, dim, near, address, scale, *place, _DTYPE[src.dtype])
+
+
+class _QKNormRopeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, wq, wk, hq, hkv, eps, rotary, positions, seq, offset):
+        src = _unit(qkv)
+        out = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        _norm_forward(src, out, hq, hkv, wq, wk, eps, (rotary, positions, seq, offset))
+        ctx.save_for_backward(src, wq, wk, positions)
+        ctx.refs = (wq, wk)
+        ctx.cfg = (hq, hkv, eps, rotary, seq, offset)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, wq, wk, positions = ctx.saved_tensors
+        hq, hkv, eps, rotary, seq, offset = ctx.cfg
+        tokens, heads, hd = x.shape
+        dy = _unit(dy)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        want = [w is not None and ctx.needs_input_grad[k] for k, w in ((1, wq), (2, wk))]
+        wide = next((w.dtype == torch.float32 for w in (wq, wk) if w is not None), False)
+        dw, accumulate = [None, None], False
+        partial = None
+        if any(want):
+            # gathered weights collect their gradient in fp32 beside them
+            main = [main_grad_now(getattr(r, "main_grad", None), getattr(r, "main_grad_owner", None), ctx, k) if wanted
+                    else None for k, r, wanted in ((1, ctx.refs[0], want[0]), (2, ctx.refs[1], want[1]))]
+            accumulate = all(m is not None for m, wanted in zip(main, want) if wanted)
+            dw = main if accumulate else [torch.empty(hd, dtype=w.dtype, device=x.device) if wanted else None
+                                          for w, wanted in zip((wq, wk), want)]
+            with torch.cuda.device(x.device):
+                parts = _native.lib().dd_heads_parts()
+            partial = torch.empty(parts * 2 * hd, dtype=torch.float32, device=x.device)
+        (dim, near, address, scale), place = _turn_args((rotary, positions, seq, offset), hd)
+        call_on(x, "dd_norm_heads_bwd", *_heads(x), *_heads(dy), *_heads(dx), ptr(wq), ptr(wk), int(wide), eps, ptr(dw[0]),
+                ptr(dw[1]), int(accumulate), ptr(partial), tokens, hq, hkv, heads - hq - hkv, hd, dim, near, address, scale,
+                *place, _DTYPE[x.dtype])
+        if accumulate:
+            dw = [None, None]
+        return dx, dw[0], dw[1], None, None, None, None, None, None, None
+
+
+def _norm_args(qkv, hq, hkv, wq, wk, rotary, seq, offset, ranges, positions):
+    _check_heads(qkv, hq + hkv)
+    if hq < 0 or hkv < 0:
+        raise ValueError(f"numbers of heads are not negative: {hq}, {hkv}")
+    for w in (wq, wk):
+        if w is not None and (w.numel() != qkv.shape[2] or not w.is_floating_point()):
+            raise ValueError(f"a weight of the norm has one value per component ({qkv.shape[2]}), not {tuple(w.shape)}")
+    where = _where(qkv, rotary, seq, offset, ranges, positions)
+    if rotary is not None:
+        rotary.rotated(qkv.shape[2])
+    native = (_native_ok(qkv) and _weight_ok(wq, qkv) and _weight_ok(wk, qkv)
+              and (wq is None or wk is None or wq.dtype == wk.dtype))
+    # (a weight that is a row already stays the tensor that it is: its accumulator is an attribute of it)
+    flat = [w if w is None or (w.dim() == 1 and w.is_contiguous()) else w.reshape(-1).contiguous() for w in (wq, wk)]
+    return where, native, flat
+
+
+def qk_norm_rope(qkv: torch.Tensor, seq: int, hq: int, hkv: int, q_weight=None, k_weight=None, *, rotary: Rotary = None,
+                 offset: int = 0, ranges=None, positions=None, eps: float = 1e-6) -> torch.Tensor:
+    """The RMS norm of every query and key head, and the rotation by their positions in the same pass: the first ``hq`` heads
+    of ``qkv [tokens, heads, head_dim]`` become ``R(u * q_weight)``, ``u = x / sqrt(mean x^2 + eps)`` over a head, the next
+    ``hkv`` the same with ``k_weight``; the heads behind (the values) are copied.  Weights ``[head_dim]`` of ``qkv``'s type or
+    in fp32, or None; ``rotary`` None: the norm alone.  Positions as for :func:`rope`.
+
+    The result is a new tensor and the backward pass reads ``qkv`` again, so that it stays as it is;
+    :func:`qk_norm_rope_` works in place where no gradient is wanted."""
+    where, native, (wq, wk) = _norm_args(qkv, hq, hkv, q_weight, k_weight, rotary, seq, offset, ranges, positions)
+    if native:
+        return _QKNormRopeFn.apply(qkv, wq, wk, hq, hkv, float(eps), *where)
+    return _plain_qk_norm_rope(qkv, hq, hkv, wq, wk, eps, where)
+
+
+def qk_norm_rope_(qkv: torch.Tensor, seq: int, hq: int, hkv: int, q_weight=None, k_weight=None, *, rotary: Rotary = None,
+                  offset: int = 0, ranges=None, positions=None, eps: float = 1e-6) -> torch.Tensor:
+    """:func:`qk_norm_rope` in place, for inference: refused where a gradient would be wanted."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (qkv, q_weight, k_weight)):
+        raise RuntimeError("qk_norm_rope_ overwrites what its gradient would need: use qk_norm_rope, or torch.no_grad()")
+    where, native, (wq, wk) = _norm_args(qkv, hq, hkv, q_weight, k_weight, rotary, seq, offset, ranges, positions)
+    if _overlaps(qkv):
+        raise ValueError("a tensor that is changed in place must not overlap itself: use ops.qk_norm_rope")
+    if native and (qkv.stride(2) == 1 or qkv.shape[2] == 1):
+        with torch.no_grad():
+            _norm_forward(qkv, qkv, hq, hkv, wq, wk, float(eps), where)
+        if not qkv.is_inference():
+            torch.autograd.graph.increment_version(qkv)
+        return qkv
+    with torch.no_grad():
+        qkv.copy_(_plain_qk_norm_rope(qkv, hq, hkv, wq, wk, eps, where))
+    return qkv
