@@ -13,12 +13,14 @@
 //    every position below 2^31, where 32 bits are off by radians), then sin and cos in 32 bits, once per lane for all heads of
 //    a chunk.  The frequencies travel as arguments of the kernel: no table, no copy, nothing to capture or to keep;
 //  * the backward pass recomputes r from x, which it needs anyway.
-// A unit of work is a token's chunk of up to kChunkHeads heads of one kind (query / key / rest); units are dealt to the
-// groups of a grid of two CTAs per SM, kind by kind, so that the lanes of a warp nearly always do the same.
+// A unit of work is a token's chunk of heads of one kind (query / key / rest); units are dealt to the groups of a grid of two
+// CTAs per SM, kind by kind, so that the lanes of a warp do the same and what belongs to a kind is held once.
 #include "common.cuh"
 #include "runtime.cuh"
 
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 using namespace dd;
 
@@ -26,14 +28,13 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 256;        // heads of up to 512 components
-constexpr int kCtasPerSm = 2;
+constexpr int kCtasPerSm = 2;         // (128 registers a thread: heads side by side count for more than further warps)
 
-enum Kind { kRope = 0, kNormFwd = 1, kNormBwd = 2 };
-// How a lane finds the other component of a pair.
+enum Kind { kRope = 0, kNorm = 1 };
+// Where a lane finds the two components of a pair.
 enum Pairing {
-  kApart = 0,     // halves, rd / 2 whole vectors: in the lane's other vector
-  kInside = 1,    // neighbours: in the same vector
-  kShared = 2,    // halves at any distance, and single components: through shared memory
+  kApart = 0,     // halves that are whole vectors: at the same place of its two vectors
+  kInside = 1,    // next to one another in a vector; with single components, any pair of components that it holds
 };
 
 struct HeadArgs {
@@ -53,7 +54,7 @@ struct HeadArgs {
   int chunk[3], chunks[3];    // heads per unit, units per token
   int hd, rd, group;          // group: lanes per head (a power of two)
   int wide_positions, wide_weights, neighbours;
-  float magnitude, sign, eps;
+  float magnitude, sign, eps, inv_hd;
   double turns[kMaxPairs];    // frequency of each pair in turns per position
 };
 
@@ -83,259 +84,487 @@ __device__ __forceinline__ void clear(Pack<T, VE>& r) {
   if constexpr (VE == 1) r.v = from_f<T>(0.f);
   else r.v = make_uint4(0u, 0u, 0u, 0u);
 }
-__device__ __forceinline__ float2 two(uint32_t u, __nv_bfloat16) {
-  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+__device__ __forceinline__ uint64_t two(uint32_t u, __nv_bfloat16) { return pack_u32x2(u << 16, u & 0xffff0000u); }
+__device__ __forceinline__ uint64_t two(uint32_t u, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+  return pack_f32x2(f.x, f.y);
 }
-__device__ __forceinline__ float2 two(uint32_t u, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
-__device__ __forceinline__ uint32_t word(float a, float b, __nv_bfloat16) { return pack_bf16x2(a, b); }
-__device__ __forceinline__ uint32_t word(float a, float b, __half) {
-  const __half2 v = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&v);
+__device__ __forceinline__ uint32_t word(uint64_t v, __nv_bfloat16) {
+  const float2 f = unpack_f32x2(v);
+  return pack_bf16x2(f.x, f.y);
 }
-template <typename T, int VE>
-__device__ __forceinline__ void unpack(const Pack<T, VE>& r, float* f) {
+__device__ __forceinline__ uint32_t word(uint64_t v, __half) {
+  const float2 f = unpack_f32x2(v);
+  const __half2 h = __floats2half2_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// NV packs as pairs of fp32 values, one instruction for both (single components pair up as they come).
+template <typename T, int VE, int NV>
+__device__ __forceinline__ void unpack(const Pack<T, VE> (&r)[NV], uint64_t (&f)[NV * VE / 2]) {
   if constexpr (VE == 1) {
-    f[0] = to_f(r.v);
-  } else if constexpr (VE == 4) {
-    f[0] = __uint_as_float(r.v.x); f[1] = __uint_as_float(r.v.y); f[2] = __uint_as_float(r.v.z); f[3] = __uint_as_float(r.v.w);
+#pragma unroll
+    for (int i = 0; i < NV / 2; ++i) f[i] = pack_f32x2(to_f(r[2 * i].v), to_f(r[2 * i + 1].v));
   } else {
-    const float2 a = two(r.v.x, T()), b = two(r.v.y, T()), c = two(r.v.z, T()), d = two(r.v.w, T());
-    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
+#pragma unroll
+    for (int s = 0; s < NV; ++s) {
+      uint64_t* g = f + s * VE / 2;
+      if constexpr (VE == 4) {
+        g[0] = pack_u32x2(r[s].v.x, r[s].v.y); g[1] = pack_u32x2(r[s].v.z, r[s].v.w);
+      } else {
+        g[0] = two(r[s].v.x, T()); g[1] = two(r[s].v.y, T()); g[2] = two(r[s].v.z, T()); g[3] = two(r[s].v.w, T());
+      }
+    }
+  }
+}
+template <typename T, int VE, int NV>
+__device__ __forceinline__ void pack(const uint64_t (&f)[NV * VE / 2], Pack<T, VE> (&r)[NV]) {
+  if constexpr (VE == 1) {
+#pragma unroll
+    for (int i = 0; i < NV / 2; ++i) {
+      const float2 g = unpack_f32x2(f[i]);
+      r[2 * i].v = from_f<T>(g.x); r[2 * i + 1].v = from_f<T>(g.y);
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < NV; ++s) {
+      const uint64_t* g = f + s * VE / 2;
+      if constexpr (VE == 4) {
+        const float2 a = unpack_f32x2(g[0]), b = unpack_f32x2(g[1]);
+        r[s].v = make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+      } else {
+        r[s].v = make_uint4(word(g[0], T()), word(g[1], T()), word(g[2], T()), word(g[3], T()));
+      }
+    }
   }
 }
 template <typename T, int VE>
-__device__ __forceinline__ void store_pack(T* p, const float* f) {
-  if constexpr (VE == 1) *p = from_f<T>(f[0]);
-  else if constexpr (VE == 4) *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-  else *reinterpret_cast<uint4*>(p) = make_uint4(word(f[0], f[1], T()), word(f[2], f[3], T()), word(f[4], f[5], T()),
-                                                 word(f[6], f[7], T()));
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, VE>& r) {
+  if constexpr (VE == 1) *p = r.v;
+  else *reinterpret_cast<uint4*>(p) = r.v;
 }
 
+// Sine and cosine of 2 pi t, |t| <= 1/2.  For 16-bit heads the fast functions: 2^-21 off at most, a hundredth of a rounding
+// step of the result, and the accurate ones are a fifth of the instructions of a pass.
+template <typename T>
+__device__ __forceinline__ void sin_cos_turns(float t, float* s, float* c) {
+  if constexpr (sizeof(T) == 2) {
+    *s = __sinf(6.283185307179586f * t);
+    *c = __cosf(6.283185307179586f * t);
+  } else {
+    sincospif(2.f * t, s, c);
+  }
+}
+
+// Sums over the lanes of a group (a power of two, the same for all of the kernel), two side by side.
+__device__ __forceinline__ void group_sums(float& v, float& u, int group) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (group > o) {
+      v += __shfl_xor_sync(0xffffffffu, v, o);
+      u += __shfl_xor_sync(0xffffffffu, u, o);
+    }
+}
 __device__ __forceinline__ float group_sum(float v, int group) {
-  for (int o = group >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (group > o) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// NV vectors of VE components per lane and head.
-template <typename T, int VE, int NV, int PAIRING, int KIND>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_kernel(const __grid_constant__ HeadArgs a) {
-  constexpr int N = NV * VE;                                  // components per lane
-  constexpr int ANGLES = PAIRING == kShared ? N : N / 2;      // pairs per lane (kShared: of every component its pair's)
-  constexpr int U = VE == 1 ? 1 : KIND == kNormBwd ? 2 : 4;   // heads whose loads are in flight together
-  extern __shared__ float smem[];                             // kShared: a head per group; later dw sums
-  grid_dependency_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane & (a.group - 1), per_warp = 32 / a.group, in_warp = lane / a.group;
-  const int vectors = a.hd / VE, half = a.rd >> 1;
-  float* exchange = smem + (size_t)(warp * per_warp + in_warp) * a.hd;
+// What a lane of a group holds of a head: NV vectors of VE components; FULL: every lane has all of them.
+template <typename T, int VE, int NV, int PAIRING, bool FULL>
+struct Lane {
+  static constexpr int N = NV * VE, M = N / 2;                // components, pairs of them as they are computed with
+  int at[NV];                                                 // first component of each vector, -1: none
+  int half;                                                   // pairs of a head
+  int first_pair, paired;                                     // kApart: of this lane's components, and whether they turn
 
-  // this lane's vectors of a head, and the pair of each of its components (-1: stays)
-  int at[NV];
+  __device__ __forceinline__ Lane(const HeadArgs& a, int g) : half(a.rd >> 1) {
+    paired = g < half / VE;
+    first_pair = g * VE;
 #pragma unroll
-  for (int s = 0; s < NV; ++s) {
-    if constexpr (PAIRING == kApart) {
-      const int paired = half / VE;                           // lanes that hold a vector of each half
-      at[s] = (g < paired ? g + s * paired : 2 * paired + 2 * (g - paired) + s) * VE;
-    } else {
-      at[s] = (s * a.group + g) * VE;
+    for (int s = 0; s < NV; ++s) {
+      if constexpr (PAIRING == kApart) {
+        const int lanes = half / VE;                          // that hold a vector of each half; the others, what stays
+        at[s] = (paired ? g + s * lanes : 2 * lanes + 2 * (g - lanes) + s) * VE;
+      } else if constexpr (VE > 1) {
+        at[s] = (s * a.group + g) * VE;
+      } else {
+        const int pair = (s / 2) * a.group + g;
+        at[s] = pair >= half ? 2 * pair + s % 2 : a.neighbours ? 2 * pair + s % 2 : pair + s % 2 * half;
+      }
+      if (!FULL && at[s] + VE > a.hd) at[s] = -1;
     }
-    if (at[s] >= vectors * VE) at[s] = -1;
   }
-  auto pair_of = [&](int i) -> int {                          // i-th angle of this lane
-    if constexpr (PAIRING == kApart) {
-      return g < half / VE ? at[0] + i : -1;
-    } else if constexpr (PAIRING == kInside) {
-      const int c = at[2 * i / VE];
-      return c < 0 || c + 2 * i % VE >= a.rd ? -1 : (c + 2 * i % VE) >> 1;
+  __device__ __forceinline__ bool has(int s) const { return FULL || at[s] >= 0; }
+  __device__ __forceinline__ int component(int i) const { return has(i / VE) ? at[i / VE] + i % VE : -1; }
+  // kInside: the pair of components (2 i, 2 i + 1) of this lane, -1 where they stay
+  __device__ __forceinline__ int pair(const HeadArgs& a, int g, int i) const {
+    if constexpr (VE > 1) {
+      const int c = component(2 * i);
+      return c >= 0 && c < a.rd ? c >> 1 : -1;
     } else {
-      const int c = at[i / VE] < 0 ? a.rd : at[i / VE] + i % VE;
-      return c >= a.rd ? -1 : a.neighbours ? c >> 1 : c < half ? c : c - half;
+      const int p = i * a.group + g;
+      return p < half ? p : -1;
     }
-  };
+  }
+};
 
+// Sine and cosine of a lane's pairs at a token's position, and the rotation of what it holds of a head by them.
+template <typename T, int VE, int NV, int PAIRING, bool FULL>
+struct Angles {
+  using L = Lane<T, VE, NV, PAIRING, FULL>;
+  static constexpr int M = L::M, A = PAIRING == kApart ? M / 2 : 1, I = PAIRING == kInside ? M : 1;
+  uint64_t c2[A], s2[A], n2[A];                               // kApart: of two pairs; n2: the sines negated
+  float c1[I], s1[I];                                         // kInside
+
+  __device__ __forceinline__ void set(const HeadArgs& a, const double* turns, const L& lane, int g, unsigned token) {
+    long long pos;
+    if (a.positions == nullptr) pos = a.offset + token % a.seq;
+    else if (a.wide_positions) pos = reinterpret_cast<const long long*>(a.positions)[token % a.seq];
+    else pos = reinterpret_cast<const int*>(a.positions)[token % a.seq];
+    const double place = (double)pos;
+    auto angle = [&](int pair, float* c, float* s) {
+      double t = place * turns[pair];
+      t -= rint(t);
+      sin_cos_turns<T>((float)t, s, c);
+      *c *= a.magnitude;
+      *s *= a.magnitude * a.sign;
+    };
+    if constexpr (PAIRING == kApart) {
+#pragma unroll
+      for (int i = 0; i < A; ++i) {
+        float c[2] = {1.f, 1.f}, s[2] = {0.f, 0.f};
+        if (lane.paired) {
+          angle(lane.first_pair + 2 * i, &c[0], &s[0]);
+          angle(lane.first_pair + 2 * i + 1, &c[1], &s[1]);
+        }
+        c2[i] = pack_f32x2(c[0], c[1]);
+        s2[i] = pack_f32x2(s[0], s[1]);
+        n2[i] = pack_f32x2(-s[0], -s[1]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        const int p = lane.pair(a, g, i);
+        if (p >= 0) angle(p, &c1[i], &s1[i]);
+      }
+    }
+  }
+  __device__ __forceinline__ void rotate(const HeadArgs& a, const L& lane, int g, uint64_t (&v)[M]) const {
+    if constexpr (PAIRING == kApart) {
+      if (lane.paired) {
+#pragma unroll
+        for (int i = 0; i < A; ++i) {
+          const uint64_t p = v[i], q = v[A + i];
+          v[i] = fma_f32x2(p, c2[i], mul_f32x2(q, n2[i]));
+          v[A + i] = fma_f32x2(q, c2[i], mul_f32x2(p, s2[i]));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        if (lane.pair(a, g, i) >= 0) {
+          const float2 p = unpack_f32x2(v[i]);
+          v[i] = pack_f32x2(p.x * c1[i] - p.y * s1[i], p.y * c1[i] + p.x * s1[i]);
+        }
+      }
+    }
+  }
+};
+
+template <int M>
+__device__ __forceinline__ float dot(const uint64_t (&v)[M], const uint64_t (&u)[M]) {
+  uint64_t sum[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < M; ++i) sum[i & 1] = fma_f32x2(v[i], u[i], sum[i & 1]);
+  const float2 f = unpack_f32x2(add_f32x2(sum[0], sum[1]));
+  return f.x + f.y;
+}
+
+template <typename T>
+__device__ __forceinline__ float weight_of(const HeadArgs& a, int kind, int c) {
+  const void* w = kind == 0 ? a.wq : a.wk;
+  if (w == nullptr || c < 0) return 1.f;
+  return a.wide_weights ? reinterpret_cast<const float*>(w)[c] : to_f(reinterpret_cast<const T*>(w)[c]);
+}
+
+// A unit of work: heads [first, first + count) of a token, of one kind.
+struct Unit {
+  unsigned token;
+  int head, count;
+  __device__ __forceinline__ Unit(const HeadArgs& a, int kind, unsigned unit, bool live) {
+    token = live ? unit / (unsigned)a.chunks[kind] : 0u;
+    const int first = live ? (int)(unit - token * (unsigned)a.chunks[kind]) * a.chunk[kind] : 0;
+    count = live ? min(a.chunk[kind], a.heads[kind] - first) : 0;
+    head = first + (kind > 0 ? a.heads[0] : 0) + (kind > 1 ? a.heads[1] : 0);
+  }
+};
+
+// The heads behind queries and keys, copied (forward: of x, backward: of dy).
+template <typename T, int VE, int NV, typename L>
+__device__ __forceinline__ void copy_rest(const HeadArgs& a, const L& lane, const void* from, long long row, long long head,
+                                          unsigned unit, unsigned stride) {
+  const unsigned units = a.tokens * (unsigned)a.chunks[2];
+  for (; unit < units; unit += stride) {
+    const Unit u(a, 2, unit, true);
+    const T* src = reinterpret_cast<const T*>(from) + (long long)u.token * row + u.head * head;
+    T* out = reinterpret_cast<T*>(a.out) + (long long)u.token * a.out_row + u.head * a.out_head;
+    constexpr int R = NV <= 4 ? 4 : 1;
+    for (int h = 0; h < u.count; h += R) {
+      Pack<T, VE> r[R][NV];
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+#pragma unroll
+        for (int s = 0; s < NV; ++s)
+          if (h + k < u.count && lane.has(s)) r[k][s] = load_pack<T, VE>(src + (h + k) * head + lane.at[s]);
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+#pragma unroll
+        for (int s = 0; s < NV; ++s)
+          if (h + k < u.count && lane.has(s)) store_pack<T, VE>(out + (h + k) * a.out_head + lane.at[s], r[k][s]);
+    }
+  }
+}
+
+// Forward.  Four heads' loads are in flight together and four heads are worked on side by side: that hides more than a
+// third or fourth CTA per SM or loads a step ahead would (16384 tokens, 48 heads of 128 bf16, us, rotation / norm and rotation:
+// two heads and 4 / 3 CTAs 80.7 / 87.4, two and the next two on their way 75.5 / 72.3, four 64.7 / 67.6).
+template <typename T, int VE, int NV, int PAIRING, int KIND, bool FULL>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_fwd_kernel(const __grid_constant__ HeadArgs a) {
+  using L = Lane<T, VE, NV, PAIRING, FULL>;
+  constexpr int M = L::M, U = NV <= 4 ? 4 : 1;
+  __shared__ double turns[kMaxPairs];
+  grid_dependency_launch();
+  for (int i = threadIdx.x; i < a.rd / 2; i += kThreads) turns[i] = a.turns[i];
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, g = threadIdx.x & (a.group - 1);
+  const int per_warp = 32 / a.group, in_warp = (threadIdx.x & 31) / a.group;
+  const L lane(a, g);
   const unsigned stride = gridDim.x * (kThreads / 32) * per_warp;
   unsigned unit0 = (blockIdx.x * (kThreads / 32) + warp) * per_warp;      // of the kind at hand
-  // Kind by kind, so that a warp's heads are all of one kind and what belongs to the kind (weights, sums) is held once.
 #pragma unroll 1
-  for (int kind = 0; kind < 3; ++kind) {
-  const bool turns = kind < 2;
-  const unsigned units = a.tokens * (unsigned)a.chunks[kind];
-  float w[KIND == kRope ? 1 : N];
-  if constexpr (KIND != kRope) {
-    const void* ws = kind == 0 ? a.wq : kind == 1 ? a.wk : nullptr;
+  for (int kind = 0; kind < 2; ++kind) {
+    const unsigned units = a.tokens * (unsigned)a.chunks[kind];
+    uint64_t w[KIND == kNorm ? M : 1];
+    if (KIND == kNorm && unit0 < units) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = at[i / VE] < 0 ? -1 : at[i / VE] + i % VE;
-      w[i] = 1.f;
-      if (ws != nullptr && c >= 0)
-        w[i] = a.wide_weights ? reinterpret_cast<const float*>(ws)[c] : to_f(reinterpret_cast<const T*>(ws)[c]);
+      for (int i = 0; i < M; ++i)
+        w[i] = pack_f32x2(weight_of<T>(a, kind, lane.component(2 * i)), weight_of<T>(a, kind, lane.component(2 * i + 1)));
     }
-  }
-  float sums[KIND == kNormBwd ? N : 1] = {};
-  for (; unit0 < units; unit0 += stride) {
-    // (every lane of the warp takes part in every step: a group without a unit works on none of its heads)
-    const unsigned unit = unit0 + in_warp;
-    const bool live = unit < units;
-    const unsigned token = live ? unit / (unsigned)a.chunks[kind] : 0u;
-    const int first = live ? (int)(unit - token * (unsigned)a.chunks[kind]) * a.chunk[kind] : 0;
-    const int count = live ? min(a.chunk[kind], a.heads[kind] - first) : 0;
-    const int head0 = first + (kind > 0 ? a.heads[0] : 0) + (kind > 1 ? a.heads[1] : 0);
-    const int most = __reduce_max_sync(0xffffffffu, count);
-
-    const T* x = reinterpret_cast<const T*>(a.x) + (long long)token * a.x_row + head0 * a.x_head;
-    const T* dy = KIND == kNormBwd ? reinterpret_cast<const T*>(a.dy) + (long long)token * a.dy_row + head0 * a.dy_head
-                                   : nullptr;
-    T* out = reinterpret_cast<T*>(a.out) + (long long)token * a.out_row + head0 * a.out_head;
-
-    // the first heads' data, before the angles are worked out
-    Pack<T, VE> rx[U][NV], rd_[KIND == kNormBwd ? U : 1][NV];
-    auto fetch = [&](int h) {
+    for (; unit0 < units; unit0 += stride) {
+      // (every lane of the warp takes part in every step: a group without a unit works on none of its heads)
+      const Unit u(a, kind, unit0 + in_warp, unit0 + in_warp < units);
+      const int most = __reduce_max_sync(0xffffffffu, u.count);
+      const T* x = reinterpret_cast<const T*>(a.x) + (long long)u.token * a.x_row + u.head * a.x_head;
+      T* out = reinterpret_cast<T*>(a.out) + (long long)u.token * a.out_row + u.head * a.out_head;
+      Pack<T, VE> raw[U][NV];
+      auto fetch = [&](int h, auto heads) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int s = 0; s < NV; ++s) {
-          if (h + u < count && at[s] >= 0) {
-            if (KIND != kNormBwd || turns) rx[u][s] = load_pack<T, VE>(x + (h + u) * a.x_head + at[s]);
-            if constexpr (KIND == kNormBwd) rd_[u][s] = load_pack<T, VE>(dy + (h + u) * a.dy_head + at[s]);
-          } else {
-            clear(rx[u][s]);
-            if constexpr (KIND == kNormBwd) clear(rd_[u][s]);
-          }
-        }
-    };
-    fetch(0);
-
-    float co[ANGLES], si[ANGLES];
-    if (turns) {
-      long long pos;
-      if (a.positions == nullptr) pos = a.offset + token % a.seq;
-      else if (a.wide_positions) pos = reinterpret_cast<const long long*>(a.positions)[token % a.seq];
-      else pos = reinterpret_cast<const int*>(a.positions)[token % a.seq];
-      const double place = (double)pos;
-#pragma unroll
-      for (int i = 0; i < ANGLES; ++i) {
-        const int pair = pair_of(i);
-        if (pair >= 0) {
-          double t = place * a.turns[pair];
-          t -= rint(t);
-          sincospif(2.f * (float)t, &si[i], &co[i]);
-          co[i] *= a.magnitude;
-          si[i] *= a.magnitude * a.sign;
-        }
-      }
-    }
-    // the rotation of this lane's components of a head
-    auto rotate = [&](float (&v)[N]) {
-      if constexpr (PAIRING == kApart) {
-        if (turns && g < half / VE) {
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const float p = v[e], q = v[VE + e];
-            v[e] = p * co[e] - q * si[e];
-            v[VE + e] = q * co[e] + p * si[e];
-          }
-        }
-      } else if constexpr (PAIRING == kInside) {
-#pragma unroll
-        for (int i = 0; i < ANGLES; ++i) {
-          if (turns && pair_of(i) >= 0) {
-            const float p = v[2 * i], q = v[2 * i + 1];
-            v[2 * i] = p * co[i] - q * si[i];
-            v[2 * i + 1] = q * co[i] + p * si[i];
-          }
-        }
-      } else {
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (at[i / VE] >= 0) exchange[at[i / VE] + i % VE] = v[i];
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int c = at[i / VE] < 0 ? a.rd : at[i / VE] + i % VE;
-          if (turns && c < a.rd) {
-            const bool second = a.neighbours ? c & 1 : c >= half;
-            const int other = a.neighbours ? c ^ 1 : second ? c - half : c + half;
-            const float q = exchange[other];
-            v[i] = second ? v[i] * co[i] + q * si[i] : v[i] * co[i] - q * si[i];
-          }
-        }
-      }
-    };
-
-    for (int h = 0; h < most; h += U) {
-      if (h > 0) fetch(h);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float v[N];
-#pragma unroll
-        for (int s = 0; s < NV; ++s) unpack(rx[u][s], v + s * VE);
-        if constexpr (KIND == kRope) {
-          rotate(v);
-        } else if constexpr (KIND == kNormFwd) {
-          float q = 0.f;
-#pragma unroll
-          for (int i = 0; i < N; ++i) q += v[i] * v[i];
-          const float r = rsqrtf(group_sum(q, a.group) / (float)a.hd + a.eps);
-          if (turns) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] *= r * w[i];
-          }
-          rotate(v);
-        } else {
-          float d[N];
-#pragma unroll
-          for (int s = 0; s < NV; ++s) unpack(rd_[u][s], d + s * VE);
-          rotate(d);                                          // (a.sign: backwards)
-          float q = 0.f, dot = 0.f;
-#pragma unroll
-          for (int i = 0; i < N; ++i) { q += v[i] * v[i]; dot += d[i] * w[i] * v[i]; }
-          q = group_sum(q, a.group);
-          dot = group_sum(dot, a.group);
-          const float r = rsqrtf(q / (float)a.hd + a.eps);
-          const float mean = dot * r / (float)a.hd;           // of g w u
-          if (turns) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-              const float unit_x = v[i] * r;
-              if (h + u < count) sums[i] += d[i] * unit_x;
-              v[i] = r * (d[i] * w[i] - unit_x * mean);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = d[i];
-          }
-        }
-        if (h + u < count) {
+        for (int k = 0; k < heads(); ++k) {
 #pragma unroll
           for (int s = 0; s < NV; ++s) {
-            if (at[s] >= 0) store_pack<T, VE>(out + (h + u) * a.out_head + at[s], v + s * VE);
+            if (h + k < u.count && lane.has(s)) raw[k][s] = load_pack<T, VE>(x + lane.at[s]);
+            else clear(raw[k][s]);
           }
+          x += a.x_head;
         }
+      };
+      Angles<T, VE, NV, PAIRING, FULL> angles;
+      auto work = [&](int h, auto heads) {
+#pragma unroll
+        for (int k = 0; k < heads(); ++k) {
+          uint64_t v[M];
+          unpack<T, VE, NV>(raw[k], v);
+          if constexpr (KIND == kNorm) {
+            const float r = rsqrtf(group_sum(dot(v, v), a.group) * a.inv_hd + a.eps);
+            const uint64_t r2 = pack_f32x2(r, r);
+#pragma unroll
+            for (int i = 0; i < M; ++i) v[i] = mul_f32x2(v[i], mul_f32x2(r2, w[i]));
+          }
+          angles.rotate(a, lane, g, v);
+          if (h + k < u.count) {
+            Pack<T, VE> res[NV];
+            pack<T, VE, NV>(v, res);
+#pragma unroll
+            for (int s = 0; s < NV; ++s)
+              if (lane.has(s)) store_pack<T, VE>(out + lane.at[s], res[s]);
+          }
+          out += a.out_head;
+        }
+      };
+      // U heads at a time, the last ones of a unit (few tokens: its only one) singly
+      const std::integral_constant<int, U> many;
+      const std::integral_constant<int, 1> one;
+      int h = 0;
+      if (most >= U) fetch(0, many);
+      else fetch(0, one);
+      angles.set(a, turns, lane, g, u.token);                 // while the first heads are on their way
+      for (; h + U <= most; h += U) {
+        if (h > 0) fetch(h, many);
+        work(h, many);
+      }
+      for (; h < most; ++h) {
+        if (h > 0) fetch(h, one);
+        work(h, one);
       }
     }
+    // the deal goes on where the last kind's ended (its units padded to whole warps, so that every group keeps its place)
+    unit0 -= (units + per_warp - 1) / per_warp * per_warp;
   }
-  // the deal goes on where the last kind's ended (its units padded to whole warps, so that every group keeps its place)
-  unit0 -= (units + per_warp - 1) / per_warp * per_warp;
-  if constexpr (KIND == kNormBwd) {
-    if (a.partial == nullptr || !turns) continue;
-    // the lanes that hold the same components: over the warp by shuffles, over the warps in their order
+  copy_rest<T, VE, NV>(a, lane, a.x, a.x_row, a.x_head, unit0 + in_warp, stride);
+}
+
+// 16 bytes global -> shared by a copy of this thread's own (zeros where it is not to read).
+__device__ __forceinline__ void copy_async(void* to, const void* from, bool read) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(read ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+constexpr int kBwdSteps = 4;                                  // heads in the ring
+constexpr int kBwdRing = kBwdSteps * 4 * 16 * kThreads;
+
+// Backward.  x and dy come through a ring in shared memory that every thread fills and reads for itself, three heads ahead
+// and across the units' ends, and w stays there: the registers are needed for the sums of dw and a head's values (16384
+// tokens, 48 heads of 128 bf16, us: loads into registers a head ahead 138, with w in shared memory 128, the ring 109, with two
+// heads side by side, which spill, 149).
+template <typename T, int VE, int NV, int PAIRING, bool FULL>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const __grid_constant__ HeadArgs a) {
+  using L = Lane<T, VE, NV, PAIRING, FULL>;
+  constexpr int N = L::N, M = L::M;
+  constexpr bool RING = VE > 1;
+  constexpr int R = RING ? kBwdSteps : 1;
+  extern __shared__ __align__(16) uint8_t ring[];             // [R][2 NV][kThreads] vectors
+  __shared__ double turns[kMaxPairs];
+  __shared__ __align__(16) float weights[2 * kMaxPairs];
+  __shared__ float reduced[kThreads / 32][2 * kMaxPairs];
+  grid_dependency_launch();
+  for (int i = threadIdx.x; i < a.rd / 2; i += kThreads) turns[i] = a.turns[i];
+  const int warp = threadIdx.x >> 5, g = threadIdx.x & (a.group - 1);
+  const int per_warp = 32 / a.group, in_warp = (threadIdx.x & 31) / a.group;
+  const L lane(a, g);
+  const unsigned stride = gridDim.x * (kThreads / 32) * per_warp;
+  unsigned unit0 = (blockIdx.x * (kThreads / 32) + warp) * per_warp;      // of the kind at hand
+#pragma unroll 1
+  for (int kind = 0; kind < 2; ++kind) {
+    const unsigned units = a.tokens * (unsigned)a.chunks[kind];
+    const int chunk = a.chunk[kind];
+    for (int c = threadIdx.x; c < a.hd; c += kThreads) weights[c] = weight_of<T>(a, kind, c);
     __syncthreads();
+    uint64_t sums[M] = {};
+
+    Pack<T, VE> rx[NV], rd[NV];
+    // the copies' place in the units, ahead of the work's
+    unsigned ahead = unit0;
+    int ahead_h = 0, ahead_count = 0;
+    const T* x = nullptr;
+    const T* dy = nullptr;
+    auto fetch = [&](int slot) {
+      if (ahead < units) {
+        if (ahead_h == 0) {
+          const Unit u(a, kind, ahead + in_warp, ahead + in_warp < units);
+          ahead_count = u.count;
+          x = reinterpret_cast<const T*>(a.x) + (long long)u.token * a.x_row + u.head * a.x_head;
+          dy = reinterpret_cast<const T*>(a.dy) + (long long)u.token * a.dy_row + u.head * a.dy_head;
+        }
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float v = sums[i];
-      for (int o = a.group; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (in_warp == 0 && at[i / VE] >= 0) smem[warp * a.hd + at[i / VE] + i % VE] = v;
+        for (int s = 0; s < NV; ++s) {
+          const bool read = ahead_h < ahead_count && lane.has(s);
+          if constexpr (RING) {
+            uint8_t* to = ring + ((slot * 2 * NV + s) * kThreads + threadIdx.x) * 16;
+            copy_async(to, read ? x + lane.at[s] : reinterpret_cast<const T*>(a.x), read);
+            copy_async(to + NV * kThreads * 16, read ? dy + lane.at[s] : reinterpret_cast<const T*>(a.x), read);
+          } else {
+            clear(rx[s]);
+            clear(rd[s]);
+            if (read) { rx[s] = load_pack<T, VE>(x + lane.at[s]); rd[s] = load_pack<T, VE>(dy + lane.at[s]); }
+          }
+        }
+        x += a.x_head;
+        dy += a.dy_head;
+        if (++ahead_h == chunk) { ahead_h = 0; ahead += stride; }
+      }
+      if constexpr (RING) copy_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < R - 1; ++i) fetch(i);
+
+    int slot = 0;
+    for (; unit0 < units; unit0 += stride) {
+      const Unit u(a, kind, unit0 + in_warp, unit0 + in_warp < units);
+      T* out = reinterpret_cast<T*>(a.out) + (long long)u.token * a.out_row + u.head * a.out_head;
+      Angles<T, VE, NV, PAIRING, FULL> angles;
+      angles.set(a, turns, lane, g, u.token);
+      for (int h = 0; h < chunk; ++h) {
+        fetch(slot == 0 ? R - 1 : slot - 1);
+        if constexpr (RING) {
+          copy_wait<R - 1>();
+#pragma unroll
+          for (int s = 0; s < NV; ++s) {
+            const uint8_t* from = ring + ((slot * 2 * NV + s) * kThreads + threadIdx.x) * 16;
+            rx[s] = *reinterpret_cast<const Pack<T, VE>*>(from);
+            rd[s] = *reinterpret_cast<const Pack<T, VE>*>(from + NV * kThreads * 16);
+          }
+          slot = slot == R - 1 ? 0 : slot + 1;
+        }
+        uint64_t v[M], d[M], gw[M];
+        unpack<T, VE, NV>(rx, v);
+        unpack<T, VE, NV>(rd, d);
+        angles.rotate(a, lane, g, d);                       // (a.sign: backwards)
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+          if constexpr (VE > 1) {
+            const float2 w = *reinterpret_cast<const float2*>(&weights[lane.has(2 * i / VE) ? lane.at[2 * i / VE] + 2 * i % VE : 0]);
+            gw[i] = mul_f32x2(d[i], pack_f32x2(w.x, w.y));
+          } else {
+            gw[i] = mul_f32x2(d[i], pack_f32x2(weights[max(lane.at[2 * i], 0)], weights[max(lane.at[2 * i + 1], 0)]));
+          }
+        }
+        float q = dot(v, v), p = dot(gw, v);
+        group_sums(q, p, a.group);
+        const float r = rsqrtf(q * a.inv_hd + a.eps);
+        const float mean = p * r * a.inv_hd;                // of g w u
+        const uint64_t r2 = pack_f32x2(r, r), m2 = pack_f32x2(-mean * r, -mean * r);
+        if (h < u.count) {
+#pragma unroll
+          for (int i = 0; i < M; ++i) {
+            const uint64_t unit_x = mul_f32x2(v[i], r2);
+            sums[i] = fma_f32x2(d[i], unit_x, sums[i]);
+            v[i] = fma_f32x2(unit_x, m2, mul_f32x2(gw[i], r2));
+          }
+          Pack<T, VE> res[NV];
+          pack<T, VE, NV>(v, res);
+#pragma unroll
+          for (int s = 0; s < NV; ++s)
+            if (lane.has(s)) store_pack<T, VE>(out + lane.at[s], res[s]);
+        }
+        out += a.out_head;
+      }
     }
-    __syncthreads();
-    for (int c = threadIdx.x; c < a.hd; c += kThreads) {
-      float v = 0.f;
-      for (int k = 0; k < kThreads / 32; ++k) v += smem[k * a.hd + c];
-      a.partial[((size_t)blockIdx.x * 2 + kind) * a.hd + c] = v;
+    if constexpr (RING) copy_wait<0>();                       // (empty groups: the ring is free for the next kind)
+    unit0 -= (units + per_warp - 1) / per_warp * per_warp;    // as in the forward pass
+    if (a.partial != nullptr) {
+      // the lanes that hold the same components: over the warp by shuffles, over the warps in their order
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float2 f = unpack_f32x2(sums[i / 2]);
+        float v = i % 2 ? f.y : f.x;
+        for (int o = a.group; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (in_warp == 0 && lane.component(i) >= 0) reduced[warp][lane.component(i)] = v;
+      }
     }
-    __syncthreads();
+    __syncthreads();                                          // (also: everybody is done with this kind's weights)
+    if (a.partial != nullptr) {
+      for (int c = threadIdx.x; c < a.hd; c += kThreads) {
+        float v = 0.f;
+        for (int k = 0; k < kThreads / 32; ++k) v += reduced[k][c];
+        a.partial[((size_t)blockIdx.x * 2 + kind) * a.hd + c] = v;
+      }
+      __syncthreads();
+    }
   }
-  }
+  copy_rest<T, VE, NV>(a, lane, a.dy, a.dy_row, a.dy_head, unit0 + in_warp, stride);
 }
 
 // dw[c] = sum over the CTAs of partial[cta][which][c], always in the same order: a warp per 32 columns of CTAs' rows, the
@@ -364,17 +593,29 @@ __global__ void __launch_bounds__(256) heads_dw_kernel(const float* __restrict__
   }
 }
 
-// Heads per unit.  More of them share a lane's angles (some 40 instructions each, as many as a head's rotation of the same
-// components), fewer give more units: as many as let every group of the grid have a few.
-constexpr int kChunkHeads = 8;
+// Heads per unit at most.  More of them share a lane's angles, fewer give more units: as many as leave every group of the
+// grid two units.
+constexpr int kChunkHeads = 16;
 
-template <typename T, int VE, int NV, int PAIRING, int KIND>
-int launch(HeadArgs& a, int ctas, cudaStream_t stream) {
-  const int groups = kThreads / a.group;
-  size_t smem = PAIRING == kShared ? (size_t)groups * a.hd * sizeof(float) : 0;
-  if (KIND == kNormBwd && a.partial != nullptr && smem < kThreads / 32 * a.hd * sizeof(float))
-    smem = kThreads / 32 * a.hd * sizeof(float);
-  heads_kernel<T, VE, NV, PAIRING, KIND><<<ctas, kThreads, smem, stream>>>(a);
+enum Pass { kRotate = 0, kForward = 1, kBackward = 2 };
+
+template <typename T, int VE, int NV, int PAIRING, bool FULL, int PASS>
+int launch(const HeadArgs& a, int ctas, cudaStream_t stream) {
+  if constexpr (PASS == kBackward) {
+    auto* kernel = heads_bwd_kernel<T, VE, NV, PAIRING, FULL>;
+    const int smem = VE > 1 ? kBwdRing : 0;
+    static bool configured[64] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (smem > 0 && !configured[dev & 63]) {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return (int)e;
+      configured[dev & 63] = true;
+    }
+    kernel<<<ctas, kThreads, smem, stream>>>(a);
+  } else {
+    heads_fwd_kernel<T, VE, NV, PAIRING, PASS == kRotate ? kRope : kNorm, FULL><<<ctas, kThreads, 0, stream>>>(a);
+  }
   return (int)cudaGetLastError();
 }
 
@@ -382,45 +623,48 @@ inline bool aligned(const void* p, long long row, long long head, int size) {
   return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && row * size % 16 == 0 && head * size % 16 == 0);
 }
 
-template <typename T, int KIND>
+template <typename T, int PASS>
 int dispatch(HeadArgs& a, int* parts, cudaStream_t stream) {
   constexpr int VE = 16 / sizeof(T);
   const int size = sizeof(T);
-  // whole vectors need heads of whole vectors at 16-byte addresses and two vectors per lane of a warp; else one component
-  // per access, in a warp per head
-  const bool vectors = a.hd % VE == 0 && a.hd <= 64 * VE && aligned(a.x, a.x_row, a.x_head, size) &&
-                       aligned(a.dy, a.dy_row, a.dy_head, size) && aligned(a.out, a.out_row, a.out_head, size);
+  // whole vectors need heads of whole vectors at 16-byte addresses, two vectors per lane of a warp, and pairs that lie inside
+  // a vector or whole vectors apart; else a warp per head and single components
+  const bool vectors = a.hd % VE == 0 && a.hd <= 64 * VE && (a.neighbours || a.rd % (2 * VE) == 0) &&
+                       aligned(a.x, a.x_row, a.x_head, size) && aligned(a.dy, a.dy_row, a.dy_head, size) &&
+                       aligned(a.out, a.out_row, a.out_head, size);
   a.group = 32;
   if (vectors)
     for (a.group = 1; a.group * 2 * VE < a.hd; a.group *= 2) {}
-  const long long groups = (long long)current_sm_count() * kCtasPerSm * (kThreads / a.group);
-  int chunk = kChunkHeads;
+  const int most = current_sm_count() * kCtasPerSm, groups_per_cta = kThreads / a.group;
   long long units;
-  for (;; chunk /= 2) {
+  for (int chunk = kChunkHeads;; chunk /= 2) {
     units = 0;
     for (int k = 0; k < 3; ++k) {
-      a.chunk[k] = a.heads[k] < chunk ? (a.heads[k] > 0 ? a.heads[k] : 1) : chunk;
-      a.chunks[k] = (a.heads[k] + a.chunk[k] - 1) / a.chunk[k];
+      a.chunks[k] = (a.heads[k] + chunk - 1) / chunk;
+      a.chunk[k] = a.chunks[k] > 0 ? (a.heads[k] + a.chunks[k] - 1) / a.chunks[k] : 1;
       units += (long long)a.tokens * a.chunks[k];
     }
-    if (chunk == 1 || units >= 2 * groups) break;
+    if (chunk == 1 || units >= 2LL * most * groups_per_cta) break;
   }
   if (units > 0x3fffffffLL) return DD_ERR_TOO_LARGE;
-  const long long want = (units + kThreads / a.group - 1) / (kThreads / a.group);
-  const int most = current_sm_count() * kCtasPerSm;
+  const long long want = (units + groups_per_cta - 1) / groups_per_cta;
   const int ctas = (int)(want < most ? want : most);
   *parts = ctas;
-  if (!vectors) return launch<T, 1, 16, kShared, KIND>(a, ctas, stream);
-  if (a.neighbours) return launch<T, VE, 2, kInside, KIND>(a, ctas, stream);
-  if (a.rd % (2 * VE) == 0) return launch<T, VE, 2, kApart, KIND>(a, ctas, stream);
-  return launch<T, VE, 2, kShared, KIND>(a, ctas, stream);
+  if (!vectors) {
+    if (a.hd <= 128) return launch<T, 1, 4, kInside, false, PASS>(a, ctas, stream);
+    return launch<T, 1, 16, kInside, false, PASS>(a, ctas, stream);
+  }
+  const bool full = a.hd == 2 * VE * a.group;
+  if (a.neighbours)
+    return full ? launch<T, VE, 2, kInside, true, PASS>(a, ctas, stream) : launch<T, VE, 2, kInside, false, PASS>(a, ctas, stream);
+  return full ? launch<T, VE, 2, kApart, true, PASS>(a, ctas, stream) : launch<T, VE, 2, kApart, false, PASS>(a, ctas, stream);
 }
 
-template <int KIND>
+template <int PASS>
 int dispatch_type(HeadArgs& a, int dtype, int* parts, cudaStream_t stream) {
-  if (dtype == 0) return dispatch<__nv_bfloat16, KIND>(a, parts, stream);
-  if (dtype == 1) return dispatch<__half, KIND>(a, parts, stream);
-  if (dtype == 2) return dispatch<float, KIND>(a, parts, stream);
+  if (dtype == 0) return dispatch<__nv_bfloat16, PASS>(a, parts, stream);
+  if (dtype == 1) return dispatch<__half, PASS>(a, parts, stream);
+  if (dtype == 2) return dispatch<float, PASS>(a, parts, stream);
   return DD_ERR_BAD_ARG;
 }
 
@@ -436,6 +680,7 @@ int fill(HeadArgs& a, long long tokens, int hq, int hk, int rest, int hd, int rd
   a.hd = hd; a.rd = rd; a.neighbours = neighbours;
   a.positions = positions; a.wide_positions = wide_positions; a.offset = offset;
   a.magnitude = magnitude;
+  a.inv_hd = 1.f / (float)hd;
   for (int i = 0; i < rd / 2; ++i) a.turns[i] = turns[i];
   return DD_OK;
 }
@@ -464,7 +709,7 @@ DD_API int dd_rotate_heads(const void* x, long long x_row, long long x_head, voi
   a.out = out; a.out_row = out_row; a.out_head = out_head;
   a.sign = sign;
   int parts = 0;
-  return dispatch_type<kRope>(a, dtype, &parts, reinterpret_cast<cudaStream_t>(stream));
+  return dispatch_type<kRotate>(a, dtype, &parts, reinterpret_cast<cudaStream_t>(stream));
 }
 
 // out = the first hq heads of x normed with weight wq and rotated, the next hk with wk, the `rest` behind them copied (left
@@ -485,7 +730,7 @@ DD_API int dd_norm_heads_fwd(const void* x, long long x_row, long long x_head, v
   a.wq = wq; a.wk = wk; a.wide_weights = wide_weights; a.eps = eps;
   a.sign = 1.f;
   int parts = 0;
-  return dispatch_type<kNormFwd>(a, dtype, &parts, reinterpret_cast<cudaStream_t>(stream));
+  return dispatch_type<kForward>(a, dtype, &parts, reinterpret_cast<cudaStream_t>(stream));
 }
 
 // Its gradients: dx [tokens, hq + hk + rest, hd] by strides, dwq / dwk [hd] (null: not wanted) of the weights' type, or with
@@ -510,7 +755,7 @@ DD_API int dd_norm_heads_bwd(const void* x, long long x_row, long long x_head, c
     a.wq = wq; a.wk = wk; a.wide_weights = wide_weights; a.eps = eps;
     a.partial = dwq != nullptr || dwk != nullptr ? partial : nullptr;
     a.sign = -1.f;
-    const int e = dispatch_type<kNormBwd>(a, dtype, &parts, st);
+    const int e = dispatch_type<kBackward>(a, dtype, &parts, st);
     if (e) return e;
   }
   if (dwq == nullptr && dwk == nullptr) return DD_OK;

@@ -1,0 +1,594 @@
+// Routing of tokens to experts in its general form: softmax or sigmoid scores, a bias that takes part in the choice only,
+// choice within the best groups of experts, weights renormalised or not; up to 512 experts, 32 of them per token.  (The plain
+// softmax form for up to 64 bf16 experts is in moe.cu.)
+//
+//   score    s = softmax(l) or 1 / (1 + e^-l) over the E logits of a token;  p = s / sum s
+//   choice   c = s + bias; of the groups (E / groups experts each) the top_groups with the largest value (the largest c, or the
+//            sum of the two largest), of their experts the k largest c; ties go to the lowest number
+//   weights  w = scale * s, or scale * s / (sum of the chosen s)
+//   backward with g on w and q on sum_t p:  d s_i of the chosen from g, d p from q, and ds / dl = s (1 - s) (sigmoid),
+//            written out per case at the kernel
+//
+// An expert whose logit is -inf is never chosen; a token with fewer than k others has -1 and weight 0 in the places left,
+// one with none of them routes nowhere and adds nothing.  A NaN (softmax: also +inf) makes the weights of its token, its p and
+// its gradient NaN, and counts as the best, so that a token of NaN alone is not lost either.
+//
+// The choice is that of exact arithmetic.  Where it follows the logits (no bias, no sums) they are compared themselves.  Else
+// scores in 32 bits decide only where their distance is beyond their error; a token with a closer pair (some in a thousand)
+// is decided in 64 bits, so that neither the order of sums nor the fast exponential shows in the experts.
+//
+// A warp works on a token, its lanes on C consecutive experts each; the k best are taken one by one with a warp-wide integer
+// maximum over order-preserving keys.  A latency below some thousand tokens, above them instructions (some 350 per token of
+// 256 experts) and the logits' bytes.  Slots follow in a second kernel (route_slot_kernel): a pair's slot is its rank in
+// pair order among the pairs of its expert, so nothing depends on how CTAs are scheduled; sums of p are formed per chunk
+// of tokens and then over the chunks, always in the same order.
+#include "common.cuh"
+
+#include <cuda_fp16.h>
+
+using namespace dd;
+
+namespace {
+
+constexpr int kMaxExperts = 512, kMaxChoices = 32, kMaxGroups = 32;
+constexpr int kWarps = 8;
+constexpr int kRows = 32;                                     // tokens of a chunk (a CTA of the first kernel)
+constexpr int kSlotRows = 256, kSlotThreads = 1024;           // tokens and threads of a CTA of the second
+
+struct RouteArgs {
+  const void* logits;       // [tokens, ld]
+  const float* bias;        // [E] or null
+  int* ids;                 // [tokens, k]
+  float* w;                 // [tokens, k]
+  int* hist;                // [chunks][E4]: pairs per expert
+  float* psum;              // [chunks][E4]: sums of p
+  int ld, tokens, E, E4, k;
+  int groups, top_groups, size;                               // size: experts of a group
+  bool group_sum, sigmoid, renormalize, by_logit, vectors;
+  float scale;
+};
+
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f(float v) { return v; }
+template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+
+// C values of one lane in memory, moved in pieces of up to 16 bytes.
+template <typename T, int C> struct alignas(C * sizeof(T) < 16 ? C * sizeof(T) : 16) Row { T v[C]; };
+
+template <typename T, int C>
+__device__ __forceinline__ void load_row(const T* p, bool vectors, int left, float (&l)[C]) {
+  if (vectors && left >= C) {
+    const Row<T, C> r = *reinterpret_cast<const Row<T, C>*>(p);
+#pragma unroll
+    for (int j = 0; j < C; ++j) l[j] = to_f(r.v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < C; ++j) l[j] = j < left ? to_f(p[j]) : -INFINITY;
+  }
+}
+
+// Order-preserving: a < b as floats, key(a) < key(b) as integers; 0 stands for "not to be chosen" (-inf, NaN).
+__device__ __forceinline__ unsigned key_of(float v) {
+  if (!(v > -INFINITY)) return 0u;
+  if (v == 0.f) v = 0.f;                                      // -0 is 0
+  const unsigned u = __float_as_uint(v);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(unsigned key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+__device__ __forceinline__ double warp_sum_d(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// The largest value and the lowest number that has it (-1: all are -inf), over the warp.
+__device__ __forceinline__ void warp_best_d(double& v, int& e) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const double u = __shfl_xor_sync(0xffffffffu, v, o);
+    const int f = __shfl_xor_sync(0xffffffffu, e, o);
+    if (u > v || (u == v && (unsigned)f < (unsigned)e)) { v = u; e = f; }
+  }
+}
+
+// The choice of one token in 64 bits: lane i gets the i-th expert, -1 where there is none.  l_in: this lane's logits (-inf: not
+// to be chosen, or bad: the best), first: its first expert.
+template <int C>
+__device__ __noinline__ int choose_in_64_bits(const RouteArgs& a, const float* l_in, int first, unsigned bad) {
+  const int lane = threadIdx.x & 31;
+  double c[C], top = -INFINITY;
+  for (int j = 0; j < C; ++j) top = fmax(top, (double)l_in[j]);
+  for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+  double z = 0.0;
+  for (int j = 0; j < C; ++j) {
+    const double l = l_in[j];
+    c[j] = a.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top);
+    z += c[j];
+  }
+  z = warp_sum_d(z);
+  for (int j = 0; j < C; ++j) {
+    if (!(l_in[j] > -INFINITY)) { c[j] = (bad >> j) & 1u ? INFINITY : -INFINITY; continue; }
+    if (!a.sigmoid) c[j] /= z;
+    if (a.bias != nullptr) c[j] += (double)a.bias[first + j];
+  }
+  if (a.groups > 1) {
+    double mine = -INFINITY;                                  // lane g: value of group g
+    for (int g = 0; g < a.groups; ++g) {
+      double best[2];
+      int was = -1;
+      for (int r = 0; r < 2; ++r) {
+        double v = -INFINITY;
+        int e = -1;
+        for (int j = 0; j < C; ++j) {
+          const int n = first + j;
+          if (n >= g * a.size && n < (g + 1) * a.size && n != was && c[j] > v) { v = c[j]; e = n; }
+        }
+        warp_best_d(v, e);
+        best[r] = v;
+        was = e;
+      }
+      const double v = a.group_sum && best[1] > -INFINITY ? best[0] + best[1] : best[0];
+      if (lane == g) mine = v;
+    }
+    int place = 0;
+    for (int g = 0; g < a.groups; ++g) {
+      const double v = __shfl_sync(0xffffffffu, mine, g);
+      place += v > mine || (v == mine && g < lane);
+    }
+    const unsigned kept = __ballot_sync(0xffffffffu, lane < a.groups && place < a.top_groups);
+    for (int j = 0; j < C; ++j)
+      if (first + j < a.E && !((kept >> ((first + j) / a.size)) & 1u)) c[j] = -INFINITY;
+  }
+  int chosen = -1;
+  for (int i = 0; i < a.k; ++i) {
+    double v = -INFINITY;
+    int e = -1;
+    for (int j = 0; j < C; ++j)
+      if (c[j] > v) { v = c[j]; e = first + j; }
+    warp_best_d(v, e);
+    if (lane == i) chosen = e;
+    for (int j = 0; j < C; ++j)
+      if (first + j == e) c[j] = -INFINITY;
+  }
+  return chosen;
+}
+
+// Takes the logits without a number (NaN; softmax: +inf) out of a lane's, as bits of `bad`; whether the token has any.
+template <int C>
+__device__ __forceinline__ bool take_bad(float (&l)[C], bool sigmoid, unsigned& bad) {
+#pragma unroll
+  for (int j = 0; j < C; ++j)
+    if (l[j] != l[j] || (!sigmoid && l[j] == INFINITY)) {
+      bad |= 1u << j;
+      l[j] = -INFINITY;
+    }
+  return __any_sync(0xffffffffu, bad != 0u);
+}
+
+// Scores of a token, p = s / sum s (0 in rows without an expert), and what they are computed with.
+template <int C>
+struct Scores {
+  float top;                // largest logit
+  float inv;                // p = part * inv
+  float part[C];            // softmax: e^(l - top); sigmoid: s / e^min(top, 0), which does not underflow in whole rows
+  bool none;                // no expert may be chosen
+
+  __device__ __forceinline__ void set(const float (&l)[C], bool sigmoid) {
+    top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < C; ++j) top = fmaxf(top, l[j]);
+    top = warp_max(top);
+    none = top == -INFINITY;
+    float z = 0.f;
+    const float shift = sigmoid ? fminf(top, 0.f) : top;
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      if (sigmoid) {
+        const float e = __expf(-fabsf(l[j]));
+        part[j] = __fdividef(l[j] > 0.f ? 1.f : shift == 0.f ? e : __expf(l[j] - shift), 1.f + e);
+      } else {
+        part[j] = __expf(l[j] - shift);
+      }
+      if (none || l[j] == -INFINITY) part[j] = 0.f;
+      z += part[j];
+    }
+    inv = none ? 0.f : 1.f / warp_sum(z);
+  }
+};
+
+template <typename T, int C>
+__global__ void __launch_bounds__(kWarps * 32) route_kernel(const __grid_constant__ RouteArgs a) {
+  __shared__ int s_hist[kMaxExperts];
+  __shared__ __align__(16) float s_row[kWarps][32 * C];       // a warp's values by expert; at the end its sums of p
+  grid_dependency_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = threadIdx.x; e < a.E; e += kWarps * 32) s_hist[e] = 0;
+  __syncthreads();
+  const int first = lane * C;
+  const int left = min(max(a.E - first, 0), C);               // experts of this lane
+  float bias[C];
+#pragma unroll
+  for (int j = 0; j < C; ++j) bias[j] = a.bias != nullptr && j < left ? a.bias[first + j] : 0.f;
+  float sums[C];
+#pragma unroll
+  for (int j = 0; j < C; ++j) sums[j] = 0.f;
+
+  for (int row = warp; row < kRows; row += kWarps) {
+    const int t = blockIdx.x * kRows + row;
+    if (t >= a.tokens) break;
+    const T* from = reinterpret_cast<const T*>(a.logits) + (size_t)t * a.ld;
+    float l[C];
+    load_row<T, C>(from + first, a.vectors, left, l);
+    unsigned bad = 0u;                                        // this lane's experts without a number
+    const bool nan = take_bad<C>(l, a.sigmoid, bad);
+    Scores<C> s;
+    s.set(l, a.sigmoid);
+    unsigned key[C];
+    float near = 0.f;                                         // distances up to here (and 4e-7 of the value) are within errors
+    if (a.by_logit) {
+#pragma unroll
+      for (int j = 0; j < C; ++j) key[j] = j < left ? key_of(l[j]) : 0u;
+    } else {
+      // sigmoid: 4e-7 off at most (its slope times the exponential's error, a division); softmax: 4e-6 of the largest
+      const float back = a.sigmoid ? __expf(fminf(s.top, 0.f)) : s.inv;
+      near = a.sigmoid ? 2e-6f : 8e-6f * s.inv;
+#pragma unroll
+      for (int j = 0; j < C; ++j) key[j] = j < left && l[j] > -INFINITY ? key_of(s.part[j] * back + bias[j]) : 0u;
+    }
+    bool close = false;
+    if (nan) {
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+        if ((bad >> j) & 1u) key[j] = 0xffffffffu;
+    }
+    if (a.groups > 1) {
+      // value of every group, by lane g; through shared memory, where a group may begin and end at any lane
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+        if (j < left) s_row[warp][first + j] = key[j] ? ((bad >> j) & 1u ? INFINITY : value_of(key[j])) : -INFINITY;
+      __syncwarp();
+      float value = -INFINITY;
+      // (lanes that share a group's scan: as many as there are for every group)
+      const int share = a.groups > 16 ? 1 : a.groups > 8 ? 2 : a.groups > 4 ? 4 : a.groups > 2 ? 8 : 16;
+      {
+        const int g = lane / share;
+        float b0 = -INFINITY, b1 = -INFINITY;
+        if (g < a.groups)
+          for (int i = lane % share; i < a.size; i += share) {
+            const float v = s_row[warp][g * a.size + i];
+            b1 = fmaxf(b1, fminf(b0, v));
+            b0 = fmaxf(b0, v);
+          }
+        for (int o = share >> 1; o > 0; o >>= 1) {
+          const float o0 = __shfl_xor_sync(0xffffffffu, b0, o), o1 = __shfl_xor_sync(0xffffffffu, b1, o);
+          b1 = fmaxf(fmaxf(b1, o1), fminf(b0, o0));
+          b0 = fmaxf(b0, o0);
+        }
+        const float v = a.group_sum && b1 > -INFINITY ? b0 + b1 : b0;
+        value = __shfl_sync(0xffffffffu, v, min(lane * share, 31));
+        if (lane >= a.groups) value = -INFINITY;
+      }
+      __syncwarp();
+      int place = 0;
+      for (int g = 0; g < a.groups; ++g) {
+        const float v = __shfl_sync(0xffffffffu, value, g);
+        place += v > value || (v == value && g < lane);
+      }
+      const bool in = lane < a.groups && place < a.top_groups;
+      const unsigned kept = __ballot_sync(0xffffffffu, in);
+      if (!a.by_logit && a.top_groups < a.groups) {
+        const float least = -warp_max(in ? -value : -INFINITY), most = warp_max(!in ? value : -INFINITY);
+        close = least - most <= 2.f * near + 4e-7f * fmaxf(fabsf(least), fabsf(most));
+      }
+      int g = first / a.size, at = first - g * a.size;
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        if (!((kept >> (g & 31)) & 1u)) key[j] = 0u;
+        if (++at == a.size) { at = 0; ++g; }
+      }
+    }
+    // the k best one by one: lane i keeps the i-th
+    int chosen = -1, was = -1;
+    unsigned best = 0u, was_key = 0u;
+#pragma unroll
+    for (int j = 0; j < C; ++j) best = max(best, key[j]);
+    const int rounds = a.k + (a.by_logit ? 0 : 1);            // (one more: the first that is left out must not be close)
+    for (int i = 0; i < rounds; ++i) {
+      const unsigned top = __reduce_max_sync(0xffffffffu, best);
+      if (top == 0u) break;
+      const int owner = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
+      int e = 0;
+#pragma unroll
+      for (int j = C - 1; j >= 0; --j) e = key[j] == top ? first + j : e;
+      e = __shfl_sync(0xffffffffu, e, owner);
+      if (!a.by_logit && i > 0) {
+        const float hi = value_of(was_key), lo = value_of(top);
+        if (hi - lo <= near + 4e-7f * fmaxf(fabsf(hi), fabsf(lo))) {
+          // two alike in logit and bias are alike, and in order
+          close |= to_f(from[was]) != to_f(from[e]) || (a.bias != nullptr && a.bias[was] != a.bias[e]);
+        }
+        was_key = top;
+      } else {
+        was_key = top;
+      }
+      was = e;
+      if (lane == i && i < a.k) chosen = e;
+      if (lane == owner) {
+        best = 0u;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+          if (first + j == e) key[j] = 0u;
+          best = max(best, key[j]);
+        }
+      }
+    }
+    if (close) {                                              // (the same on every lane)
+      float again[C];
+#pragma unroll
+      for (int j = 0; j < C; ++j) again[j] = l[j];
+      chosen = choose_in_64_bits<C>(a, again, first, bad);
+    }
+    // the weights, from the chosen logits: sums of k lanes, shifted so that the largest does not underflow
+    float weight = 0.f;
+    {
+      const float lc = chosen >= 0 && !nan ? to_f(from[chosen]) : -INFINITY;
+      const float top = a.renormalize ? warp_max(lc) : s.top;
+      float v;
+      if (a.sigmoid) {
+        const float shift = a.renormalize ? fminf(top, 0.f) : 0.f, e = __expf(-fabsf(lc));
+        v = __fdividef(lc > 0.f ? 1.f : shift == 0.f ? e : __expf(lc - shift), 1.f + e);
+      } else {
+        v = __expf(lc - top);
+      }
+      if (chosen < 0) v = 0.f;
+      if (a.renormalize) v = __fdividef(v, warp_sum(v));
+      else if (!a.sigmoid) v *= s.inv;
+      weight = chosen < 0 ? 0.f : a.scale * v;
+      if (nan && chosen >= 0) weight = __int_as_float(0x7fffffff);
+    }
+    if (lane < a.k) {
+      a.ids[(size_t)t * a.k + lane] = chosen;
+      a.w[(size_t)t * a.k + lane] = weight;
+      if (chosen >= 0) atomicAdd(&s_hist[chosen], 1);
+    }
+#pragma unroll
+    for (int j = 0; j < C; ++j) sums[j] += nan ? __int_as_float(0x7fffffff) : s.part[j] * s.inv;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < C; ++j) s_row[warp][first + j] = sums[j];
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.E4; e += kWarps * 32) {
+    float v = 0.f;
+    for (int k = 0; k < kWarps; ++k) v += s_row[k][e];
+    a.psum[(size_t)blockIdx.x * a.E4 + e] = e < a.E ? v : 0.f;
+    a.hist[(size_t)blockIdx.x * a.E4 + e] = e < a.E ? s_hist[e] : 0;
+  }
+}
+
+// slot[pair] = rank of the pair among those of its expert in pair order, -1 from the capacity on (and for -1 in ids).  The
+// experts of a token differ, so that the rank is the number of earlier tokens: whole CTAs before (sums over the chunks'
+// histograms), words of 32 tokens before, lower bits in the word.
+__global__ void __launch_bounds__(kSlotThreads)
+route_slot_kernel(const int* __restrict__ ids, int tokens, int k, int E, int E4, int capacity, const int* __restrict__ hist,
+                  const float* __restrict__ psum, int chunks, int* __restrict__ counts, float* __restrict__ prob_sum,
+                  int* __restrict__ slot) {
+  constexpr int W = kSlotRows / 32;
+  __shared__ unsigned s_mask[W][kMaxExperts];
+  __shared__ __align__(16) int s_part[kSlotThreads * 4];      // sums before this CTA; then [W][kMaxExperts] bases
+  grid_dependency_launch();
+  const int tid = threadIdx.x, lane = tid & 31;
+  for (int i = tid; i < W * kMaxExperts; i += kSlotThreads) (&s_mask[0][0])[i] = 0u;
+  const int quads = E4 / 4, lanes = kSlotThreads / quads;     // threads per four experts
+  const int t0 = blockIdx.x * kSlotRows;
+  {
+    const int q = tid % quads, r0 = tid / quads;
+    const int before = min(t0 / kRows, chunks);
+    int4 sum = make_int4(0, 0, 0, 0);
+    if (r0 < lanes) {
+#pragma unroll 8
+      for (int r = r0; r < before; r += lanes) {
+        const int4 v = *reinterpret_cast<const int4*>(hist + (size_t)r * E4 + q * 4);
+        sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+      }
+      *reinterpret_cast<int4*>(&s_part[(r0 * quads + q) * 4]) = sum;
+    }
+  }
+  __syncthreads();
+  const int pairs = min(tokens - t0, kSlotRows) * k;
+  for (int p = tid; p < pairs; p += kSlotThreads) {
+    const int e = ids[(size_t)t0 * k + p];
+    if (e >= 0 && e < E) atomicOr(&s_mask[(p / k) >> 5][e], 1u << ((p / k) & 31));
+  }
+  int run = 0;
+  if (tid < E)
+    for (int r = 0; r < min(lanes, t0 / kRows); ++r) run += s_part[r * E4 + tid];
+  __syncthreads();
+  if (tid < E) {
+    for (int w = 0; w < W; ++w) {
+      s_part[w * kMaxExperts + tid] = run;
+      run += __popc(s_mask[w][tid]);
+    }
+    if (blockIdx.x == gridDim.x - 1) counts[tid] = run;
+  }
+  __syncthreads();
+  for (int p = tid; p < pairs; p += kSlotThreads) {
+    const int e = ids[(size_t)t0 * k + p], tok = p / k;
+    int s = -1;
+    if (e >= 0 && e < E) {
+      s = s_part[(tok >> 5) * kMaxExperts + e] + __popc(s_mask[tok >> 5][e] & ((1u << (tok & 31)) - 1u));
+      if (s >= capacity) s = -1;
+    }
+    slot[(size_t)t0 * k + p] = s;
+  }
+  // the sums of p over the chunks: a warp of the grid per four experts, its lanes every 32nd chunk
+  for (int q = blockIdx.x * (kSlotThreads / 32) + (tid >> 5); q < quads; q += gridDim.x * (kSlotThreads / 32)) {
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int r = lane; r < chunks; r += 32) {
+      const float4 v = *reinterpret_cast<const float4*>(psum + (size_t)r * E4 + q * 4);
+      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+    }
+    const float out[4] = {warp_sum(sum.x), warp_sum(sum.y), warp_sum(sum.z), warp_sum(sum.w)};
+    if (lane < 4 && q * 4 + lane < E) prob_sum[q * 4 + lane] = out[lane];
+  }
+}
+
+// dl of a token.  With w = scale * what the weights are without it, D = sum over the chosen of (w / scale) dw:
+//   renormalised: G_i = w_i (dw_i - D) for the chosen i;  else G_i = w_i dw_i (softmax: and -p_e scale D for all e)
+//   dl_e = f_e (G_e + p_e (q_e - sum p q)),  f = 1 (softmax) or 1 - s_e (sigmoid)
+template <typename T, int C>
+__global__ void __launch_bounds__(kWarps * 32)
+route_bwd_kernel(const __grid_constant__ RouteArgs a, const float* __restrict__ dw, const float* __restrict__ dprob, T* __restrict__ dlogits) {
+  __shared__ __align__(16) float s_row[kWarps][32 * C];
+  grid_dependency_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = lane * C, left = min(max(a.E - first, 0), C);
+  float coef[C];
+#pragma unroll
+  for (int j = 0; j < C; ++j) coef[j] = dprob != nullptr && j < left ? dprob[first + j] : 0.f;
+  for (int t = blockIdx.x * kWarps + warp; t < a.tokens; t += gridDim.x * kWarps) {
+    float l[C];
+    load_row<T, C>(reinterpret_cast<const T*>(a.logits) + (size_t)t * a.ld + first, a.vectors, left, l);
+    int id = -1;
+    float w = 0.f, g = 0.f;
+    if (lane < a.k) {
+      id = a.ids[(size_t)t * a.k + lane];
+      w = a.w[(size_t)t * a.k + lane];
+      if (dw != nullptr && id >= 0) g = dw[(size_t)t * a.k + lane];
+    }
+#pragma unroll
+    for (int j = 0; j < C; ++j) s_row[warp][first + j] = 0.f;
+    const float wd = warp_sum(id >= 0 ? w * g : 0.f);         // scale * D
+    const float grad = a.renormalize ? w * (g - __fdividef(wd, a.scale)) : w * g;
+    __syncwarp();
+    if (id >= 0 && id < a.E) s_row[warp][id] = grad;
+    unsigned bad = 0u;
+    const bool nan = take_bad<C>(l, a.sigmoid, bad);
+    Scores<C> s;
+    s.set(l, a.sigmoid);
+    float p[C], pq = 0.f;
+#pragma unroll
+    for (int j = 0; j < C; ++j) { p[j] = s.part[j] * s.inv; pq += p[j] * coef[j]; }
+    pq = warp_sum(pq);
+    const float all = !a.renormalize && !a.sigmoid ? wd : 0.f;
+    __syncwarp();
+    Row<T, C> out;
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const float f = a.sigmoid ? __fdividef(l[j] > 0.f ? __expf(-l[j]) : 1.f, 1.f + __expf(-fabsf(l[j]))) : 1.f;
+      const float v = f * (s_row[warp][first + j] + p[j] * (coef[j] - pq - all));
+      out.v[j] = from_f<T>(j >= left ? 0.f : nan ? __int_as_float(0x7fffffff) : v);
+    }
+    T* to = dlogits + (size_t)t * a.ld;
+    if (a.vectors) {
+      if (first < a.ld) *reinterpret_cast<Row<T, C>*>(to + first) = out;
+    } else {
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+        if (first + j < a.ld) to[first + j] = out.v[j];
+    }
+    for (int e = 32 * C + lane; e < a.ld; e += 32) to[e] = from_f<T>(0.f);
+    __syncwarp();
+  }
+}
+
+bool fill(RouteArgs& a, const void* logits, int ld, int size, int tokens, int E, int k, int sigmoid, int renormalize,
+          float scale, int* c) {
+  if (E < 1 || E > kMaxExperts || k < 1 || k > kMaxChoices || k > E || ld < E || tokens < 1 || logits == nullptr) return false;
+  if ((long long)tokens * k > 0x7fffffffLL) return false;
+  a.logits = logits;
+  a.ld = ld; a.tokens = tokens; a.E = E; a.k = k;
+  a.E4 = (E + 3) / 4 * 4;
+  a.sigmoid = sigmoid != 0; a.renormalize = renormalize != 0; a.scale = scale;
+  int C = 1;
+  while (32 * C < E) C *= 2;
+  *c = C;
+  // rows of whole lanes at addresses that a lane's values can be moved at in one piece (or in pieces of 16 bytes)
+  const int piece = C * size < 16 ? C * size : 16;
+  a.vectors = ld % C == 0 && (long long)ld * size % piece == 0 && reinterpret_cast<uintptr_t>(logits) % piece == 0;
+  return true;
+}
+
+template <typename T>
+int forward(const RouteArgs& a, int C, int chunks, cudaStream_t s) {
+  constexpr int threads = kWarps * 32;
+  if (C == 1) route_kernel<T, 1><<<chunks, threads, 0, s>>>(a);
+  else if (C == 2) route_kernel<T, 2><<<chunks, threads, 0, s>>>(a);
+  else if (C == 4) route_kernel<T, 4><<<chunks, threads, 0, s>>>(a);
+  else if (C == 8) route_kernel<T, 8><<<chunks, threads, 0, s>>>(a);
+  else route_kernel<T, 16><<<chunks, threads, 0, s>>>(a);
+  return (int)cudaGetLastError();
+}
+template <typename T>
+int backward(const RouteArgs& a, int C, const float* dw, const float* dprob, void* dlogits, cudaStream_t s) {
+  constexpr int threads = kWarps * 32;
+  const int want = (a.tokens + kWarps - 1) / kWarps, grid = want < 148 * 32 ? want : 148 * 32;
+  T* d = reinterpret_cast<T*>(dlogits);
+  if (C == 1) route_bwd_kernel<T, 1><<<grid, threads, 0, s>>>(a, dw, dprob, d);
+  else if (C == 2) route_bwd_kernel<T, 2><<<grid, threads, 0, s>>>(a, dw, dprob, d);
+  else if (C == 4) route_bwd_kernel<T, 4><<<grid, threads, 0, s>>>(a, dw, dprob, d);
+  else if (C == 8) route_bwd_kernel<T, 8><<<grid, threads, 0, s>>>(a, dw, dprob, d);
+  else route_bwd_kernel<T, 16><<<grid, threads, 0, s>>>(a, dw, dprob, d);
+  return (int)cudaGetLastError();
+}
+
+}  // namespace
+
+// logits [tokens, ld], the first E columns (dtype 0 bf16, 1 fp16, 2 fp32); bias [E] fp32 or null; ids, w, slot [tokens * k];
+// counts, prob_sum [E]; scratch: `words` words, 16-byte aligned, two for every expert (in fours) and 32 tokens.
+DD_API int dd_route_fwd(const void* logits, int ld, int dtype, int tokens, int E, int k, int capacity, const float* bias,
+                        int groups, int top_groups, int group_sum, int sigmoid, int renormalize, float scale, int* ids,
+                        float* w, int* slot, int* counts, float* prob_sum, int* scratch, long long words,
+                        void* stream) {
+  RouteArgs a = {};
+  int C;
+  const int size = dtype == 2 ? 4 : 2;
+  if (dtype < 0 || dtype > 2 || !fill(a, logits, ld, size, tokens, E, k, sigmoid, renormalize, scale, &C)) return DD_ERR_BAD_ARG;
+  if (groups < 1 || groups > kMaxGroups || E % groups != 0 || top_groups < 1 || top_groups > groups) return DD_ERR_BAD_ARG;
+  if (ids == nullptr || w == nullptr || slot == nullptr || counts == nullptr || prob_sum == nullptr || scratch == nullptr)
+    return DD_ERR_BAD_ARG;
+  if (reinterpret_cast<uintptr_t>(scratch) % 16 != 0) return DD_ERR_ALIGN;
+  const int chunks = (tokens + kRows - 1) / kRows;
+  if (words < 2LL * chunks * a.E4) return DD_ERR_BAD_ARG;
+  a.bias = bias;
+  a.groups = top_groups == groups ? 1 : groups;               // (all groups: no choice among them)
+  a.top_groups = top_groups; a.size = E / groups; a.group_sum = group_sum != 0;
+  a.by_logit = bias == nullptr && !(a.groups > 1 && a.group_sum && a.size > 1);
+  a.ids = ids; a.w = w;
+  a.hist = scratch;
+  a.psum = reinterpret_cast<float*>(scratch + (size_t)chunks * a.E4);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int e = dtype == 0   ? forward<__nv_bfloat16>(a, C, chunks, s)
+                : dtype == 1 ? forward<__half>(a, C, chunks, s)
+                             : forward<float>(a, C, chunks, s);
+  if (e) return e;
+  route_slot_kernel<<<(tokens + kSlotRows - 1) / kSlotRows, kSlotThreads, 0, s>>>(ids, tokens, k, E, a.E4, capacity, a.hist,
+                                                                                 a.psum, chunks, counts, prob_sum, slot);
+  return (int)cudaGetLastError();
+}
+
+// dlogits [tokens, ld] from the gradients of w (dw [tokens, k], or null) and of prob_sum (dprob [E], or null).
+DD_API int dd_route_bwd(const void* logits, int ld, int dtype, int tokens, int E, int k, int sigmoid, int renormalize,
+                        float scale, const int* ids, const float* w, const float* dw, const float* dprob, void* dlogits,
+                        void* stream) {
+  RouteArgs a = {};
+  int C;
+  const int size = dtype == 2 ? 4 : 2;
+  if (dtype < 0 || dtype > 2 || !fill(a, logits, ld, size, tokens, E, k, sigmoid, renormalize, scale, &C)) return DD_ERR_BAD_ARG;
+  if (ids == nullptr || w == nullptr || dlogits == nullptr) return DD_ERR_BAD_ARG;
+  if (reinterpret_cast<uintptr_t>(dlogits) % 16 != 0) return DD_ERR_ALIGN;
+  a.ids = const_cast<int*>(ids);
+  a.w = const_cast<float*>(w);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == 0) return backward<__nv_bfloat16>(a, C, dw, dprob, dlogits, s);
+  if (dtype == 1) return backward<__half>(a, C, dw, dprob, dlogits, s);
+  return backward<float>(a, C, dw, dprob, dlogits, s);
+}

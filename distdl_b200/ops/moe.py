@@ -5,11 +5,13 @@ the reference (its expert layers expect already-routed ``[expert, capacity,
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
 from .. import _native
-from ._util import ptr, stream_ptr, use_native
+from ._util import call_on, ptr, stream_ptr, use_native
+from .pad import _plain
 
 _v, _i, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
 _native.declare("dd_moe_assign", [_v, _i, _i, _i, _v, _v, _v])
@@ -66,16 +68,221 @@ class _RouterFn(torch.autograd.Function):
         return dlogits, None, None, None
 
 
-def route(logits: torch.Tensor, num_experts: int, k: int, capacity: int):
+_native.declare("dd_route_fwd", [_v, _i, _i, _i, _i, _i, _i, _v, _i, _i, _i, _i, _i, _f, _v, _v, _v, _v, _v, _v,
+                                 ctypes.c_longlong, _v])
+_native.declare("dd_route_bwd", [_v, _i, _i, _i, _i, _i, _i, _i, _f, _v, _v, _v, _v, _v, _v])
+_DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_MOST_EXPERTS, _MOST_CHOICES, _MOST_GROUPS = 512, 32, 32
+
+
+def _route_forward(logits, E, k, capacity, how):
+    score, bias, groups, top_groups, group_score, renormalize, scale = how
+    T, ld = logits.shape
+    dev = logits.device
+    ids = torch.empty(T * k, dtype=torch.int32, device=dev)
+    slot = torch.empty(T * k, dtype=torch.int32, device=dev)
+    counts = torch.empty(E, dtype=torch.int32, device=dev)
+    w = torch.empty(T, k, dtype=torch.float32, device=dev)
+    prob_sum = torch.empty(E, dtype=torch.float32, device=dev)
+    words = 2 * ((T + 31) // 32) * ((E + 3) // 4 * 4)
+    scratch = torch.empty(words, dtype=torch.int32, device=dev)
+    call_on(logits, "dd_route_fwd", logits.data_ptr(), ld, _DTYPE[logits.dtype], T, E, k, capacity, ptr(bias), groups,
+            top_groups, int(group_score == "top2"), int(score == "sigmoid"), int(renormalize), scale, ids.data_ptr(),
+            w.data_ptr(), slot.data_ptr(), counts.data_ptr(), prob_sum.data_ptr(), scratch.data_ptr(), words)
+    return w, prob_sum, ids, slot, counts
+
+
+class _RouteFn(torch.autograd.Function):
+    """:func:`route` in its general form: two kernels, and one for the backward pass."""
+
+    @staticmethod
+    def forward(ctx, logits, E, k, capacity, how):
+        w, prob_sum, ids, slot, counts = _route_forward(logits, E, k, capacity, how)
+        ctx.save_for_backward(logits, ids, w)
+        ctx.cfg = (E, k, how)
+        ctx.mark_non_differentiable(ids, slot, counts)
+        ctx.set_materialize_grads(False)
+        return w, prob_sum, ids, slot, counts
+
+    @staticmethod
+    def backward(ctx, dw, dprob, _dids, _dslot, _dcounts):
+        logits, ids, w = ctx.saved_tensors
+        E, k, how = ctx.cfg
+        if torch.is_grad_enabled() or not all(g is None or _plain(g) for g in (dw, dprob)):
+            # differentiated itself, or under a function transform: elementary operations, with the experts as they are
+            with torch.enable_grad():
+                outs = _route_weights(logits, E, ids.reshape(-1, k), how)
+                outs, grads = zip(*[(o, g) for o, g in zip(outs, (dw, dprob)) if g is not None])
+                (d,) = torch.autograd.grad(outs, logits, grads, create_graph=True)
+            return d, None, None, None, None
+        if dw is None and dprob is None:
+            return None, None, None, None, None
+        dw, dprob = (g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) else g.float().contiguous()
+                     for g in (dw, dprob))
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        call_on(logits, "dd_route_bwd", logits.data_ptr(), logits.shape[1], _DTYPE[logits.dtype], logits.shape[0], E, k,
+                int(how[0] == "sigmoid"), int(how[5]), how[6], ids.data_ptr(), w.data_ptr(), ptr(dw), ptr(dprob),
+                dlogits.data_ptr())
+        return dlogits, None, None, None, None
+
+
+def _scores(logits, E, score):
+    """(scores, what they are over their sum) in the type of ``logits``; zeros in rows without an expert."""
+    l = logits[:, :E]
+    none = (l == -math.inf).all(-1, keepdim=True)
+    l = torch.where(none, torch.zeros_like(l), l)
+    if score == "softmax":
+        s = torch.softmax(l, -1)
+        p = s
+    else:
+        s = torch.sigmoid(l)
+        p = torch.softmax(torch.nn.functional.logsigmoid(l), -1)         # s / sum s, however small they are
+    return s.masked_fill(none, 0.0), p.masked_fill(none, 0.0)
+
+
+def _route_weights(logits, E, ids, how):
+    """Weights ``[tokens, k]`` and sums of probabilities for chosen experts ``ids`` (-1: none), fp32."""
+    score, _bias, _groups, _top, _by, renormalize, scale = how
+    wide = logits.double()
+    s, p = _scores(wide, E, score)
+    at = ids.long().clamp(min=0)
+    here = ids >= 0
+    if renormalize:
+        l = wide[:, :E].gather(1, at)
+        l = (l if score == "softmax" else torch.nn.functional.logsigmoid(l)).masked_fill(~here, -math.inf)
+        some = here.any(-1, keepdim=True)
+        w = torch.softmax(torch.where(some, l, torch.zeros_like(l)), -1)
+    else:
+        w = s.gather(1, at)
+    w = (scale * w).masked_fill(~here, 0.0)
+    bad = _bad(wide[:, :E], score)
+    w = torch.where(bad & here, torch.full_like(w, math.nan), w)
+    p = torch.where(bad, torch.full_like(p, math.nan), p)
+    return w.float(), p.sum(0).float()
+
+
+def _bad(l, score):
+    return (torch.isnan(l) | ((l == math.inf) if score == "softmax" else torch.zeros_like(l, dtype=torch.bool))).any(
+        -1, keepdim=True)
+
+
+def _choose(logits, E, k, how):
+    """The experts ``[tokens, k]`` of :func:`route` (-1: none left), in 64 bits."""
+    score, bias, groups, top_groups, group_score, _renormalize, _scale = how
+    l = logits[:, :E].detach().double()
+    c = _scores(l.masked_fill(torch.isnan(l), -math.inf), E, score)[0]
+    if bias is not None:
+        c = c + bias.double()
+    elif groups == 1 or group_score == "max":
+        c = l                                               # the same order, also where scores are no longer told apart
+    c = c.masked_fill(l == -math.inf, -math.inf).masked_fill(torch.isnan(l), math.inf)
+    if score == "softmax":
+        c = c.masked_fill(l == math.inf, math.inf)
+    if top_groups < groups:
+        best = c.reshape(len(c), groups, E // groups).sort(dim=-1, descending=True).values
+        value = best[..., 0]
+        if group_score == "top2" and E > groups:
+            value = torch.where(best[..., 1] > -math.inf, value + best[..., 1], value)
+        kept = value.sort(dim=-1, descending=True, stable=True).indices[:, :top_groups]
+        live = torch.zeros_like(value, dtype=torch.bool).scatter(1, kept, True)
+        c = c.masked_fill(~live.repeat_interleave(E // groups, dim=1), -math.inf)
+    top = c.sort(dim=-1, descending=True, stable=True)
+    ids = top.indices[:, :k].masked_fill(top.values[:, :k] == -math.inf, -1)
+    return ids.to(torch.int32).contiguous()
+
+
+def route(logits: torch.Tensor, num_experts: int, k: int, capacity: int, *, score: str = "softmax", bias=None,
+          groups: int = 1, top_groups: int = None, group_score: str = "max", renormalize: bool = True, scale: float = 1.0):
     """Top-k routing of ``logits [tokens, >= num_experts]`` (extra columns are padding).
 
     Returns ``(weights [tokens, k] fp32, prob_sum [E] fp32, ids [tokens * k] int32, slot
-    [tokens * k] int32, counts [E] int32)``: the renormalised softmax weights of the chosen
-    experts, the sum over tokens of the softmax probabilities (for the load-balancing loss), the
-    chosen experts, each pair's slot in its expert's capacity buffer (-1 = dropped) and the number
-    of pairs routed to every expert.  ``weights`` and ``prob_sum`` carry gradients back to
-    ``logits``."""
+    [tokens * k] int32, counts [E] int32)``: the weights of the chosen experts, the sum over tokens
+    of the probabilities (for a load-balancing loss), the chosen experts in falling order, each pair's slot in its
+    expert's capacity buffer (-1 = dropped) and the number of pairs routed to every expert.  ``weights`` and
+    ``prob_sum`` carry gradients back to ``logits``.
+
+    * ``score``: ``"softmax"`` of the logits, or ``"sigmoid"``; the probabilities are the scores over their sum.
+    * ``bias`` (fp32 ``[num_experts]``): added to the scores for the choice alone (balance without a loss:
+      :func:`balance_bias_`); it carries no gradient.
+    * ``groups``: the experts lie in as many groups of equal size; only those of the ``top_groups`` best are chosen from.  A
+      group counts what its best expert does (``group_score="max"``) or its two best together (``"top2"``).
+    * ``renormalize``: the weights of a token add up to ``scale``; else they are ``scale`` times the scores.
+
+    Equal scores go to the lowest expert, and scores are told apart as exact arithmetic would.  An expert with a logit of
+    -inf is never chosen; where fewer than ``k`` are left the places have id -1, slot -1 and weight 0, and a row of -inf (a
+    padding token) routes nowhere and adds nothing to ``prob_sum``.  A NaN makes the token's weights NaN.  (With all settings
+    at their defaults and up to 64 experts every logit is a finite number, and scores are told apart in fp32.)  bf16, fp16 and
+    fp32 logits of up to 512 experts, with 32 choices and 32 groups at most, run on the kernels."""
     E = num_experts
+    if score == "softmax" and bias is None and groups == 1 and renormalize and scale == 1.0 \
+            and (E <= 64 or not use_native(logits)):
+        return _route_plain_softmax(logits, E, k, capacity)
+    how = _route_check(logits, E, k, score, bias, groups, top_groups, group_score, renormalize, scale)
+    if use_native(logits) and logits.dtype in _DTYPE and E <= _MOST_EXPERTS and k <= _MOST_CHOICES \
+            and groups <= _MOST_GROUPS and logits.numel() and logits.shape[0] * k < 2 ** 31:
+        logits = logits if logits.is_contiguous() else logits.contiguous()
+        if torch.is_grad_enabled() and logits.requires_grad:
+            return _RouteFn.apply(logits, E, k, int(capacity), how)
+        return _route_forward(logits, E, k, int(capacity), how)
+    ids = _choose(logits, E, k, how)
+    w, prob_sum = _route_weights(logits, E, ids, how)
+    slot, counts = _slots_in_order(ids.reshape(-1), E, capacity)
+    return w, prob_sum, ids.reshape(-1), slot, counts
+
+
+def _route_check(logits, E, k, score, bias, groups, top_groups, group_score, renormalize, scale):
+    if logits.dim() != 2 or not logits.is_floating_point():
+        raise ValueError(f"logits come as a floating-point matrix [tokens, experts], not {tuple(logits.shape)} {logits.dtype}")
+    if not 1 <= E <= logits.shape[1]:
+        raise ValueError(f"{E} experts, {logits.shape[1]} logits per token")
+    if not 1 <= k <= E:
+        raise ValueError(f"between 1 and {E} experts per token, not {k}")
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f"score must be 'softmax' or 'sigmoid', not {score!r}")
+    if group_score not in ("max", "top2"):
+        raise ValueError(f"group_score must be 'max' or 'top2', not {group_score!r}")
+    if groups < 1 or E % groups:
+        raise ValueError(f"{E} experts do not lie in {groups} equal groups")
+    top_groups = groups if top_groups is None else top_groups
+    if not 1 <= top_groups <= groups:
+        raise ValueError(f"between 1 and {groups} groups are chosen from, not {top_groups}")
+    if k > top_groups * (E // groups):
+        raise ValueError(f"{top_groups} groups of {E // groups} experts have no {k} to choose")
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"scale must be positive and finite, not {scale}")
+    if bias is not None:
+        if bias.numel() != E or bias.device != logits.device or not bias.is_floating_point():
+            raise ValueError(f"the bias has one value per expert ({E}), on the device of the logits")
+        bias = bias.detach().reshape(-1)
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = bias.float().contiguous()
+    return score, bias, int(groups), int(top_groups), group_score, bool(renormalize), float(scale)
+
+
+@torch.no_grad()
+def balance_bias_(bias: torch.Tensor, counts: torch.Tensor, rate: float) -> torch.Tensor:
+    """One step towards equal load without a loss: the bias of every expert with fewer pairs than the mean of ``counts``
+    (pairs per expert, summed over all workers) grows by ``rate``, that of one with more shrinks by it."""
+    if bias.numel() != counts.numel():
+        raise ValueError(f"{bias.numel()} values of the bias, {counts.numel()} counts")
+    c = counts.reshape(bias.shape).double()
+    return bias.add_((torch.sign(c.mean() - c) * rate).to(bias.dtype))
+
+
+def _slots_in_order(flat, E, capacity):
+    """(slots, counts) for ids in pair order, -1 among them, by a stable sort (any number of experts, any device)."""
+    here = flat >= 0
+    key = torch.where(here, flat, torch.full_like(flat, E)).long()
+    counts = torch.zeros(E + 1, dtype=torch.int64, device=flat.device).scatter_add(0, key, torch.ones_like(key))
+    order = key.sort(stable=True).indices
+    rank = torch.empty_like(key)
+    rank[order] = torch.arange(key.numel(), device=key.device) - (counts.cumsum(0) - counts)[key[order]]
+    slot = torch.where(here & (rank < capacity), rank, torch.full_like(rank, -1))
+    return slot.to(torch.int32), counts[:E].to(torch.int32)
+
+
+def _route_plain_softmax(logits, E, k, capacity):
+    """Softmax, top-k, renormalised: up to 64 bf16 experts on the kernels of ``csrc/moe.cu``."""
     if use_native(logits) and logits.dtype == torch.bfloat16 and E <= 64 and k <= 8 and logits.is_contiguous():
         return _RouterFn.apply(logits, E, k, capacity)
     probs = torch.softmax(logits[:, :E].float(), dim=-1)

@@ -12,6 +12,7 @@ import torch
 
 from .. import _native
 from ._util import call_on, main_grad_now, ptr, use_native
+from .pad import _plain
 
 _v, _i, _l, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 _native.declare("dd_rotate_heads", [_v, _l, _l, _v, _l, _l, _l, _i, _i, _i, _i, _i, _v, _f, _f, _v, _i, _l, _l, _i, _v])
@@ -359,46 +360,66 @@ def _norm_forward(src, dst, hq, hkv, wq, wk, eps, where):
             heads - hq - hkv, hd, dim, near, address, scale, *place, _DTYPE[src.dtype])
 
 
+@functools.lru_cache(maxsize=64)
+def _parts(device: int) -> int:
+    """CTAs of the backward kernel at most, each with a row of sums."""
+    with torch.cuda.device(device):
+        return _native.lib().dd_heads_parts()
+
+
+def _norm_backward(x, dy, wq, wk, hq, hkv, eps, where, want, main=(None, None)):
+    """(dx, dwq, dwk) of :func:`qk_norm_rope`; ``want``: which weights' gradients; ``main``: fp32 accumulators that they are
+    added to instead (both that are wanted, or neither)."""
+    tokens, heads, hd = x.shape
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    w = wq if wq is not None else wk
+    accumulate = main[0] is not None or main[1] is not None
+    dwq, dwk, partial = main[0], main[1], None
+    if want[0] or want[1]:
+        partial = torch.empty(_parts(x.get_device()) * 2 * hd, dtype=torch.float32, device=x.device)
+        if not accumulate:
+            dwq = torch.empty(hd, dtype=w.dtype, device=x.device) if want[0] else None
+            dwk = torch.empty(hd, dtype=w.dtype, device=x.device) if want[1] else None
+    (dim, near, address, scale), place = _turn_args(where, hd)
+    call_on(x, "dd_norm_heads_bwd", *_heads(x), *_heads(dy), *_heads(dx), ptr(wq), ptr(wk),
+            int(w is not None and w.dtype == torch.float32), eps, ptr(dwq), ptr(dwk), int(accumulate), ptr(partial), tokens, hq,
+            hkv, heads - hq - hkv, hd, dim, near, address, scale, *place, _DTYPE[x.dtype])
+    return (dx, None, None) if accumulate else (dx, dwq, dwk)
+
+
 class _QKNormRopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, wq, wk, hq, hkv, eps, rotary, positions, seq, offset):
-        src = _unit(qkv)
         out = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        _norm_forward(src, out, hq, hkv, wq, wk, eps, (rotary, positions, seq, offset))
-        ctx.save_for_backward(src, wq, wk, positions)
+        _norm_forward(_unit(qkv), out, hq, hkv, wq, wk, eps, (rotary, positions, seq, offset))
+        ctx.save_for_backward(qkv, wq, wk, positions)
         ctx.refs = (wq, wk)
         ctx.cfg = (hq, hkv, eps, rotary, seq, offset)
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, wq, wk, positions = ctx.saved_tensors
+        qkv, wq, wk, positions = ctx.saved_tensors
         hq, hkv, eps, rotary, seq, offset = ctx.cfg
-        tokens, heads, hd = x.shape
-        dy = _unit(dy)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        want = [w is not None and ctx.needs_input_grad[k] for k, w in ((1, wq), (2, wk))]
-        wide = next((w.dtype == torch.float32 for w in (wq, wk) if w is not None), False)
-        dw, accumulate = [None, None], False
-        partial = None
-        if any(want):
+        where = (rotary, positions, seq, offset)
+        need = ctx.needs_input_grad
+        if torch.is_grad_enabled() or not _plain(dy):
+            # differentiated itself, or under a function transform: elementary operations
+            leaves = [t for t, n in zip((qkv, wq, wk), need) if n]
+            with torch.enable_grad():
+                out = _plain_qk_norm_rope(qkv, hq, hkv, wq, wk, eps, where)
+                got = iter(torch.autograd.grad(out, leaves, dy, create_graph=True))
+            return (*(next(got) if n else None for n in need[:3]), None, None, None, None, None, None, None)
+        want = need[1:3]
+        main = (None, None)
+        if want[0] or want[1]:
             # gathered weights collect their gradient in fp32 beside them
-            main = [main_grad_now(getattr(r, "main_grad", None), getattr(r, "main_grad_owner", None), ctx, k) if wanted
-                    else None for k, r, wanted in ((1, ctx.refs[0], want[0]), (2, ctx.refs[1], want[1]))]
-            accumulate = all(m is not None for m, wanted in zip(main, want) if wanted)
-            dw = main if accumulate else [torch.empty(hd, dtype=w.dtype, device=x.device) if wanted else None
-                                          for w, wanted in zip((wq, wk), want)]
-            with torch.cuda.device(x.device):
-                parts = _native.lib().dd_heads_parts()
-            partial = torch.empty(parts * 2 * hd, dtype=torch.float32, device=x.device)
-        (dim, near, address, scale), place = _turn_args((rotary, positions, seq, offset), hd)
-        call_on(x, "dd_norm_heads_bwd", *_heads(x), *_heads(dy), *_heads(dx), ptr(wq), ptr(wk), int(wide), eps, ptr(dw[0]),
-                ptr(dw[1]), int(accumulate), ptr(partial), tokens, hq, hkv, heads - hq - hkv, hd, dim, near, address, scale,
-                *place, _DTYPE[x.dtype])
-        if accumulate:
-            dw = [None, None]
-        return dx, dw[0], dw[1], None, None, None, None, None, None, None
+            main = [main_grad_now(getattr(r, "main_grad", None), getattr(r, "main_grad_owner", None), ctx, k) if n else None
+                    for k, r, n in ((1, ctx.refs[0], want[0]), (2, ctx.refs[1], want[1]))]
+            if any(m is None for m, n in zip(main, want) if n):
+                main = (None, None)
+        dx, dwq, dwk = _norm_backward(_unit(qkv), _unit(dy), wq, wk, hq, hkv, eps, where, want, main)
+        return dx, dwq, dwk, None, None, None, None, None, None, None
 
 
 def _norm_args(qkv, hq, hkv, wq, wk, rotary, seq, offset, ranges, positions):
