@@ -1,10 +1,19 @@
-"""Fused AdamW step and sum-of-squares kernels on flat fp32 buffers."""
+"""Fused AdamW step and sum-of-squares kernels on flat fp32 buffers; the norm of many gradients and their clipping."""
 from __future__ import annotations
+
+import array
+import ctypes
+import functools
 
 import torch
 
 from .. import _native
-from ._util import ptr, stream_ptr, use_native
+from ._util import call_on, ptr, stream_ptr, use_native
+
+_native.declare("dd_grad_norm_parts", [ctypes.c_int])
+_native.declare("dd_grad_norm", [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
+                                 ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_double, ctypes.c_int, ctypes.c_int,
+                                 ctypes.c_void_p])
 
 
 def adamw_step_(master, m, v, grad, param_bf16, *, lr, beta1, beta2, eps, weight_decay, step,
@@ -58,3 +67,114 @@ def accumulate_f32_(acc: torch.Tensor, g: torch.Tensor, scale: float = 1.0) -> N
         _native.call("dd_cast_bf16_f32", g.data_ptr(), acc.data_ptr(), g.numel(), float(scale), 1, stream_ptr())
     else:
         acc.add_(g.reshape(-1).to(acc.dtype), alpha=scale)
+
+
+_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the elements of ``t`` fill a piece of memory without holes and without sharing any, in whatever order."""
+    if t.is_contiguous():
+        return True
+    need = 1
+    for stride, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != need:
+            return False
+        need *= n
+    return True
+
+
+def _tensors(tensors):
+    """(addresses, sizes, type codes) as C arrays and their number, the tensors' device, and whether the kernels take them
+    (CUDA, bf16 / fp16 / fp32, dense, all on one device)."""
+    device = tensors[0].device
+    native = use_native(tensors[0])
+    for t in tensors:
+        if t.device != device:
+            raise ValueError(f"gradients on {device} and on {t.device}: a norm is of one device's tensors")
+        if t.layout is not torch.strided:
+            raise ValueError(f"gradients are dense tensors, not {t.layout}")
+        if t.dtype not in _CODES:
+            if not t.is_floating_point():
+                raise ValueError(f"gradients are floating-point tensors, not {t.dtype}")
+            native = False
+        elif native and not t.is_contiguous() and not _dense(t):
+            native = False
+    if not native:
+        return None
+    return (array.array("Q", [t.data_ptr() for t in tensors]), array.array("q", [t.numel() for t in tensors]),
+            array.array("B", [_CODES[t.dtype] for t in tensors]))
+
+
+def _flat(tensors):
+    if isinstance(tensors, torch.Tensor):
+        tensors = [tensors]
+    return [t for t in tensors if t is not None]
+
+
+def _plain_sumsq(tensors):
+    return torch.stack([t.detach().double().square().sum() for t in tensors]).sum()
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_parts(device: int, count: int) -> int:
+    with torch.cuda.device(device):
+        return _native.lib().dd_grad_norm_parts(count)
+
+
+def _grad_norm(tensors, lists, norm, squared, max_norm, given, clip):
+    p, n, code = (a.buffer_info()[0] for a in lists)
+    parts = 0 if given else _norm_parts(tensors[0].get_device(), len(tensors))
+    scratch = None if given else torch.empty(parts, dtype=torch.float64, device=tensors[0].device)
+    call_on(tensors[0], "dd_grad_norm", p, n, code, len(tensors), ptr(scratch), parts, ptr(norm), ptr(squared), max_norm,
+            int(given), int(clip))
+
+
+@torch.no_grad()
+def grad_norm(tensors, squared: bool = False) -> torch.Tensor:
+    """The 2-norm of all elements of ``tensors`` (one tensor, or an iterable; None is passed over) as an fp32 scalar on their
+    device, or with ``squared`` the sum of squares in fp64 (to be added over workers).  Squares and sums are formed in 64
+    bits, in an order that does not change from run to run.  bf16, fp16 and fp32, mixed as they come, run on the kernels."""
+    tensors = _flat(tensors)
+    if not tensors:
+        return torch.zeros((), dtype=torch.float64 if squared else torch.float32)
+    lists = _tensors(tensors)
+    if lists is None:
+        total = _plain_sumsq(tensors)
+        return total if squared else total.sqrt().float()
+    out = torch.empty((), dtype=torch.float64 if squared else torch.float32, device=tensors[0].device)
+    _grad_norm(tensors, lists, None if squared else out, out if squared else None, 0.0, False, False)
+    return out
+
+
+@torch.no_grad()
+def clip_grad_norm_(tensors, max_norm: float, norm: torch.Tensor = None) -> torch.Tensor:
+    """Scales gradients in place by ``min(1, max_norm / (norm + 1e-6))``, ``norm`` being their 2-norm, which is returned (an
+    fp32 scalar on their device; nothing waits for it).  ``tensors``: gradients, or parameters (whose ``.grad`` is meant:
+    leaves that require a gradient), None passed over.  ``norm`` given (an fp32 scalar on their device, say of the gradients
+    of all workers): that norm is taken.  Where the norm is not above ``max_norm`` nothing is written; one that is not a
+    number makes all gradients so.  The tensors must not share memory with one another."""
+    tensors = [t.grad if t.requires_grad and t.is_leaf else t for t in _flat(tensors)]
+    tensors = _flat(tensors)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative, and a number: {max_norm}")
+    if norm is not None and (norm.numel() != 1 or norm.dtype != torch.float32):
+        raise ValueError(f"norm must be an fp32 scalar, not {tuple(norm.shape)} {norm.dtype}")
+    if not tensors:
+        return torch.zeros((), dtype=torch.float32) if norm is None else norm
+    if norm is not None and norm.device != tensors[0].device:
+        raise ValueError(f"the norm is on {norm.device}, the gradients on {tensors[0].device}")
+    lists = _tensors(tensors)
+    if lists is None:
+        norm = _plain_sumsq(tensors).sqrt().float() if norm is None else norm
+        scale = (max_norm / (norm + 1e-6)).clamp(max=1.0).reshape(())
+        for t in tensors:
+            t.copy_(t * scale if t.dtype == torch.float64 else t.float() * scale)
+        return norm
+    given = norm is not None
+    if not given:
+        norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
+    _grad_norm(tensors, lists, norm, None, max_norm, given, True)
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    return norm
