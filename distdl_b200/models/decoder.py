@@ -22,6 +22,7 @@ from __future__ import annotations
 import math
 import os
 from dataclasses import dataclass
+from typing import Optional
 
 import numpy as np
 import torch
@@ -74,6 +75,16 @@ class DecoderConfig:
                                       # head counts must divide by cp)
     collect_state: bool = False       # state_dict() / load_state_dict() in the serial layout on the first worker:
                                       # a checkpoint that loads on any worker grid
+    rotary: Optional[ops.Rotary] = None   # other rotations than of whole heads by rope_theta: pairings, a part of the
+                                          # head, scaling for long contexts (ops.Rotary)
+    qk_norm: bool = False        # RMS norm of every query and key head, in one pass with the rotation
+    router_score: str = "softmax"         # "softmax" | "sigmoid"; this and the following as ops.moe.route takes them
+    router_bias: bool = False             # a bias per expert for the choice alone, moved by Decoder.balance_routers()
+    router_groups: int = 1
+    router_top_groups: Optional[int] = None
+    router_group_score: str = "max"       # "max" | "top2"
+    router_renormalize: bool = True
+    router_scale: float = 1.0
 
     @property
     def head_dim(self):
@@ -90,7 +101,7 @@ class DecoderConfig:
         if self.n_experts:
             ffn = ffn * self.n_experts + d * self.n_experts
         emb = 2 * self.vocab_size * d + (0 if self.rope else self.max_seq * d)
-        return L * (attn + ffn + 2 * d) + emb + d
+        return L * (attn + ffn + 2 * d + (2 * hd if self.qk_norm else 0)) + emb + d
 
     def train_flops_per_token(self, seq: int = None):
         """Model FLOPs of one training token (forward + backward, no recomputation): 6 per weight
@@ -176,6 +187,12 @@ class Attention(torch.nn.Module):
         self.qkv = _col(cfg, layout, cfg.d_model, (cfg.n_heads + 2 * cfg.n_kv_heads) * hd, num_heads=cfg.n_heads,
                         num_heads_kv=cfg.n_kv_heads)
         self.out = _row(cfg, layout, cfg.n_heads * hd, cfg.d_model, num_heads=cfg.n_heads)
+        self.qk_norm = None
+        if cfg.qk_norm:
+            rotary = (cfg.rotary or ops.Rotary(theta=cfg.rope_theta)) if cfg.rope else None
+            self.qk_norm = dnn.DistributedQKNormRope(
+                layout.P_seq, hd, rotary=rotary, eps=cfg.eps, dtype=cfg.dtype, collect_state=cfg.collect_state,
+                auto_clear_buffer=not (cfg.keep_gathered or cfg.keep_norms_gathered))
         self.ring = None
         if layout.cp > 1:
             if cfg.cp_mode == "a2a":
@@ -192,18 +209,20 @@ class Attention(torch.nn.Module):
         del x
         b, s = qkv.shape[0], qkv.shape[1]
         lay3 = (b * s, self.hq + 2 * self.hkv, cfg.head_dim)
+        # the positions of this worker's block of the sequence are global
+        place = {}
+        if self.ring is not None and cfg.cp_mode == "zigzag":
+            place = dict(ranges=zigzag_ranges(self.layout.cp, self.layout.cp_index, s * self.layout.cp))
+        elif self.ring is not None:
+            place = dict(offset=self.layout.cp_index * s)
+        if self.qk_norm is not None:
+            qkv = self.qk_norm(qkv.reshape(lay3), s, self.hq, self.hkv, **place)
+        elif cfg.rope:
+            qkv = ops.rope_(qkv, s, self.hq + self.hkv, cfg.rope_theta, layout=lay3, rotary=cfg.rotary, **place)
         if self.ring is None:
-            if cfg.rope:
-                qkv = ops.rope_(qkv, s, self.hq + self.hkv, cfg.rope_theta, layout=lay3)
             o = ops.attention_packed(qkv.reshape(lay3), self.hq, self.hkv, b, s, causal=True)
         else:
-            # context parallel: s is this worker's block of the sequence; positions are global
-            if cfg.rope and cfg.cp_mode == "zigzag":
-                qkv = ops.rope_(qkv, s, self.hq + self.hkv, cfg.rope_theta, layout=lay3,
-                                ranges=zigzag_ranges(self.layout.cp, self.layout.cp_index, s * self.layout.cp))
-            elif cfg.rope:
-                qkv = ops.rope_(qkv, s, self.hq + self.hkv, cfg.rope_theta, offset=self.layout.cp_index * s,
-                                layout=lay3)
+            # context parallel: s is this worker's block of the sequence
             t = qkv.reshape(b, s, self.hq + 2 * self.hkv, cfg.head_dim)
             q, k, v = t.split([self.hq, self.hkv, self.hkv], dim=2)
             o = self.ring(q.contiguous(), k.contiguous(), v.contiguous())
@@ -278,7 +297,7 @@ class Block(torch.nn.Module):
         h = tok * (-(-ffn // tp)) * e
         if cfg.n_experts:
             h = int(h * cfg.top_k * cfg.capacity_factor * 1.5) + 4 * tok * d * e
-        kept = 2 * x + 2 * gathered + qkv + o + h
+        kept = 2 * x + 2 * gathered + qkv * (2 if cfg.qk_norm else 1) + o + h      # (heads before and behind their norm)
         import os
         if os.environ.get("DISTDL_FORCE_TORCH", "0") == "1":
             # the library operators keep more: the rotary embedding is not in place (a second copy of the
@@ -552,6 +571,18 @@ class Decoder(torch.nn.Module):
         if delta is None:
             return self.final_norm(x)
         return _add_norm(self.final_norm, x, delta)[1]
+
+    def balance_routers(self, rate: float):
+        """One step of the routers' biases (``DecoderConfig.router_bias``) towards equal load, after an optimizer step:
+        experts that got fewer of the pairs routed since the last call than the mean are favoured by ``rate``, the others
+        the reverse (``ops.moe.balance_bias_``).  The pairs of all workers count; collective over them."""
+        mlps = [b.mlp for b in self.blocks if getattr(b.mlp, "router_bias", None) is not None]
+        if not mlps:
+            return
+        counts = np.stack([m.take_routed() for m in mlps])
+        counts = torch.as_tensor(self.layout.P_grid.allreduce_data(counts))
+        for m, c in zip(mlps, counts):
+            ops.moe.balance_bias_(m.router_bias, c.to(m.router_bias.device), rate)
 
     def loss(self, tokens, targets, scale=None, unit_grad=False):
         """Sum of this worker's token losses times ``scale`` (default: 1 / local

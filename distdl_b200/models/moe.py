@@ -14,6 +14,7 @@ from __future__ import annotations
 import math
 import os
 
+import numpy as np
 import torch
 import torch.distributed as dist
 
@@ -109,6 +110,12 @@ class MoEFeedForward(torch.nn.Module):
             self.w_down.normal_(0.0, cfg.init_std / math.sqrt(2 * cfg.n_layers))
         self.aux_loss = None
         self.last_dropped = None
+        self.router_bias = None
+        self._routed = None             # pairs per expert since the last take_routed()
+        if cfg.router_bias:
+            # the same on all workers: moved by the counts of all of them (Decoder.balance_routers)
+            del self.router_bias
+            self.register_buffer("router_bias", torch.zeros(E, dtype=torch.float32, device=dev))
         self.collect_state = collect
         if collect:
             # serial layout: all experts along dimension 0, on the first worker only
@@ -129,6 +136,8 @@ class MoEFeedForward(torch.nn.Module):
             full = self.gather_experts[name](destination.pop(prefix + name).detach())
             if self.P_root.active:
                 destination[prefix + name] = full
+        if self.router_bias is not None and not self.P_root.active:
+            destination.pop(prefix + "router_bias")
         return destination
 
     def _scatter_state_dict(self, destination, prefix, *args):
@@ -138,7 +147,18 @@ class MoEFeedForward(torch.nn.Module):
             full = destination.pop(prefix + name, None)
             full = full.to(p.device) if self.P_root.active else zero_volume_tensor(device=p.device, dtype=p.dtype)
             destination[prefix + name] = self.scatter_experts[name](full)
+        if self.router_bias is not None:
+            # the first worker's, on all of them
+            mine = destination.get(prefix + "router_bias") if self.P_root.active else torch.zeros(self.cfg.n_experts)
+            destination[prefix + "router_bias"] = torch.as_tensor(
+                self.P_ep.allreduce_data(mine.detach().cpu().numpy())).to(self.router_bias.device)
         return destination
+
+    def take_routed(self):
+        """Pairs that this worker has routed to every expert in training since the last call, as a numpy array; starts
+        over.  (A block that recomputes its forward pass counts it twice, all experts alike.)"""
+        counts, self._routed = self._routed, None
+        return np.zeros(self.cfg.n_experts, dtype=np.int64) if counts is None else counts.cpu().numpy().astype(np.int64)
 
     def forward(self, x):
         cfg = self.cfg
@@ -149,7 +169,12 @@ class MoEFeedForward(torch.nn.Module):
         logits = self.router(x).reshape(T, -1)
         C = int(math.ceil(cfg.capacity_factor * T * k / E / 8.0) * 8)
         # softmax, top-k, renormalisation, slot assignment and the probability sums: one kernel
-        topw, prob_sum, ids, slot, counts = moe_ops.route(logits, E, k, C)
+        topw, prob_sum, ids, slot, counts = moe_ops.route(
+            logits, E, k, C, score=cfg.router_score, bias=self.router_bias, groups=cfg.router_groups,
+            top_groups=cfg.router_top_groups, group_score=cfg.router_group_score, renormalize=cfg.router_renormalize,
+            scale=cfg.router_scale)
+        if self.router_bias is not None and self.training:
+            self._routed = counts.long() if self._routed is None else self._routed + counts
         # load-balancing auxiliary loss (fraction routed x mean router probability)
         frac = counts.float() / float(T * k)
         self.aux_loss = E * (frac.detach() * (prob_sum / float(T))).sum()

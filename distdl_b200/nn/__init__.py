@@ -19,6 +19,7 @@ from .linear_ag_zero import DistributedLinearAllGatherZero  # noqa: F401,E402
 from .linear_rs import DistributedLinearReduceScatter  # noqa: F401,E402
 from .linear_rs_zero import DistributedLinearReduceScatterZero  # noqa: F401,E402
 from .rmsnorm_zero import DistributedRMSNormZero  # noqa: F401,E402
+from .qk_norm import DistributedQKNormRope  # noqa: F401,E402
 from . import loss  # noqa: F401,E402
 from .batchnorm import DistributedBatchNorm  # noqa: F401,E402
 from .conv_feature import (DistributedFeatureConv1d, DistributedFeatureConv2d, DistributedFeatureConv3d,  # noqa: F401,E402
@@ -56,7 +57,7 @@ __all__ = [
     "DistributedChannelAllGatherConvTranspose1d", "DistributedChannelAllGatherConvTranspose2d",
     "DistributedChannelAllGatherConvTranspose3d", "DistributedGeneralConv1d", "DistributedGeneralConv2d",
     "DistributedGeneralConv3d", "HaloExchange", "DistributedEmbeddingZero", "DistributedEmbedding",
-    "DistributedLayerNormZero", "DistributedLayerNorm", "DistributedRMSNormZero", "DistributedLinear",
+    "DistributedLayerNormZero", "DistributedLayerNorm", "DistributedRMSNormZero", "DistributedQKNormRope", "DistributedLinear",
     "DistributedLinearAllGather", "DistributedLinearAllGatherZero", "DistributedLinearReduceScatter",
     "DistributedLinearReduceScatterZero", "DistributedExpertAllGather", "DistributedExpertReduceScatter",
     "DistributedL1Loss", "DistributedMSELoss", "DistributedPoissonNLLLoss", "DistributedBCELoss",

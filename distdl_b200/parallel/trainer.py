@@ -117,7 +117,7 @@ class Trainer:
                                                            for k, v in vars(cfg).items()},
                         "files": [f"rank{r}.pt" for r in range(world)], "extra": extra or {}}
             with open(os.path.join(directory, "manifest.json"), "w") as fh:
-                json.dump(manifest, fh, indent=1)
+                json.dump(manifest, fh, indent=1, default=str)
         if dist.is_initialized() and world > 1:
             dist.barrier()
 
