@@ -13,15 +13,18 @@
 // one with none of them routes nowhere and adds nothing.  A NaN (softmax: also +inf) makes the weights of its token, its p and
 // its gradient NaN, and counts as the best, so that a token of NaN alone is not lost either.
 //
-// The choice is that of exact arithmetic.  Where it follows the logits (no bias, no sums) they are compared themselves.  Else
-// scores in 32 bits decide only where their distance is beyond their error; a token with a closer pair (some in a thousand)
-// is decided in 64 bits, so that neither the order of sums nor the fast exponential shows in the experts.
+// The choice is that of exact arithmetic.  Experts are compared as integers: 23 bits of value over 9 bits that favour the
+// lower number.  16-bit logits that decide themselves (no bias, no sums of scores) fit into them; everything else is cut to
+// steps of 2^-23 of the token's range, and where two neighbours of the order are closer than their errors (and not alike in
+// logit and bias) the token is decided in 64 bits: some in a thousand.  So neither the order of sums nor the fast
+// exponential shows in the experts.
 //
-// A warp works on a token, its lanes on C consecutive experts each; the k best are taken one by one with a warp-wide integer
-// maximum over order-preserving keys.  A latency below some thousand tokens, above them instructions (some 350 per token of
-// 256 experts) and the logits' bytes.  Slots follow in a second kernel (route_slot_kernel): a pair's slot is its rank in
-// pair order among the pairs of its expert, so nothing depends on how CTAs are scheduled; sums of p are formed per chunk
-// of tokens and then over the chunks, always in the same order.
+// A warp works on a token, its lanes on C consecutive experts each, which they sort; the k best are then the largest of the
+// lanes' first ones, k times, one warp-wide integer maximum each.  Some 500 instructions per token of 256 experts bound it
+// above some thousand tokens (with the experts unsorted and the winner's place looked for by ballot and shuffle 1 130 to
+// 1 920, 16384 tokens 34 to 66 us), a latency below.  Slots follow in a second kernel (route_slot_kernel): a pair's
+// slot is its rank in pair order among the pairs of its expert, so nothing depends on how CTAs are scheduled; sums of p are
+// formed per chunk of tokens and then over the chunks, always in the same order.
 #include "common.cuh"
 
 #include <cuda_fp16.h>
@@ -32,8 +35,14 @@ namespace {
 
 constexpr int kMaxExperts = 512, kMaxChoices = 32, kMaxGroups = 32;
 constexpr int kWarps = 8;
-constexpr int kRows = 32;                                     // tokens of a chunk (a CTA of the first kernel)
-constexpr int kSlotRows = 256, kSlotThreads = 1024;           // tokens and threads of a CTA of the second
+constexpr int kMostRows = 256;                                // tokens of a chunk (a CTA of the first kernel) at most
+constexpr int kSlotThreads = 1024;                            // of a CTA of the second kernel, which takes whole chunks
+
+// Tokens of a chunk: a token per warp while that gives every SM up to two CTAs, then so many that it still does.
+inline int rows_of(int tokens) {
+  const int per_warp = (tokens - 1) / (kWarps * 2 * 148) + 1;
+  return kWarps * (per_warp < kMostRows / kWarps ? per_warp : kMostRows / kWarps);
+}
 
 struct RouteArgs {
   const void* logits;       // [tokens, ld]
@@ -42,8 +51,9 @@ struct RouteArgs {
   float* w;                 // [tokens, k]
   int* hist;                // [chunks][E4]: pairs per expert
   float* psum;              // [chunks][E4]: sums of p
-  int ld, tokens, E, E4, k;
+  int ld, tokens, rows, E, E4, k;
   int groups, top_groups, size;                               // size: experts of a group
+  int lanes;                                                  // of a group, where it begins and ends with a lane's; else 0
   bool group_sum, sigmoid, renormalize, by_logit, vectors;
   float scale;
 };
@@ -72,16 +82,30 @@ __device__ __forceinline__ void load_row(const T* p, bool vectors, int left, flo
   }
 }
 
-// Order-preserving: a < b as floats, key(a) < key(b) as integers; 0 stands for "not to be chosen" (-inf, NaN).
-__device__ __forceinline__ unsigned key_of(float v) {
-  if (!(v > -INFINITY)) return 0u;
+// Order-preserving: a < b as floats, ordered(a) < ordered(b) as integers.
+__device__ __forceinline__ unsigned ordered(float v) {
   if (v == 0.f) v = 0.f;                                      // -0 is 0
   const unsigned u = __float_as_uint(v);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ float value_of(unsigned key) {
-  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+// Falling, by Batcher's odd-even merges.
+template <int C>
+__device__ __forceinline__ void sort_falling(unsigned (&key)[C]) {
+#pragma unroll
+  for (int p = 1; p < C; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int j = q % p; j + q < C; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < C && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const unsigned x = key[i + j], y = key[i + j + q];
+            key[i + j] = max(x, y);
+            key[i + j + q] = min(x, y);
+          }
 }
+__device__ __forceinline__ float warp_min(float v) { return -warp_max(-v); }
 
 __device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
@@ -115,6 +139,7 @@ __device__ __noinline__ int choose_in_64_bits(const RouteArgs& a, const float* l
   z = warp_sum_d(z);
   for (int j = 0; j < C; ++j) {
     if (!(l_in[j] > -INFINITY)) { c[j] = (bad >> j) & 1u ? INFINITY : -INFINITY; continue; }
+    if (a.by_logit) { c[j] = l_in[j]; continue; }
     if (!a.sigmoid) c[j] /= z;
     if (a.bias != nullptr) c[j] += (double)a.bias[first + j];
   }
@@ -213,6 +238,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const __grid_constan
   __syncthreads();
   const int first = lane * C;
   const int left = min(max(a.E - first, 0), C);               // experts of this lane
+  const bool exact = a.by_logit && sizeof(T) == 2;            // the logits fit into a key's value
   float bias[C];
 #pragma unroll
   for (int j = 0; j < C; ++j) bias[j] = a.bias != nullptr && j < left ? a.bias[first + j] : 0.f;
@@ -220,8 +246,8 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const __grid_constan
 #pragma unroll
   for (int j = 0; j < C; ++j) sums[j] = 0.f;
 
-  for (int row = warp; row < kRows; row += kWarps) {
-    const int t = blockIdx.x * kRows + row;
+  for (int row = warp; row < a.rows; row += kWarps) {
+    const int t = blockIdx.x * a.rows + row;
     if (t >= a.tokens) break;
     const T* from = reinterpret_cast<const T*>(a.logits) + (size_t)t * a.ld;
     float l[C];
@@ -230,103 +256,126 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const __grid_constan
     const bool nan = take_bad<C>(l, a.sigmoid, bad);
     Scores<C> s;
     s.set(l, a.sigmoid);
-    unsigned key[C];
-    float near = 0.f;                                         // distances up to here (and 4e-7 of the value) are within errors
-    if (a.by_logit) {
+    unsigned key[C];                                          // value << 9 | 511 - expert; 0: not to be chosen
+    int near = 0;                                             // differences of values up to here say nothing
+    if (exact) {
 #pragma unroll
-      for (int j = 0; j < C; ++j) key[j] = j < left ? key_of(l[j]) : 0u;
+      for (int j = 0; j < C; ++j) key[j] = l[j] > -INFINITY ? (ordered(l[j]) & ~511u) | (511 - first - j) : 0u;
     } else {
-      // sigmoid: 4e-7 off at most (its slope times the exponential's error, a division); softmax: 4e-6 of the largest
-      const float back = a.sigmoid ? __expf(fminf(s.top, 0.f)) : s.inv;
-      near = a.sigmoid ? 2e-6f : 8e-6f * s.inv;
+      float v[C], hi = -INFINITY, lo = INFINITY;
+      const float back = a.by_logit ? 0.f : a.sigmoid ? __expf(fminf(s.top, 0.f)) : s.inv;
 #pragma unroll
-      for (int j = 0; j < C; ++j) key[j] = j < left && l[j] > -INFINITY ? key_of(s.part[j] * back + bias[j]) : 0u;
+      for (int j = 0; j < C; ++j) {
+        v[j] = a.by_logit ? l[j] : s.part[j] * back + bias[j];
+        if (l[j] > -INFINITY) { hi = fmaxf(hi, v[j]); lo = fminf(lo, v[j]); }
+      }
+      hi = warp_max(hi);
+      lo = warp_min(lo);
+      const float range = hi - lo, steps = range > 1e-25f && range < 1e38f ? __fdividef(8388600.f, range) : 0.f;
+      // scores: sigmoid 4e-7 off at most (its slope times the exponential's error, a division), softmax 4e-6 of the largest,
+      // the bias's addition; the cut itself: a step each way
+      const float off = a.by_logit ? 0.f : (a.sigmoid ? 2e-6f : 8e-6f * s.inv) + 4e-7f * fmaxf(fabsf(hi), fabsf(lo));
+      near = (int)fminf(off * steps + 3.f, 8388607.f);
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+        key[j] = l[j] > -INFINITY ? (unsigned)((int)((v[j] - lo) * steps) + 1) << 9 | (511 - first - j) : 0u;
     }
-    bool close = false;
     if (nan) {
 #pragma unroll
       for (int j = 0; j < C; ++j)
-        if ((bad >> j) & 1u) key[j] = 0xffffffffu;
+        if ((bad >> j) & 1u) key[j] = 0xfffffe00u | (511 - first - j);
     }
+    bool close = false;
     if (a.groups > 1) {
-      // value of every group, by lane g; through shared memory, where a group may begin and end at any lane
-#pragma unroll
-      for (int j = 0; j < C; ++j)
-        if (j < left) s_row[warp][first + j] = key[j] ? ((bad >> j) & 1u ? INFINITY : value_of(key[j])) : -INFINITY;
-      __syncwarp();
-      float value = -INFINITY;
-      // (lanes that share a group's scan: as many as there are for every group)
-      const int share = a.groups > 16 ? 1 : a.groups > 8 ? 2 : a.groups > 4 ? 4 : a.groups > 2 ? 8 : 16;
-      {
-        const int g = lane / share;
-        float b0 = -INFINITY, b1 = -INFINITY;
-        if (g < a.groups)
-          for (int i = lane % share; i < a.size; i += share) {
-            const float v = s_row[warp][g * a.size + i];
-            b1 = fmaxf(b1, fminf(b0, v));
-            b0 = fmaxf(b0, v);
-          }
-        for (int o = share >> 1; o > 0; o >>= 1) {
-          const float o0 = __shfl_xor_sync(0xffffffffu, b0, o), o1 = __shfl_xor_sync(0xffffffffu, b1, o);
-          b1 = fmaxf(fmaxf(b1, o1), fminf(b0, o0));
-          b0 = fmaxf(b0, o0);
+      int value = 0, g = a.groups;                            // of this lane's group; 0: none of its experts may be chosen
+      bool single = false;                                    // sums: with one expert only, which needs its score itself
+      int step;                                               // the groups' values are those of every step-th lane
+      if (a.lanes > 0) {
+        sort_falling<C>(key);
+        int b0 = (int)(key[0] >> 9), b1 = C > 1 ? (int)(key[C > 1] >> 9) : 0;
+        for (int o = 1; o < a.lanes; o <<= 1) {
+          const int o0 = __shfl_xor_sync(0xffffffffu, b0, o), o1 = __shfl_xor_sync(0xffffffffu, b1, o);
+          b1 = max(max(b1, o1), min(b0, o0));
+          b0 = max(b0, o0);
         }
-        const float v = a.group_sum && b1 > -INFINITY ? b0 + b1 : b0;
-        value = __shfl_sync(0xffffffffu, v, min(lane * share, 31));
-        if (lane >= a.groups) value = -INFINITY;
-      }
-      __syncwarp();
-      int place = 0;
-      for (int g = 0; g < a.groups; ++g) {
-        const float v = __shfl_sync(0xffffffffu, value, g);
-        place += v > value || (v == value && g < lane);
-      }
-      const bool in = lane < a.groups && place < a.top_groups;
-      const unsigned kept = __ballot_sync(0xffffffffu, in);
-      if (!a.by_logit && a.top_groups < a.groups) {
-        const float least = -warp_max(in ? -value : -INFINITY), most = warp_max(!in ? value : -INFINITY);
-        close = least - most <= 2.f * near + 4e-7f * fmaxf(fabsf(least), fabsf(most));
-      }
-      int g = first / a.size, at = first - g * a.size;
-#pragma unroll
-      for (int j = 0; j < C; ++j) {
-        if (!((kept >> (g & 31)) & 1u)) key[j] = 0u;
-        if (++at == a.size) { at = 0; ++g; }
-      }
-    }
-    // the k best one by one: lane i keeps the i-th
-    int chosen = -1, was = -1;
-    unsigned best = 0u, was_key = 0u;
-#pragma unroll
-    for (int j = 0; j < C; ++j) best = max(best, key[j]);
-    const int rounds = a.k + (a.by_logit ? 0 : 1);            // (one more: the first that is left out must not be close)
-    for (int i = 0; i < rounds; ++i) {
-      const unsigned top = __reduce_max_sync(0xffffffffu, best);
-      if (top == 0u) break;
-      const int owner = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
-      int e = 0;
-#pragma unroll
-      for (int j = C - 1; j >= 0; --j) e = key[j] == top ? first + j : e;
-      e = __shfl_sync(0xffffffffu, e, owner);
-      if (!a.by_logit && i > 0) {
-        const float hi = value_of(was_key), lo = value_of(top);
-        if (hi - lo <= near + 4e-7f * fmaxf(fabsf(hi), fabsf(lo))) {
-          // two alike in logit and bias are alike, and in order
-          close |= to_f(from[was]) != to_f(from[e]) || (a.bias != nullptr && a.bias[was] != a.bias[e]);
-        }
-        was_key = top;
+        step = a.lanes;
+        g = lane / a.lanes;
+        value = a.group_sum ? b0 + b1 : b0;
+        single = b0 > 0 && b1 == 0;
       } else {
-        was_key = top;
+        // a group begins and ends at any expert: through shared memory, a lane or several for every group's scan
+        int* values = reinterpret_cast<int*>(s_row[warp]);
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+          if (j < left) values[first + j] = (int)(key[j] >> 9);
+        __syncwarp();
+        step = a.groups > 16 ? 1 : a.groups > 8 ? 2 : a.groups > 4 ? 4 : a.groups > 2 ? 8 : 16;
+        g = lane / step;
+        int b0 = 0, b1 = 0;
+        if (g < a.groups)
+          for (int i = lane % step; i < a.size; i += step) {
+            const int v = values[g * a.size + i];
+            b1 = max(b1, min(b0, v));
+            b0 = max(b0, v);
+          }
+        for (int o = 1; o < step; o <<= 1) {
+          const int o0 = __shfl_xor_sync(0xffffffffu, b0, o), o1 = __shfl_xor_sync(0xffffffffu, b1, o);
+          b1 = max(max(b1, o1), min(b0, o0));
+          b0 = max(b0, o0);
+        }
+        value = a.group_sum ? b0 + b1 : b0;
+        single = b0 > 0 && b1 == 0;
+        __syncwarp();
       }
-      was = e;
-      if (lane == i && i < a.k) chosen = e;
-      if (lane == owner) {
-        best = 0u;
+      int place = 0;
+      for (int i = 0; i < a.groups; ++i) {
+        const int v = __shfl_sync(0xffffffffu, value, i * step);
+        place += v > value || (v == value && i < g);
+      }
+      const bool in = g < a.groups && place < a.top_groups;
+      if (!exact) {
+        const int least = (int)__reduce_min_sync(0xffffffffu, in ? (unsigned)value : 0x7fffffffu);
+        const int most = (int)__reduce_max_sync(0xffffffffu, !in && g < a.groups ? (unsigned)value : 0u);
+        close = most > 0 && least - most <= (a.group_sum ? 2 * near : near);
+        if (a.group_sum && a.size > 1) close |= __any_sync(0xffffffffu, g < a.groups && single);
+      }
+      if (a.lanes > 0) {
+        if (!in) {
+#pragma unroll
+          for (int j = 0; j < C; ++j) key[j] = 0u;
+        }
+      } else {
+        const unsigned kept = __ballot_sync(0xffffffffu, in);
+        int of = first / a.size, at = first - of * a.size;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-          if (first + j == e) key[j] = 0u;
-          best = max(best, key[j]);
+          if (j >= left || !((kept >> (of * step)) & 1u)) key[j] = 0u;
+          if (++at == a.size) { at = 0; ++of; }
         }
+        sort_falling<C>(key);
+      }
+    } else {
+      sort_falling<C>(key);
+    }
+    // the k best one by one: lane i keeps the i-th
+    int chosen = -1;
+    unsigned was = 0u;
+    const int rounds = a.k + (exact ? 0 : 1);                 // (one more: the first that is left out must not be close)
+    for (int i = 0; i < rounds; ++i) {
+      const unsigned top = __reduce_max_sync(0xffffffffu, key[0]);
+      if (top == 0u) break;
+      const int e = 511 - (int)(top & 511u);
+      if (!exact && i > 0 && (int)(was >> 9) - (int)(top >> 9) <= near) {
+        // two alike in logit and bias are alike, and in order
+        const int f = 511 - (int)(was & 511u);
+        close |= to_f(from[f]) != to_f(from[e]) || (a.bias != nullptr && a.bias[f] != a.bias[e]);
+      }
+      was = top;
+      if (lane == i && i < a.k) chosen = e;
+      if (key[0] == top) {
+#pragma unroll
+        for (int j = 0; j + 1 < C; ++j) key[j] = key[j + 1];
+        key[C - 1] = 0u;
       }
     }
     if (close) {                                              // (the same on every lane)
@@ -378,19 +427,18 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const __grid_constan
 // histograms), words of 32 tokens before, lower bits in the word.
 __global__ void __launch_bounds__(kSlotThreads)
 route_slot_kernel(const int* __restrict__ ids, int tokens, int k, int E, int E4, int capacity, const int* __restrict__ hist,
-                  const float* __restrict__ psum, int chunks, int* __restrict__ counts, float* __restrict__ prob_sum,
-                  int* __restrict__ slot) {
-  constexpr int W = kSlotRows / 32;
+                  const float* __restrict__ psum, int chunks, int chunk, int per_cta, int* __restrict__ counts,
+                  float* __restrict__ prob_sum, int* __restrict__ slot) {
+  constexpr int W = kMostRows / 32;
   __shared__ unsigned s_mask[W][kMaxExperts];
   __shared__ __align__(16) int s_part[kSlotThreads * 4];      // sums before this CTA; then [W][kMaxExperts] bases
   grid_dependency_launch();
   const int tid = threadIdx.x, lane = tid & 31;
   for (int i = tid; i < W * kMaxExperts; i += kSlotThreads) (&s_mask[0][0])[i] = 0u;
   const int quads = E4 / 4, lanes = kSlotThreads / quads;     // threads per four experts
-  const int t0 = blockIdx.x * kSlotRows;
+  const int before = blockIdx.x * per_cta, t0 = before * chunk;          // chunks and tokens before this CTA's
   {
     const int q = tid % quads, r0 = tid / quads;
-    const int before = min(t0 / kRows, chunks);
     int4 sum = make_int4(0, 0, 0, 0);
     if (r0 < lanes) {
 #pragma unroll 8
@@ -402,14 +450,14 @@ route_slot_kernel(const int* __restrict__ ids, int tokens, int k, int E, int E4,
     }
   }
   __syncthreads();
-  const int pairs = min(tokens - t0, kSlotRows) * k;
+  const int pairs = min(tokens - t0, per_cta * chunk) * k;
   for (int p = tid; p < pairs; p += kSlotThreads) {
     const int e = ids[(size_t)t0 * k + p];
     if (e >= 0 && e < E) atomicOr(&s_mask[(p / k) >> 5][e], 1u << ((p / k) & 31));
   }
   int run = 0;
   if (tid < E)
-    for (int r = 0; r < min(lanes, t0 / kRows); ++r) run += s_part[r * E4 + tid];
+    for (int r = 0; r < min(lanes, before); ++r) run += s_part[r * E4 + tid];
   __syncthreads();
   if (tid < E) {
     for (int w = 0; w < W; ++w) {
@@ -508,6 +556,7 @@ bool fill(RouteArgs& a, const void* logits, int ld, int size, int tokens, int E,
   a.ld = ld; a.tokens = tokens; a.E = E; a.k = k;
   a.E4 = (E + 3) / 4 * 4;
   a.sigmoid = sigmoid != 0; a.renormalize = renormalize != 0; a.scale = scale;
+  a.rows = rows_of(tokens);
   int C = 1;
   while (32 * C < E) C *= 2;
   *c = C;
@@ -542,8 +591,14 @@ int backward(const RouteArgs& a, int C, const float* dw, const float* dprob, voi
 
 }  // namespace
 
+// Words of scratch of dd_route_fwd (a multiple of 4).
+DD_API int dd_route_words(int tokens, int E) {
+  if (tokens < 1 || E < 1 || E > kMaxExperts) return 0;
+  return 2 * ((tokens - 1) / rows_of(tokens) + 1) * ((E + 3) / 4 * 4);
+}
+
 // logits [tokens, ld], the first E columns (dtype 0 bf16, 1 fp16, 2 fp32); bias [E] fp32 or null; ids, w, slot [tokens * k];
-// counts, prob_sum [E]; scratch: `words` words, 16-byte aligned, two for every expert (in fours) and 32 tokens.
+// counts, prob_sum [E]; scratch: `words` words, dd_route_words or more, 16-byte aligned.
 DD_API int dd_route_fwd(const void* logits, int ld, int dtype, int tokens, int E, int k, int capacity, const float* bias,
                         int groups, int top_groups, int group_sum, int sigmoid, int renormalize, float scale, int* ids,
                         float* w, int* slot, int* counts, float* prob_sum, int* scratch, long long words,
@@ -556,12 +611,14 @@ DD_API int dd_route_fwd(const void* logits, int ld, int dtype, int tokens, int E
   if (ids == nullptr || w == nullptr || slot == nullptr || counts == nullptr || prob_sum == nullptr || scratch == nullptr)
     return DD_ERR_BAD_ARG;
   if (reinterpret_cast<uintptr_t>(scratch) % 16 != 0) return DD_ERR_ALIGN;
-  const int chunks = (tokens + kRows - 1) / kRows;
+  const int chunks = (tokens - 1) / a.rows + 1;
   if (words < 2LL * chunks * a.E4) return DD_ERR_BAD_ARG;
   a.bias = bias;
   a.groups = top_groups == groups ? 1 : groups;               // (all groups: no choice among them)
   a.top_groups = top_groups; a.size = E / groups; a.group_sum = group_sum != 0;
   a.by_logit = bias == nullptr && !(a.groups > 1 && a.group_sum && a.size > 1);
+  const int lanes = a.size / C;
+  a.lanes = a.size % C == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
   a.ids = ids; a.w = w;
   a.hist = scratch;
   a.psum = reinterpret_cast<float*>(scratch + (size_t)chunks * a.E4);
@@ -570,8 +627,9 @@ DD_API int dd_route_fwd(const void* logits, int ld, int dtype, int tokens, int E
                 : dtype == 1 ? forward<__half>(a, C, chunks, s)
                              : forward<float>(a, C, chunks, s);
   if (e) return e;
-  route_slot_kernel<<<(tokens + kSlotRows - 1) / kSlotRows, kSlotThreads, 0, s>>>(ids, tokens, k, E, a.E4, capacity, a.hist,
-                                                                                 a.psum, chunks, counts, prob_sum, slot);
+  const int per_cta = kMostRows / a.rows;
+  route_slot_kernel<<<(chunks - 1) / per_cta + 1, kSlotThreads, 0, s>>>(ids, tokens, k, E, a.E4, capacity, a.hist, a.psum, chunks,
+                                                                       a.rows, per_cta, counts, prob_sum, slot);
   return (int)cudaGetLastError();
 }
 

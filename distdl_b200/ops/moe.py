@@ -68,6 +68,7 @@ class _RouterFn(torch.autograd.Function):
         return dlogits, None, None, None
 
 
+_native.declare("dd_route_words", [_i, _i])
 _native.declare("dd_route_fwd", [_v, _i, _i, _i, _i, _i, _i, _v, _i, _i, _i, _i, _i, _f, _v, _v, _v, _v, _v, _v,
                                  ctypes.c_longlong, _v])
 _native.declare("dd_route_bwd", [_v, _i, _i, _i, _i, _i, _i, _i, _f, _v, _v, _v, _v, _v, _v])
@@ -79,12 +80,13 @@ def _route_forward(logits, E, k, capacity, how):
     score, bias, groups, top_groups, group_score, renormalize, scale = how
     T, ld = logits.shape
     dev = logits.device
+    # (pieces of their own: whoever changes one of them in place must not seem to change what the backward pass has kept)
     ids = torch.empty(T * k, dtype=torch.int32, device=dev)
-    slot = torch.empty(T * k, dtype=torch.int32, device=dev)
+    slot = torch.empty_like(ids)
     counts = torch.empty(E, dtype=torch.int32, device=dev)
     w = torch.empty(T, k, dtype=torch.float32, device=dev)
     prob_sum = torch.empty(E, dtype=torch.float32, device=dev)
-    words = 2 * ((T + 31) // 32) * ((E + 3) // 4 * 4)
+    words = _native.lib().dd_route_words(T, E)
     scratch = torch.empty(words, dtype=torch.int32, device=dev)
     call_on(logits, "dd_route_fwd", logits.data_ptr(), ld, _DTYPE[logits.dtype], T, E, k, capacity, ptr(bias), groups,
             top_groups, int(group_score == "top2"), int(score == "sigmoid"), int(renormalize), scale, ids.data_ptr(),

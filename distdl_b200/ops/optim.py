@@ -85,25 +85,24 @@ def _dense(t: torch.Tensor) -> bool:
 
 
 def _tensors(tensors):
-    """(addresses, sizes, type codes) as C arrays and their number, the tensors' device, and whether the kernels take them
-    (CUDA, bf16 / fp16 / fp32, dense, all on one device)."""
+    """(addresses, sizes, type codes) of the tensors as C arrays, or None where the kernels do not take them (CUDA, bf16 /
+    fp16 / fp32, dense)."""
     device = tensors[0].device
-    native = use_native(tensors[0])
-    for t in tensors:
-        if t.device != device:
-            raise ValueError(f"gradients on {device} and on {t.device}: a norm is of one device's tensors")
-        if t.layout is not torch.strided:
-            raise ValueError(f"gradients are dense tensors, not {t.layout}")
-        if t.dtype not in _CODES:
+    where = device.index if device.type == "cuda" else -1
+    if any([t.get_device() != where for t in tensors]):
+        raise ValueError(f"gradients on {device} and elsewhere: a norm is of one device's tensors")
+    if any([t.layout is not torch.strided for t in tensors]):
+        raise ValueError("gradients are dense tensors")
+    codes = [_CODES.get(t.dtype, 9) for t in tensors]
+    if 9 in codes:
+        for t in tensors:
             if not t.is_floating_point():
                 raise ValueError(f"gradients are floating-point tensors, not {t.dtype}")
-            native = False
-        elif native and not t.is_contiguous() and not _dense(t):
-            native = False
-    if not native:
+        return None
+    if not use_native(tensors[0]) or not all([t.is_contiguous() or _dense(t) for t in tensors]):
         return None
     return (array.array("Q", [t.data_ptr() for t in tensors]), array.array("q", [t.numel() for t in tensors]),
-            array.array("B", [_CODES[t.dtype] for t in tensors]))
+            array.array("B", codes))
 
 
 def _flat(tensors):
@@ -130,7 +129,6 @@ def _grad_norm(tensors, lists, norm, squared, max_norm, given, clip):
             int(given), int(clip))
 
 
-@torch.no_grad()
 def grad_norm(tensors, squared: bool = False) -> torch.Tensor:
     """The 2-norm of all elements of ``tensors`` (one tensor, or an iterable; None is passed over) as an fp32 scalar on their
     device, or with ``squared`` the sum of squares in fp64 (to be added over workers).  Squares and sums are formed in 64
@@ -147,7 +145,6 @@ def grad_norm(tensors, squared: bool = False) -> torch.Tensor:
     return out
 
 
-@torch.no_grad()
 def clip_grad_norm_(tensors, max_norm: float, norm: torch.Tensor = None) -> torch.Tensor:
     """Scales gradients in place by ``min(1, max_norm / (norm + 1e-6))``, ``norm`` being their 2-norm, which is returned (an
     fp32 scalar on their device; nothing waits for it).  ``tensors``: gradients, or parameters (whose ``.grad`` is meant:
@@ -167,14 +164,17 @@ def clip_grad_norm_(tensors, max_norm: float, norm: torch.Tensor = None) -> torc
         raise ValueError(f"the norm is on {norm.device}, the gradients on {tensors[0].device}")
     lists = _tensors(tensors)
     if lists is None:
-        norm = _plain_sumsq(tensors).sqrt().float() if norm is None else norm
-        scale = (max_norm / (norm + 1e-6)).clamp(max=1.0).reshape(())
-        for t in tensors:
-            t.copy_(t * scale if t.dtype == torch.float64 else t.float() * scale)
+        with torch.no_grad():
+            norm = _plain_sumsq(tensors).sqrt().float() if norm is None else norm
+            scale = (max_norm / (norm + 1e-6)).clamp(max=1.0).reshape(())
+            for t in tensors:
+                t.copy_(t * scale if t.dtype == torch.float64 else t.float() * scale)
         return norm
     given = norm is not None
     if not given:
         norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
     _grad_norm(tensors, lists, norm, None, max_norm, given, True)
-    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    if any([t.is_inference() for t in tensors]):
+        tensors = [t for t in tensors if not t.is_inference()]
+    torch.autograd.graph.increment_version(tensors)
     return norm

@@ -5,7 +5,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, fields
 from typing import Optional
 
 import torch
@@ -85,6 +85,25 @@ class Rotary:
             raise ValueError("scaling 'ntk' needs more than one pair")
         return dim
 
+    def _plan(self, head_dim: int):
+        """(components that turn, neighbours?, address of the frequencies in turns per position, what multiplies) for the
+        kernels, kept with the settings (the array that holds the frequencies as its last entry)."""
+        plans = self.__dict__.get("_plans")
+        if plans is None:
+            plans = self.__dict__["_plans"] = {}
+        plan = plans.get(head_dim)
+        if plan is None:
+            dim = self.rotated(head_dim)
+            arr = (ctypes.c_double * max(1, dim // 2))(*(f / (2 * math.pi) for f in _frequencies(self, dim)))
+            plan = plans[head_dim] = (dim, int(self.interleaved), ctypes.addressof(arr), self.scale, arr)
+        return plan
+
+    def __getstate__(self):                 # (copies and pickles hold the settings; addresses are this process's)
+        return {f.name: getattr(self, f.name) for f in fields(self)}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+
     @property
     def scale(self) -> float:
         """What multiplies the turned components."""
@@ -119,14 +138,6 @@ def _frequencies(rotary: Rotary, dim: int) -> tuple:
             f = (1.0 - slowed) * f + slowed * f / factor
         out.append(f)
     return tuple(out)
-
-
-@functools.lru_cache(maxsize=256)
-def _turns(rotary: Rotary, head_dim: int):
-    """(components that turn, frequencies in turns per position as a C array, its address)."""
-    dim = rotary.rotated(head_dim)
-    arr = (ctypes.c_double * max(1, dim // 2))(*(f / (2 * math.pi) for f in _frequencies(rotary, dim)))
-    return dim, arr, ctypes.addressof(arr)
 
 
 _range_positions = {}
@@ -168,9 +179,8 @@ def _where(qkv, rotary, seq, offset, ranges, positions):
     if n != tokens and n != seq or (n == 0 and tokens) or (n and tokens % n):
         raise ValueError(f"{n} positions for {tokens} tokens in sequences of {seq}: one per token, or one per place in a "
                          f"sequence")
-    positions = positions.reshape(-1)
-    if not positions.is_contiguous():
-        positions = positions.contiguous()
+    if positions.dim() != 1 or not positions.is_contiguous():
+        positions = positions.reshape(-1).contiguous()
     return rotary, positions, max(1, n), 0
 
 
@@ -198,9 +208,10 @@ def _wide(x):
     return x if x.dtype == torch.float64 else x.float()
 
 
-def _plain_rope(qkv, nheads, where):
+def _plain_rope(qkv, nheads, where, sign=1.0):
     rotary, positions, seq, offset = where
     cos, sin = _angles(qkv, rotary, positions, seq, offset)
+    sin = sign * sin
     y = _rotated(_wide(qkv[:, :nheads]), cos, sin, rotary.rotated(qkv.shape[2]), rotary.interleaved)
     return torch.cat([y.to(qkv.dtype), qkv[:, nheads:]], dim=1)
 
@@ -215,16 +226,16 @@ def _unit(t):
 
 
 def _heads(t):
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    stride = t.stride()
+    return t.data_ptr(), stride[0], stride[1]
 
 
 def _turn_args(where, head_dim):
     rotary, positions, seq, offset = where
     if rotary is None:
         return (0, 0, 0, 1.0), (0, 0, 0, 1)
-    dim, _arr, address = _turns(rotary, head_dim)
-    wide = positions is not None and positions.dtype == torch.int64
-    return (dim, int(rotary.interleaved), address, rotary.scale), (ptr(positions), int(wide), offset, seq)
+    place = (0, 0, offset, seq) if positions is None else (positions.data_ptr(), int(positions.dtype == torch.int64), 0, seq)
+    return rotary._plan(head_dim)[:4], place
 
 
 def _rotate(src, dst, nheads, where, sign):
@@ -234,23 +245,36 @@ def _rotate(src, dst, nheads, where, sign):
             *place, _DTYPE[src.dtype])
 
 
+def _rotated_copy(qkv, nheads, where, sign):
+    src = _unit(qkv)
+    out = torch.empty_like(src, memory_format=torch.contiguous_format)
+    _rotate(src, out, nheads, where, sign)
+    return out
+
+
 class _RopeFn(torch.autograd.Function):
     """The rotation into a new tensor; its gradient is the rotation backwards, a call of the same function."""
 
     @staticmethod
-    def forward(ctx, qkv, nheads, rotary, positions, seq, offset, sign):
-        ctx.save_for_backward(positions)
-        ctx.cfg = (nheads, rotary, seq, offset, sign)
-        src = _unit(qkv)
-        out = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        _rotate(src, out, nheads, (rotary, positions, seq, offset), sign)
-        return out
+    def forward(ctx, qkv, cfg):
+        nheads, where, sign = cfg
+        ctx.save_for_backward(where[1])
+        ctx.cfg = cfg
+        return _rotated_copy(qkv, nheads, where, sign)
 
     @staticmethod
     def backward(ctx, d):
-        nheads, rotary, seq, offset, sign = ctx.cfg
-        (positions,) = ctx.saved_tensors
-        return _RopeFn.apply(d, nheads, rotary, positions, seq, offset, -sign), None, None, None, None, None, None
+        nheads, where, sign = ctx.cfg
+        return _turned_back(ctx, d, nheads, where, -sign), None
+
+
+def _turned_back(ctx, d, nheads, where, sign):
+    where = (where[0], ctx.saved_tensors[0], *where[2:])
+    if not _plain(d):                       # under a function transform: elementary operations
+        return _plain_rope(d, nheads, where, sign)
+    if torch.is_grad_enabled():             # differentiated itself
+        return _RopeFn.apply(d, (nheads, where, sign))
+    return _rotated_copy(d, nheads, where, sign)
 
 
 class _RopeInPlaceFn(torch.autograd.Function):
@@ -258,20 +282,19 @@ class _RopeInPlaceFn(torch.autograd.Function):
     into a new tensor: the incoming one may be the caller's own.)"""
 
     @staticmethod
-    def forward(ctx, qkv, layout, nheads, rotary, positions, seq, offset):
+    def forward(ctx, qkv, cfg):
+        layout, nheads, where = cfg
         ctx.mark_dirty(qkv)
-        ctx.save_for_backward(positions)
-        ctx.cfg = (layout, nheads, rotary, seq, offset)
+        ctx.save_for_backward(where[1])
+        ctx.cfg = cfg
         t = qkv.view(layout)
-        _rotate(t, t, nheads, (rotary, positions, seq, offset), 1.0)
+        _rotate(t, t, nheads, where, 1.0)
         return qkv
 
     @staticmethod
     def backward(ctx, d):
-        layout, nheads, rotary, seq, offset = ctx.cfg
-        (positions,) = ctx.saved_tensors
-        g = _RopeFn.apply(d.reshape(layout), nheads, rotary, positions, seq, offset, -1.0)
-        return g.reshape(d.shape), None, None, None, None, None, None
+        layout, nheads, where = ctx.cfg
+        return _turned_back(ctx, d.reshape(layout), nheads, where, -1.0).reshape(d.shape), None
 
 
 def _check_heads(qkv, nheads):
@@ -284,6 +307,8 @@ def _check_heads(qkv, nheads):
 
 def _overlaps(t):
     """Whether elements of ``t [tokens, heads, head_dim]`` may share memory (as those of an expanded tensor do)."""
+    if t.is_contiguous():
+        return False
     need = 1
     for stride, n in sorted(zip(t.stride(), t.shape)):
         if n > 1:
@@ -307,31 +332,43 @@ def rope(qkv: torch.Tensor, seq: int, nheads: int, *, rotary: Rotary, offset: in
     if rotary is None:
         raise ValueError("rope needs a Rotary")
     where = _where(qkv, rotary, seq, offset, ranges, positions)
-    rotary.rotated(qkv.shape[2])
-    if _native_ok(qkv):
-        return _RopeFn.apply(qkv, nheads, *where, 1.0)
-    return _plain_rope(qkv, nheads, where)
+    rotary._plan(qkv.shape[2])
+    if not _native_ok(qkv):
+        return _plain_rope(qkv, nheads, where)
+    if qkv.requires_grad and torch.is_grad_enabled():
+        return _RopeFn.apply(qkv, (nheads, where, 1.0))
+    return _rotated_copy(qkv, nheads, where, 1.0)
 
 
 def rope_in_place(qkv, seq, nheads, rotary, offset=0, ranges=None, positions=None, layout=None):
     """:func:`distdl_b200.ops.rope_` with a :class:`Rotary`."""
-    shape = tuple(qkv.shape) if layout is None else tuple(int(v) for v in layout)
-    if layout is not None and qkv.numel() != math.prod(shape):
-        raise ValueError(f"a tensor {tuple(qkv.shape)} cannot be read as {shape}")
-    try:
-        t = qkv.detach().view(shape)
-    except RuntimeError:                    # its strides do not allow it
-        t = None
-    read = qkv.detach().reshape(shape) if t is None else t
+    if layout is None:
+        shape, read = tuple(qkv.shape), qkv
+    else:
+        shape = tuple(int(v) for v in layout)
+        if qkv.numel() != math.prod(shape):
+            raise ValueError(f"a tensor {tuple(qkv.shape)} cannot be read as {shape}")
+        try:
+            read = qkv.detach().view(shape)
+        except RuntimeError:                # its strides do not allow it
+            read = None
+    held = read is not None                 # in memory as it is read
+    if not held:
+        read = qkv.detach().reshape(shape)
     _check_heads(read, nheads)
     where = _where(read, rotary, seq, offset, ranges, positions)
-    rotary.rotated(shape[2])
+    rotary._plan(shape[2])
     if not _native_ok(read):
         return _plain_rope(qkv.reshape(shape), nheads, where).reshape(qkv.shape)
-    if t is None or _overlaps(t) or (t.stride(2) != 1 and shape[2] > 1):
+    if not held or _overlaps(read) or (read.stride(2) != 1 and shape[2] > 1):
         raise ValueError("a tensor that is turned in place must have its heads' components next to one another in memory "
                          "of their own: use ops.rope")
-    return _RopeInPlaceFn.apply(qkv, shape, nheads, *where)
+    if qkv.requires_grad and torch.is_grad_enabled():
+        return _RopeInPlaceFn.apply(qkv, (shape, nheads, where))
+    _rotate(read, read, nheads, where, 1.0)
+    if not qkv.is_inference():
+        torch.autograd.graph.increment_version(qkv)
+    return qkv
 
 
 # ------------------------------------------------------------------------------- norm of the heads and rotation
@@ -355,9 +392,17 @@ def _plain_qk_norm_rope(qkv, hq, hkv, wq, wk, eps, where):
 def _norm_forward(src, dst, hq, hkv, wq, wk, eps, where):
     tokens, heads, hd = src.shape
     (dim, near, address, scale), place = _turn_args(where, hd)
-    wide = (wq if wq is not None else wk) is not None and (wq if wq is not None else wk).dtype == torch.float32
-    call_on(src, "dd_norm_heads_fwd", *_heads(src), *_heads(dst), ptr(wq), ptr(wk), int(wide), eps, tokens, hq, hkv,
-            heads - hq - hkv, hd, dim, near, address, scale, *place, _DTYPE[src.dtype])
+    w = wk if wq is None else wq
+    call_on(src, "dd_norm_heads_fwd", *_heads(src), *_heads(dst), ptr(wq), ptr(wk),
+            int(w is not None and w.dtype == torch.float32), eps, tokens, hq, hkv, heads - hq - hkv, hd, dim, near, address,
+            scale, *place, _DTYPE[src.dtype])
+
+
+def _normed_copy(qkv, hq, hkv, wq, wk, eps, where):
+    src = _unit(qkv)
+    out = torch.empty_like(src, memory_format=torch.contiguous_format)
+    _norm_forward(src, out, hq, hkv, wq, wk, eps, where)
+    return out
 
 
 @functools.lru_cache(maxsize=64)
@@ -371,15 +416,15 @@ def _norm_backward(x, dy, wq, wk, hq, hkv, eps, where, want, main=(None, None)):
     """(dx, dwq, dwk) of :func:`qk_norm_rope`; ``want``: which weights' gradients; ``main``: fp32 accumulators that they are
     added to instead (both that are wanted, or neither)."""
     tokens, heads, hd = x.shape
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    w = wq if wq is not None else wk
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    w = wk if wq is None else wq
     accumulate = main[0] is not None or main[1] is not None
     dwq, dwk, partial = main[0], main[1], None
     if want[0] or want[1]:
         partial = torch.empty(_parts(x.get_device()) * 2 * hd, dtype=torch.float32, device=x.device)
         if not accumulate:
-            dwq = torch.empty(hd, dtype=w.dtype, device=x.device) if want[0] else None
-            dwk = torch.empty(hd, dtype=w.dtype, device=x.device) if want[1] else None
+            dwq = torch.empty_like(wq) if want[0] else None
+            dwk = torch.empty_like(wk) if want[1] else None
     (dim, near, address, scale), place = _turn_args(where, hd)
     call_on(x, "dd_norm_heads_bwd", *_heads(x), *_heads(dy), *_heads(dx), ptr(wq), ptr(wk),
             int(w is not None and w.dtype == torch.float32), eps, ptr(dwq), ptr(dwk), int(accumulate), ptr(partial), tokens, hq,
@@ -389,19 +434,18 @@ def _norm_backward(x, dy, wq, wk, hq, hkv, eps, where, want, main=(None, None)):
 
 class _QKNormRopeFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, wq, wk, hq, hkv, eps, rotary, positions, seq, offset):
-        out = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        _norm_forward(_unit(qkv), out, hq, hkv, wq, wk, eps, (rotary, positions, seq, offset))
-        ctx.save_for_backward(qkv, wq, wk, positions)
+    def forward(ctx, qkv, wq, wk, cfg):
+        hq, hkv, eps, where = cfg
+        ctx.save_for_backward(qkv, wq, wk, where[1])
         ctx.refs = (wq, wk)
-        ctx.cfg = (hq, hkv, eps, rotary, seq, offset)
-        return out
+        ctx.cfg = cfg
+        return _normed_copy(qkv, hq, hkv, wq, wk, eps, where)
 
     @staticmethod
     def backward(ctx, dy):
         qkv, wq, wk, positions = ctx.saved_tensors
-        hq, hkv, eps, rotary, seq, offset = ctx.cfg
-        where = (rotary, positions, seq, offset)
+        hq, hkv, eps, where = ctx.cfg
+        where = (where[0], positions, *where[2:])
         need = ctx.needs_input_grad
         if torch.is_grad_enabled() or not _plain(dy):
             # differentiated itself, or under a function transform: elementary operations
@@ -409,7 +453,7 @@ class _QKNormRopeFn(torch.autograd.Function):
             with torch.enable_grad():
                 out = _plain_qk_norm_rope(qkv, hq, hkv, wq, wk, eps, where)
                 got = iter(torch.autograd.grad(out, leaves, dy, create_graph=True))
-            return (*(next(got) if n else None for n in need[:3]), None, None, None, None, None, None, None)
+            return (*(next(got) if n else None for n in need[:3]), None)
         want = need[1:3]
         main = (None, None)
         if want[0] or want[1]:
@@ -418,11 +462,11 @@ class _QKNormRopeFn(torch.autograd.Function):
                     for k, r, n in ((1, ctx.refs[0], want[0]), (2, ctx.refs[1], want[1]))]
             if any(m is None for m, n in zip(main, want) if n):
                 main = (None, None)
-        dx, dwq, dwk = _norm_backward(_unit(qkv), _unit(dy), wq, wk, hq, hkv, eps, where, want, main)
-        return dx, dwq, dwk, None, None, None, None, None, None, None
+        return (*_norm_backward(_unit(qkv), _unit(dy), wq, wk, hq, hkv, eps, where, want, main), None)
 
 
 def _norm_args(qkv, hq, hkv, wq, wk, rotary, seq, offset, ranges, positions):
+    """(where, whether the kernels take it, wq, wk): the weights as rows."""
     _check_heads(qkv, hq + hkv)
     if hq < 0 or hkv < 0:
         raise ValueError(f"numbers of heads are not negative: {hq}, {hkv}")
@@ -431,12 +475,15 @@ def _norm_args(qkv, hq, hkv, wq, wk, rotary, seq, offset, ranges, positions):
             raise ValueError(f"a weight of the norm has one value per component ({qkv.shape[2]}), not {tuple(w.shape)}")
     where = _where(qkv, rotary, seq, offset, ranges, positions)
     if rotary is not None:
-        rotary.rotated(qkv.shape[2])
+        rotary._plan(qkv.shape[2])
     native = (_native_ok(qkv) and _weight_ok(wq, qkv) and _weight_ok(wk, qkv)
               and (wq is None or wk is None or wq.dtype == wk.dtype))
     # (a weight that is a row already stays the tensor that it is: its accumulator is an attribute of it)
-    flat = [w if w is None or (w.dim() == 1 and w.is_contiguous()) else w.reshape(-1).contiguous() for w in (wq, wk)]
-    return where, native, flat
+    if wq is not None and (wq.dim() != 1 or not wq.is_contiguous()):
+        wq = wq.reshape(-1).contiguous()
+    if wk is not None and (wk.dim() != 1 or not wk.is_contiguous()):
+        wk = wk.reshape(-1).contiguous()
+    return where, native, wq, wk
 
 
 def qk_norm_rope(qkv: torch.Tensor, seq: int, hq: int, hkv: int, q_weight=None, k_weight=None, *, rotary: Rotary = None,
@@ -448,10 +495,13 @@ def qk_norm_rope(qkv: torch.Tensor, seq: int, hq: int, hkv: int, q_weight=None, 
 
     The result is a new tensor and the backward pass reads ``qkv`` again, so that it stays as it is;
     :func:`qk_norm_rope_` works in place where no gradient is wanted."""
-    where, native, (wq, wk) = _norm_args(qkv, hq, hkv, q_weight, k_weight, rotary, seq, offset, ranges, positions)
-    if native:
-        return _QKNormRopeFn.apply(qkv, wq, wk, hq, hkv, float(eps), *where)
-    return _plain_qk_norm_rope(qkv, hq, hkv, wq, wk, eps, where)
+    where, native, wq, wk = _norm_args(qkv, hq, hkv, q_weight, k_weight, rotary, seq, offset, ranges, positions)
+    if not native:
+        return _plain_qk_norm_rope(qkv, hq, hkv, wq, wk, eps, where)
+    if torch.is_grad_enabled() and (qkv.requires_grad or (wq is not None and wq.requires_grad)
+                                    or (wk is not None and wk.requires_grad)):
+        return _QKNormRopeFn.apply(qkv, wq, wk, (hq, hkv, float(eps), where))
+    return _normed_copy(qkv, hq, hkv, wq, wk, float(eps), where)
 
 
 def qk_norm_rope_(qkv: torch.Tensor, seq: int, hq: int, hkv: int, q_weight=None, k_weight=None, *, rotary: Rotary = None,
@@ -459,12 +509,11 @@ def qk_norm_rope_(qkv: torch.Tensor, seq: int, hq: int, hkv: int, q_weight=None,
     """:func:`qk_norm_rope` in place, for inference: refused where a gradient would be wanted."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (qkv, q_weight, k_weight)):
         raise RuntimeError("qk_norm_rope_ overwrites what its gradient would need: use qk_norm_rope, or torch.no_grad()")
-    where, native, (wq, wk) = _norm_args(qkv, hq, hkv, q_weight, k_weight, rotary, seq, offset, ranges, positions)
+    where, native, wq, wk = _norm_args(qkv, hq, hkv, q_weight, k_weight, rotary, seq, offset, ranges, positions)
     if _overlaps(qkv):
         raise ValueError("a tensor that is changed in place must not overlap itself: use ops.qk_norm_rope")
     if native and (qkv.stride(2) == 1 or qkv.shape[2] == 1):
-        with torch.no_grad():
-            _norm_forward(qkv, qkv, hq, hkv, wq, wk, float(eps), where)
+        _norm_forward(qkv, qkv, hq, hkv, wq, wk, float(eps), where)
         if not qkv.is_inference():
             torch.autograd.graph.increment_version(qkv)
         return qkv
