@@ -26,6 +26,7 @@
 // slot is its rank in pair order among the pairs of its expert, so nothing depends on how CTAs are scheduled; sums of p are
 // formed per chunk of tokens and then over the chunks, always in the same order.
 #include "common.cuh"
+#include "runtime.cuh"
 
 #include <cuda_fp16.h>
 
@@ -38,9 +39,9 @@ constexpr int kWarps = 8;
 constexpr int kMostRows = 256;                                // tokens of a chunk (a CTA of the first kernel) at most
 constexpr int kSlotThreads = 1024;                            // of a CTA of the second kernel, which takes whole chunks
 
-// Tokens of a chunk: a token per warp while that gives every SM up to two CTAs, then so many that it still does.
+// Tokens of a chunk: a token per warp while that gives every SM up to three CTAs, then so many that it still does.
 inline int rows_of(int tokens) {
-  const int per_warp = (tokens - 1) / (kWarps * 2 * 148) + 1;
+  const int per_warp = (tokens - 1) / (kWarps * 3 * 148) + 1;
   return kWarps * (per_warp < kMostRows / kWarps ? per_warp : kMostRows / kWarps);
 }
 
@@ -84,9 +85,25 @@ __device__ __forceinline__ void load_row(const T* p, bool vectors, int left, flo
 
 // Order-preserving: a < b as floats, ordered(a) < ordered(b) as integers.
 __device__ __forceinline__ unsigned ordered(float v) {
-  if (v == 0.f) v = 0.f;                                      // -0 is 0
-  const unsigned u = __float_as_uint(v);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  unsigned u = __float_as_uint(v);
+  if (u == 0x80000000u) u = 0u;                               // -0 is 0
+  return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+// Largest and smallest value of a warp; a NaN is the largest.
+__device__ __forceinline__ float top_of_warp(float v) {
+  float r;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float low_of_warp(float v) {
+  float r;
+  asm("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 // Falling, by Batcher's odd-even merges.
 template <int C>
@@ -105,8 +122,6 @@ __device__ __forceinline__ void sort_falling(unsigned (&key)[C]) {
             key[i + j + q] = min(x, y);
           }
 }
-__device__ __forceinline__ float warp_min(float v) { return -warp_max(-v); }
-
 __device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -185,51 +200,62 @@ __device__ __noinline__ int choose_in_64_bits(const RouteArgs& a, const float* l
   return chosen;
 }
 
-// Takes the logits without a number (NaN; softmax: +inf) out of a lane's, as bits of `bad`; whether the token has any.
+// The largest logit of a token.  Logits without a number (NaN; softmax: +inf) are taken out of a lane's, as bits of `bad`;
+// `nan`: whether the token has any.
 template <int C>
-__device__ __forceinline__ bool take_bad(float (&l)[C], bool sigmoid, unsigned& bad) {
+__device__ __forceinline__ float top_logit(float (&l)[C], bool sigmoid, unsigned& bad, bool& nan) {
+  float top = l[0];
 #pragma unroll
-  for (int j = 0; j < C; ++j)
-    if (l[j] != l[j] || (!sigmoid && l[j] == INFINITY)) {
-      bad |= 1u << j;
-      l[j] = -INFINITY;
-    }
-  return __any_sync(0xffffffffu, bad != 0u);
-}
-
-// Scores of a token, p = s / sum s (0 in rows without an expert), and what they are computed with.
-template <int C>
-struct Scores {
-  float top;                // largest logit
-  float inv;                // p = part * inv
-  float part[C];            // softmax: e^(l - top); sigmoid: s / e^min(top, 0), which does not underflow in whole rows
-  bool none;                // no expert may be chosen
-
-  __device__ __forceinline__ void set(const float (&l)[C], bool sigmoid) {
+  for (int j = 1; j < C; ++j) top = max_or_nan(top, l[j]);
+  top = top_of_warp(top);
+  nan = top != top || (!sigmoid && top == INFINITY);
+  if (nan) {
     top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < C; ++j) top = fmaxf(top, l[j]);
-    top = warp_max(top);
-    none = top == -INFINITY;
-    float z = 0.f;
-    const float shift = sigmoid ? fminf(top, 0.f) : top;
-#pragma unroll
     for (int j = 0; j < C; ++j) {
-      if (sigmoid) {
-        const float e = __expf(-fabsf(l[j]));
-        part[j] = __fdividef(l[j] > 0.f ? 1.f : shift == 0.f ? e : __expf(l[j] - shift), 1.f + e);
-      } else {
-        part[j] = __expf(l[j] - shift);
+      if (l[j] != l[j] || (!sigmoid && l[j] == INFINITY)) {
+        bad |= 1u << j;
+        l[j] = -INFINITY;
       }
-      if (none || l[j] == -INFINITY) part[j] = 0.f;
-      z += part[j];
+      top = fmaxf(top, l[j]);
     }
-    inv = none ? 0.f : 1.f / warp_sum(z);
+    top = top_of_warp(top);
+  }
+  return top;
+}
+
+// Scores of a token, p = s / sum s (0 in rows without an expert), from the largest logit.
+template <int C>
+struct Scores {
+  float inv;                // p = part * inv
+  float part[C];            // softmax: e^(l - top); sigmoid: s / e^min(top, 0), which does not underflow in whole rows
+
+  __device__ __forceinline__ void set(const float (&l)[C], bool sigmoid, float top) {
+    const bool none = top == -INFINITY;
+    float z = 0.f;
+    if (!sigmoid) {
+      const float shift = none ? 0.f : top;
+#pragma unroll
+      for (int j = 0; j < C; ++j) part[j] = __expf(l[j] - shift);
+    } else if (top >= 0.f) {
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const float e = __expf(-fabsf(l[j]));
+        part[j] = __fdividef(l[j] > 0.f ? 1.f : e, 1.f + e);
+      }
+    } else {
+      const float shift = none ? 0.f : top;
+#pragma unroll
+      for (int j = 0; j < C; ++j) part[j] = __fdividef(__expf(l[j] - shift), 1.f + __expf(l[j]));
+    }
+#pragma unroll
+    for (int j = 0; j < C; ++j) z += part[j];
+    inv = none ? 0.f : __fdividef(1.f, warp_sum(z));
   }
 };
 
 template <typename T, int C>
-__global__ void __launch_bounds__(kWarps * 32) route_kernel(const __grid_constant__ RouteArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(const __grid_constant__ RouteArgs a) {
   __shared__ int s_hist[kMaxExperts];
   __shared__ __align__(16) float s_row[kWarps][32 * C];       // a warp's values by expert; at the end its sums of p
   grid_dependency_launch();
@@ -253,9 +279,10 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const __grid_constan
     float l[C];
     load_row<T, C>(from + first, a.vectors, left, l);
     unsigned bad = 0u;                                        // this lane's experts without a number
-    const bool nan = take_bad<C>(l, a.sigmoid, bad);
+    bool nan;
+    const float top_l = top_logit<C>(l, a.sigmoid, bad, nan);
     Scores<C> s;
-    s.set(l, a.sigmoid);
+    s.set(l, a.sigmoid, top_l);
     unsigned key[C];                                          // value << 9 | 511 - expert; 0: not to be chosen
     int near = 0;                                             // differences of values up to here say nothing
     if (exact) {
@@ -263,14 +290,14 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const __grid_constan
       for (int j = 0; j < C; ++j) key[j] = l[j] > -INFINITY ? (ordered(l[j]) & ~511u) | (511 - first - j) : 0u;
     } else {
       float v[C], hi = -INFINITY, lo = INFINITY;
-      const float back = a.by_logit ? 0.f : a.sigmoid ? __expf(fminf(s.top, 0.f)) : s.inv;
+      const float back = a.by_logit ? 0.f : a.sigmoid ? __expf(fminf(top_l, 0.f)) : s.inv;
 #pragma unroll
       for (int j = 0; j < C; ++j) {
         v[j] = a.by_logit ? l[j] : s.part[j] * back + bias[j];
         if (l[j] > -INFINITY) { hi = fmaxf(hi, v[j]); lo = fminf(lo, v[j]); }
       }
-      hi = warp_max(hi);
-      lo = warp_min(lo);
+      hi = top_of_warp(hi);
+      lo = low_of_warp(lo);
       const float range = hi - lo, steps = range > 1e-25f && range < 1e38f ? __fdividef(8388600.f, range) : 0.f;
       // scores: sigmoid 4e-7 off at most (its slope times the exponential's error, a division), softmax 4e-6 of the largest,
       // the bias's addition; the cut itself: a step each way
@@ -388,7 +415,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const __grid_constan
     float weight = 0.f;
     {
       const float lc = chosen >= 0 && !nan ? to_f(from[chosen]) : -INFINITY;
-      const float top = a.renormalize ? warp_max(lc) : s.top;
+      const float top = a.renormalize ? top_of_warp(lc) : top_l;
       float v;
       if (a.sigmoid) {
         const float shift = a.renormalize ? fminf(top, 0.f) : 0.f, e = __expf(-fabsf(lc));
@@ -407,8 +434,9 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const __grid_constan
       a.w[(size_t)t * a.k + lane] = weight;
       if (chosen >= 0) atomicAdd(&s_hist[chosen], 1);
     }
+    const float inv = nan ? __int_as_float(0x7fffffff) : s.inv;
 #pragma unroll
-    for (int j = 0; j < C; ++j) sums[j] += nan ? __int_as_float(0x7fffffff) : s.part[j] * s.inv;
+    for (int j = 0; j < C; ++j) sums[j] += s.part[j] * inv;
   }
   __syncwarp();
 #pragma unroll
@@ -426,17 +454,32 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const __grid_constan
 // experts of a token differ, so that the rank is the number of earlier tokens: whole CTAs before (sums over the chunks'
 // histograms), words of 32 tokens before, lower bits in the word.
 __global__ void __launch_bounds__(kSlotThreads)
-route_slot_kernel(const int* __restrict__ ids, int tokens, int k, int E, int E4, int capacity, const int* __restrict__ hist,
-                  const float* __restrict__ psum, int chunks, int chunk, int per_cta, int* __restrict__ counts,
-                  float* __restrict__ prob_sum, int* __restrict__ slot) {
-  constexpr int W = kMostRows / 32;
+route_slot_kernel(const int* ids, int tokens, int k, int E, int E4, int capacity, const int* hist, const float* psum, int chunks,
+                  int chunk, int per_cta, int* counts, float* prob_sum, int* slot) {
+  constexpr int W = kMostRows / 32, kOwn = 2;                 // kOwn: pairs of a thread whose experts are fetched at once
   __shared__ unsigned s_mask[W][kMaxExperts];
   __shared__ __align__(16) int s_part[kSlotThreads * 4];      // sums before this CTA; then [W][kMaxExperts] bases
-  grid_dependency_launch();
   const int tid = threadIdx.x, lane = tid & 31;
   for (int i = tid; i < W * kMaxExperts; i += kSlotThreads) (&s_mask[0][0])[i] = 0u;
   const int quads = E4 / 4, lanes = kSlotThreads / quads;     // threads per four experts
   const int before = blockIdx.x * per_cta, t0 = before * chunk;          // chunks and tokens before this CTA's
+  const int pairs = min(tokens - t0, per_cta * chunk) * k;
+  grid_dependency_wait();                                     // (launched ahead of the end of the kernel before it)
+  grid_dependency_launch();
+  // everything that is read, first: a latency is all that this kernel is made of
+  const int* own = ids + (size_t)t0 * k;
+  int e_of[kOwn];
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) e_of[i] = tid + i * kSlotThreads < pairs ? own[tid + i * kSlotThreads] : -1;
+  const int q_sum = blockIdx.x + (tid >> 5) * gridDim.x;      // sums of p: a warp of the grid per four experts
+  float4 p_sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (q_sum < quads) {
+#pragma unroll 8
+    for (int r = lane; r < chunks; r += 32) {
+      const float4 v = *reinterpret_cast<const float4*>(psum + (size_t)r * E4 + q_sum * 4);
+      p_sum.x += v.x; p_sum.y += v.y; p_sum.z += v.z; p_sum.w += v.w;
+    }
+  }
   {
     const int q = tid % quads, r0 = tid / quads;
     int4 sum = make_int4(0, 0, 0, 0);
@@ -450,11 +493,15 @@ route_slot_kernel(const int* __restrict__ ids, int tokens, int k, int E, int E4,
     }
   }
   __syncthreads();
-  const int pairs = min(tokens - t0, per_cta * chunk) * k;
-  for (int p = tid; p < pairs; p += kSlotThreads) {
-    const int e = ids[(size_t)t0 * k + p];
+  auto each_pair = [&](auto visit) {
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i)
+      if (tid + i * kSlotThreads < pairs) visit(tid + i * kSlotThreads, e_of[i]);
+    for (int p = tid + kOwn * kSlotThreads; p < pairs; p += kSlotThreads) visit(p, own[p]);
+  };
+  each_pair([&](int p, int e) {
     if (e >= 0 && e < E) atomicOr(&s_mask[(p / k) >> 5][e], 1u << ((p / k) & 31));
-  }
+  });
   int run = 0;
   if (tid < E)
     for (int r = 0; r < min(lanes, before); ++r) run += s_part[r * E4 + tid];
@@ -467,25 +514,27 @@ route_slot_kernel(const int* __restrict__ ids, int tokens, int k, int E, int E4,
     if (blockIdx.x == gridDim.x - 1) counts[tid] = run;
   }
   __syncthreads();
-  for (int p = tid; p < pairs; p += kSlotThreads) {
-    const int e = ids[(size_t)t0 * k + p], tok = p / k;
+  each_pair([&](int p, int e) {
+    const int tok = p / k;
     int s = -1;
     if (e >= 0 && e < E) {
       s = s_part[(tok >> 5) * kMaxExperts + e] + __popc(s_mask[tok >> 5][e] & ((1u << (tok & 31)) - 1u));
       if (s >= capacity) s = -1;
     }
     slot[(size_t)t0 * k + p] = s;
-  }
-  // the sums of p over the chunks: a warp of the grid per four experts, its lanes every 32nd chunk
-  for (int q = blockIdx.x * (kSlotThreads / 32) + (tid >> 5); q < quads; q += gridDim.x * (kSlotThreads / 32)) {
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int r = lane; r < chunks; r += 32) {
-      const float4 v = *reinterpret_cast<const float4*>(psum + (size_t)r * E4 + q * 4);
-      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+  });
+  for (int q = q_sum; q < quads; q += gridDim.x * (kSlotThreads / 32)) {
+    if (q != q_sum) {                                         // (few CTAs: few chunks as well)
+      p_sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int r = lane; r < chunks; r += 32) {
+        const float4 v = *reinterpret_cast<const float4*>(psum + (size_t)r * E4 + q * 4);
+        p_sum.x += v.x; p_sum.y += v.y; p_sum.z += v.z; p_sum.w += v.w;
+      }
     }
-    const float out[4] = {warp_sum(sum.x), warp_sum(sum.y), warp_sum(sum.z), warp_sum(sum.w)};
-    if (lane < 4 && q * 4 + lane < E) prob_sum[q * 4 + lane] = out[lane];
+    const float out[4] = {warp_sum(p_sum.x), warp_sum(p_sum.y), warp_sum(p_sum.z), warp_sum(p_sum.w)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane == i && q * 4 + i < E) prob_sum[q * 4 + i] = out[i];
   }
 }
 
@@ -519,9 +568,10 @@ route_bwd_kernel(const __grid_constant__ RouteArgs a, const float* __restrict__ 
     __syncwarp();
     if (id >= 0 && id < a.E) s_row[warp][id] = grad;
     unsigned bad = 0u;
-    const bool nan = take_bad<C>(l, a.sigmoid, bad);
+    bool nan;
+    const float top_l = top_logit<C>(l, a.sigmoid, bad, nan);
     Scores<C> s;
-    s.set(l, a.sigmoid);
+    s.set(l, a.sigmoid, top_l);
     float p[C], pq = 0.f;
 #pragma unroll
     for (int j = 0; j < C; ++j) { p[j] = s.part[j] * s.inv; pq += p[j] * coef[j]; }
@@ -628,9 +678,9 @@ DD_API int dd_route_fwd(const void* logits, int ld, int dtype, int tokens, int E
                              : forward<float>(a, C, chunks, s);
   if (e) return e;
   const int per_cta = kMostRows / a.rows;
-  route_slot_kernel<<<(chunks - 1) / per_cta + 1, kSlotThreads, 0, s>>>(ids, tokens, k, E, a.E4, capacity, a.hist, a.psum, chunks,
-                                                                       a.rows, per_cta, counts, prob_sum, slot);
-  return (int)cudaGetLastError();
+  return launch_ahead(route_slot_kernel, dim3((chunks - 1) / per_cta + 1), dim3(kSlotThreads), 0, s, true, (const int*)ids,
+                      tokens, k, E, a.E4, capacity, (const int*)a.hist, (const float*)a.psum, chunks, a.rows, per_cta, counts,
+                      prob_sum, slot);
 }
 
 // dlogits [tokens, ld] from the gradients of w (dw [tokens, k], or null) and of prob_sum (dprob [E], or null).
