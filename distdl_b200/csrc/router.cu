@@ -9,7 +9,7 @@
 //   backward with g on w and q on sum_t p:  d s_i of the chosen from g, d p from q, and ds / dl = s (1 - s) (sigmoid),
 //            written out per case at the kernel
 //
-// An expert whose logit is -inf is never chosen; a token with fewer than k others has -1 and weight 0 in the places left,
+// An expert whose logit or bias is -inf is never chosen; a token with fewer than k others has -1 and weight 0 in the places left,
 // one with none of them routes nowhere and adds nothing.  A NaN (softmax: also +inf) makes the weights of its token, its p and
 // its gradient NaN, and counts as the best, so that a token of NaN alone is not lost either.
 //
@@ -105,6 +105,10 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// Keys: value (23 bits) << 9 | 511 - expert, 0 for an expert that may not be chosen.
+constexpr float kSteps = 8388600.f;
+constexpr unsigned kBad = 0xfffffe00u;
+
 // Falling, by Batcher's odd-even merges.
 template <int C>
 __device__ __forceinline__ void sort_falling(unsigned (&key)[C]) {
@@ -122,80 +126,192 @@ __device__ __forceinline__ void sort_falling(unsigned (&key)[C]) {
             key[i + j + q] = min(x, y);
           }
 }
+// The two largest values of every group of experts, each in all lanes that `step` lanes of a group share; V: int or double.
+// best: this lane's own two, where groups begin and end with a lane's experts (a.lanes), else all values by expert in shared
+// memory, `none` where there is no expert.  Returns the group of this lane.
+template <typename V>
+__device__ __forceinline__ int best_of_groups(const RouteArgs& a, const V* values, V none, V& b0, V& b1, int& step) {
+  const int lane = threadIdx.x & 31;
+  if (a.lanes > 0) {
+    step = a.lanes;
+  } else {
+    step = a.groups > 16 ? 1 : a.groups > 8 ? 2 : a.groups > 4 ? 4 : a.groups > 2 ? 8 : 16;
+    b0 = b1 = none;
+    if (lane / step < a.groups)
+      for (int i = lane % step; i < a.size; i += step) {
+        const V v = values[lane / step * a.size + i];
+        b1 = max(b1, min(b0, v));
+        b0 = max(b0, v);
+      }
+  }
+  for (int o = 1; o < step; o <<= 1) {
+    const V o0 = __shfl_xor_sync(0xffffffffu, b0, o), o1 = __shfl_xor_sync(0xffffffffu, b1, o);
+    b1 = max(max(b1, o1), min(b0, o0));
+    b0 = max(b0, o0);
+  }
+  return lane / step;
+}
+// Whether the group of this lane is among the best, the lower numbers first where they are alike.
+template <typename V>
+__device__ __forceinline__ bool among_best(const RouteArgs& a, V value, int g, int step) {
+  int place = 0;
+  for (int i = 0; i < a.groups; ++i) {
+    const V v = __shfl_sync(0xffffffffu, value, i * step);
+    place += v > value || (v == value && i < g);
+  }
+  return g < a.groups && place < a.top_groups;
+}
+// Clears what a lane holds of groups that are not kept.
+template <typename V, int C>
+__device__ __forceinline__ void clear_others(const RouteArgs& a, V (&v)[C], V none, bool in, int first, int left, int step) {
+  if (a.lanes > 0) {
+    if (!in) {
+#pragma unroll
+      for (int j = 0; j < C; ++j) v[j] = none;
+    }
+  } else {
+    const unsigned kept = __ballot_sync(0xffffffffu, in);
+    int of = first / a.size, at = first - of * a.size;
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      if (j >= left || !((kept >> (of * step)) & 1u)) v[j] = none;
+      if (++at == a.size) { at = 0; ++of; }
+    }
+  }
+}
+
+// The choice of one token from the keys of its experts: lane i gets the i-th expert, -1 where there is none.  `close` is set
+// where values within `near` of one another (near < 0: all values are exact) decide and are not those of experts alike in logit
+// and bias.
+template <typename T, int C>
+__device__ __forceinline__ int choose(const RouteArgs& a, unsigned (&key)[C], int first, int left, int near, bool& close,
+                                      int* values, const T* from) {
+  const int lane = threadIdx.x & 31;
+  if (a.groups > 1) {
+    int b0, b1, step;
+    if (a.lanes > 0) {
+      sort_falling<C>(key);
+      b0 = (int)(key[0] >> 9);
+      b1 = C > 1 ? (int)(key[C > 1] >> 9) : 0;
+    } else {
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+        if (j < left) values[first + j] = (int)(key[j] >> 9);
+      __syncwarp();
+    }
+    const int g = best_of_groups<int>(a, values, 0, b0, b1, step);
+    const int value = a.group_sum ? b0 + b1 : b0;
+    const bool in = among_best(a, value, g, step);
+    if (near >= 0) {
+      const int least = (int)__reduce_min_sync(0xffffffffu, in ? (unsigned)value : 0x7fffffffu);
+      const int most = (int)__reduce_max_sync(0xffffffffu, !in && g < a.groups ? (unsigned)value : 0u);
+      // (of a group with one expert only its value itself would have to be known)
+      close = (most > 0 && least - most <= (a.group_sum ? 2 * near : near)) ||
+              __any_sync(0xffffffffu, g < a.groups && a.group_sum && a.size > 1 && b0 > 0 && b1 == 0);
+    }
+    clear_others<unsigned, C>(a, key, 0u, in, first, left, step);
+    if (a.lanes == 0) {
+      __syncwarp();
+      sort_falling<C>(key);
+    }
+  } else {
+    sort_falling<C>(key);
+  }
+  // the k best one by one
+  int chosen = -1;
+  unsigned was = 0u;
+  const int rounds = a.k + (near >= 0 ? 1 : 0);               // (one more: the first that is left out must not be close)
+  for (int i = 0; i < rounds; ++i) {
+    const unsigned top = __reduce_max_sync(0xffffffffu, key[0]);
+    if (top == 0u) break;
+    const int e = 511 - (int)(top & 511u);
+    if (i > 0 && (int)(was >> 9) - (int)(top >> 9) <= near) {
+      const int f = 511 - (int)(was & 511u);                  // two alike in logit and bias are alike, and in order
+      close |= to_f(from[f]) != to_f(from[e]) || (a.bias != nullptr && a.bias[f] != a.bias[e]);
+    }
+    was = top;
+    if (lane == i && i < a.k) chosen = e;
+    if (key[0] == top) {
+#pragma unroll
+      for (int j = 0; j + 1 < C; ++j) key[j] = key[j + 1];
+      key[C - 1] = 0u;
+    }
+  }
+  return chosen;
+}
+
 __device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// The largest value and the lowest number that has it (-1: all are -inf), over the warp.
-__device__ __forceinline__ void warp_best_d(double& v, int& e) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const double u = __shfl_xor_sync(0xffffffffu, v, o);
-    const int f = __shfl_xor_sync(0xffffffffu, e, o);
-    if (u > v || (u == v && (unsigned)f < (unsigned)e)) { v = u; e = f; }
-  }
+// Order-preserving, as ordered(); 0: -inf.
+__device__ __forceinline__ unsigned long long ordered_d(double v) {
+  if (!(v > -INFINITY)) return 0ull;
+  const unsigned long long u = (unsigned long long)__double_as_longlong(v + 0.0);
+  return u ^ ((unsigned long long)((long long)u >> 63) | 0x8000000000000000ull);
 }
 
-// The choice of one token in 64 bits: lane i gets the i-th expert, -1 where there is none.  l_in: this lane's logits (-inf: not
-// to be chosen, or bad: the best), first: its first expert.
+// The choice of a token in 64 bits.  l_in: this lane's logits (-inf: not to be chosen, or bad: the best); top: the token's
+// largest.
 template <int C>
-__device__ __noinline__ int choose_in_64_bits(const RouteArgs& a, const float* l_in, int first, unsigned bad) {
+__device__ __noinline__ int choose_in_64_bits(const RouteArgs& a, const float* l_in, float top, unsigned bad, int first, int left,
+                                              double* values) {
   const int lane = threadIdx.x & 31;
-  double c[C], top = -INFINITY;
-  for (int j = 0; j < C; ++j) top = fmax(top, (double)l_in[j]);
-  for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-  double z = 0.0;
+  double c[C], z = 0.0;
+#pragma unroll
   for (int j = 0; j < C; ++j) {
     const double l = l_in[j];
-    c[j] = a.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top);
+    c[j] = a.by_logit ? l : a.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - (double)top);
     z += c[j];
   }
-  z = warp_sum_d(z);
+  if (!a.by_logit && !a.sigmoid) z = warp_sum_d(z);
+#pragma unroll
   for (int j = 0; j < C; ++j) {
-    if (!(l_in[j] > -INFINITY)) { c[j] = (bad >> j) & 1u ? INFINITY : -INFINITY; continue; }
-    if (a.by_logit) { c[j] = l_in[j]; continue; }
-    if (!a.sigmoid) c[j] /= z;
-    if (a.bias != nullptr) c[j] += (double)a.bias[first + j];
+    if (!a.by_logit && !a.sigmoid) c[j] /= z;
+    if (a.bias != nullptr && j < left) c[j] += (double)a.bias[first + j];
+    if (!(l_in[j] > -INFINITY) || c[j] != c[j]) c[j] = (bad >> j) & 1u ? INFINITY : -INFINITY;
   }
   if (a.groups > 1) {
-    double mine = -INFINITY;                                  // lane g: value of group g
-    for (int g = 0; g < a.groups; ++g) {
-      double best[2];
-      int was = -1;
-      for (int r = 0; r < 2; ++r) {
-        double v = -INFINITY;
-        int e = -1;
-        for (int j = 0; j < C; ++j) {
-          const int n = first + j;
-          if (n >= g * a.size && n < (g + 1) * a.size && n != was && c[j] > v) { v = c[j]; e = n; }
-        }
-        warp_best_d(v, e);
-        best[r] = v;
-        was = e;
+    double b0 = -INFINITY, b1 = -INFINITY;
+    int step;
+    if (a.lanes > 0) {
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        b1 = fmax(b1, fmin(b0, c[j]));
+        b0 = fmax(b0, c[j]);
       }
-      const double v = a.group_sum && best[1] > -INFINITY ? best[0] + best[1] : best[0];
-      if (lane == g) mine = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+        if (j < left) values[first + j] = c[j];
+      __syncwarp();
     }
-    int place = 0;
-    for (int g = 0; g < a.groups; ++g) {
-      const double v = __shfl_sync(0xffffffffu, mine, g);
-      place += v > mine || (v == mine && g < lane);
-    }
-    const unsigned kept = __ballot_sync(0xffffffffu, lane < a.groups && place < a.top_groups);
-    for (int j = 0; j < C; ++j)
-      if (first + j < a.E && !((kept >> ((first + j) / a.size)) & 1u)) c[j] = -INFINITY;
+    const int g = best_of_groups<double>(a, values, -INFINITY, b0, b1, step);
+    const double value = a.group_sum && b1 > -INFINITY ? b0 + b1 : b0;
+    const bool in = among_best(a, value, g, step);
+    clear_others<double, C>(a, c, -INFINITY, in, first, left, step);
+    __syncwarp();
   }
+  unsigned long long key[C];
+#pragma unroll
+  for (int j = 0; j < C; ++j) key[j] = ordered_d(c[j]);
   int chosen = -1;
   for (int i = 0; i < a.k; ++i) {
-    double v = -INFINITY;
-    int e = -1;
+    unsigned long long best = 0ull;
+    int e = 0;
+#pragma unroll
     for (int j = 0; j < C; ++j)
-      if (c[j] > v) { v = c[j]; e = first + j; }
-    warp_best_d(v, e);
+      if (key[j] > best) { best = key[j]; e = first + j; }
+    const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(best >> 32));
+    const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned)(best >> 32) == hi ? (unsigned)best : 0u);
+    const unsigned long long most = (unsigned long long)hi << 32 | lo;
+    if (most == 0ull) break;
+    e = __shfl_sync(0xffffffffu, e, __ffs(__ballot_sync(0xffffffffu, best == most)) - 1);
     if (lane == i) chosen = e;
+#pragma unroll
     for (int j = 0; j < C; ++j)
-      if (first + j == e) c[j] = -INFINITY;
+      if (first + j == e) key[j] = 0ull;
   }
   return chosen;
 }
@@ -257,7 +373,7 @@ struct Scores {
 template <typename T, int C>
 __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(const __grid_constant__ RouteArgs a) {
   __shared__ int s_hist[kMaxExperts];
-  __shared__ __align__(16) float s_row[kWarps][32 * C];       // a warp's values by expert; at the end its sums of p
+  __shared__ __align__(16) double s_row[kWarps][32 * C];   // a warp's values by expert; at the end its sums of p
   grid_dependency_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < a.E; e += kWarps * 32) s_hist[e] = 0;
@@ -283,8 +399,8 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
     const float top_l = top_logit<C>(l, a.sigmoid, bad, nan);
     Scores<C> s;
     s.set(l, a.sigmoid, top_l);
-    unsigned key[C];                                          // value << 9 | 511 - expert; 0: not to be chosen
-    int near = 0;                                             // differences of values up to here say nothing
+    unsigned key[C];
+    int near = -1;                                            // differences of values up to here say nothing
     if (exact) {
 #pragma unroll
       for (int j = 0; j < C; ++j) key[j] = l[j] > -INFINITY ? (ordered(l[j]) & ~511u) | (511 - first - j) : 0u;
@@ -294,122 +410,33 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
 #pragma unroll
       for (int j = 0; j < C; ++j) {
         v[j] = a.by_logit ? l[j] : s.part[j] * back + bias[j];
-        if (l[j] > -INFINITY) { hi = fmaxf(hi, v[j]); lo = fminf(lo, v[j]); }
+        if (!(l[j] > -INFINITY && v[j] > -INFINITY)) v[j] = -INFINITY;     // (a bias of -inf takes an expert out, too)
+        else { hi = fmaxf(hi, v[j]); lo = fminf(lo, v[j]); }
       }
       hi = top_of_warp(hi);
-      lo = low_of_warp(lo);
-      const float range = hi - lo, steps = range > 1e-25f && range < 1e38f ? __fdividef(8388600.f, range) : 0.f;
+      // (values far below the largest are not told apart: should they decide, they are close)
+      lo = fmaxf(low_of_warp(lo), hi - (a.by_logit ? 64.f : 8.f));
+      const float range = hi - lo, steps = range > 1e-25f ? __fdividef(kSteps, range) : 0.f;
       // scores: sigmoid 4e-7 off at most (its slope times the exponential's error, a division), softmax 4e-6 of the largest,
       // the bias's addition; the cut itself: a step each way
       const float off = a.by_logit ? 0.f : (a.sigmoid ? 2e-6f : 8e-6f * s.inv) + 4e-7f * fmaxf(fabsf(hi), fabsf(lo));
       near = (int)fminf(off * steps + 3.f, 8388607.f);
 #pragma unroll
       for (int j = 0; j < C; ++j)
-        key[j] = l[j] > -INFINITY ? (unsigned)((int)((v[j] - lo) * steps) + 1) << 9 | (511 - first - j) : 0u;
+        key[j] = v[j] > -INFINITY ? (unsigned)((int)(fmaxf(v[j] - lo, 0.f) * steps) + 1) << 9 | (511 - first - j) : 0u;
     }
     if (nan) {
 #pragma unroll
       for (int j = 0; j < C; ++j)
-        if ((bad >> j) & 1u) key[j] = 0xfffffe00u | (511 - first - j);
+        if ((bad >> j) & 1u) key[j] = kBad | (511 - first - j);
     }
     bool close = false;
-    if (a.groups > 1) {
-      int value = 0, g = a.groups;                            // of this lane's group; 0: none of its experts may be chosen
-      bool single = false;                                    // sums: with one expert only, which needs its score itself
-      int step;                                               // the groups' values are those of every step-th lane
-      if (a.lanes > 0) {
-        sort_falling<C>(key);
-        int b0 = (int)(key[0] >> 9), b1 = C > 1 ? (int)(key[C > 1] >> 9) : 0;
-        for (int o = 1; o < a.lanes; o <<= 1) {
-          const int o0 = __shfl_xor_sync(0xffffffffu, b0, o), o1 = __shfl_xor_sync(0xffffffffu, b1, o);
-          b1 = max(max(b1, o1), min(b0, o0));
-          b0 = max(b0, o0);
-        }
-        step = a.lanes;
-        g = lane / a.lanes;
-        value = a.group_sum ? b0 + b1 : b0;
-        single = b0 > 0 && b1 == 0;
-      } else {
-        // a group begins and ends at any expert: through shared memory, a lane or several for every group's scan
-        int* values = reinterpret_cast<int*>(s_row[warp]);
-#pragma unroll
-        for (int j = 0; j < C; ++j)
-          if (j < left) values[first + j] = (int)(key[j] >> 9);
-        __syncwarp();
-        step = a.groups > 16 ? 1 : a.groups > 8 ? 2 : a.groups > 4 ? 4 : a.groups > 2 ? 8 : 16;
-        g = lane / step;
-        int b0 = 0, b1 = 0;
-        if (g < a.groups)
-          for (int i = lane % step; i < a.size; i += step) {
-            const int v = values[g * a.size + i];
-            b1 = max(b1, min(b0, v));
-            b0 = max(b0, v);
-          }
-        for (int o = 1; o < step; o <<= 1) {
-          const int o0 = __shfl_xor_sync(0xffffffffu, b0, o), o1 = __shfl_xor_sync(0xffffffffu, b1, o);
-          b1 = max(max(b1, o1), min(b0, o0));
-          b0 = max(b0, o0);
-        }
-        value = a.group_sum ? b0 + b1 : b0;
-        single = b0 > 0 && b1 == 0;
-        __syncwarp();
-      }
-      int place = 0;
-      for (int i = 0; i < a.groups; ++i) {
-        const int v = __shfl_sync(0xffffffffu, value, i * step);
-        place += v > value || (v == value && i < g);
-      }
-      const bool in = g < a.groups && place < a.top_groups;
-      if (!exact) {
-        const int least = (int)__reduce_min_sync(0xffffffffu, in ? (unsigned)value : 0x7fffffffu);
-        const int most = (int)__reduce_max_sync(0xffffffffu, !in && g < a.groups ? (unsigned)value : 0u);
-        close = most > 0 && least - most <= (a.group_sum ? 2 * near : near);
-        if (a.group_sum && a.size > 1) close |= __any_sync(0xffffffffu, g < a.groups && single);
-      }
-      if (a.lanes > 0) {
-        if (!in) {
-#pragma unroll
-          for (int j = 0; j < C; ++j) key[j] = 0u;
-        }
-      } else {
-        const unsigned kept = __ballot_sync(0xffffffffu, in);
-        int of = first / a.size, at = first - of * a.size;
-#pragma unroll
-        for (int j = 0; j < C; ++j) {
-          if (j >= left || !((kept >> (of * step)) & 1u)) key[j] = 0u;
-          if (++at == a.size) { at = 0; ++of; }
-        }
-        sort_falling<C>(key);
-      }
-    } else {
-      sort_falling<C>(key);
-    }
-    // the k best one by one: lane i keeps the i-th
-    int chosen = -1;
-    unsigned was = 0u;
-    const int rounds = a.k + (exact ? 0 : 1);                 // (one more: the first that is left out must not be close)
-    for (int i = 0; i < rounds; ++i) {
-      const unsigned top = __reduce_max_sync(0xffffffffu, key[0]);
-      if (top == 0u) break;
-      const int e = 511 - (int)(top & 511u);
-      if (!exact && i > 0 && (int)(was >> 9) - (int)(top >> 9) <= near) {
-        // two alike in logit and bias are alike, and in order
-        const int f = 511 - (int)(was & 511u);
-        close |= to_f(from[f]) != to_f(from[e]) || (a.bias != nullptr && a.bias[f] != a.bias[e]);
-      }
-      was = top;
-      if (lane == i && i < a.k) chosen = e;
-      if (key[0] == top) {
-#pragma unroll
-        for (int j = 0; j + 1 < C; ++j) key[j] = key[j + 1];
-        key[C - 1] = 0u;
-      }
-    }
+    int chosen = choose<T, C>(a, key, first, left, near, close, reinterpret_cast<int*>(s_row[warp]), from);
     if (close) {                                              // (the same on every lane)
       float again[C];
 #pragma unroll
       for (int j = 0; j < C; ++j) again[j] = l[j];
-      chosen = choose_in_64_bits<C>(a, again, first, bad);
+      chosen = choose_in_64_bits<C>(a, again, top_l, bad, first, left, s_row[warp]);
     }
     // the weights, from the chosen logits: sums of k lanes, shifted so that the largest does not underflow
     float weight = 0.f;
@@ -439,12 +466,13 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
     for (int j = 0; j < C; ++j) sums[j] += s.part[j] * inv;
   }
   __syncwarp();
+  float* s_sums = reinterpret_cast<float*>(&s_row[0][0]);     // [kWarps][64 C], the first halves
 #pragma unroll
-  for (int j = 0; j < C; ++j) s_row[warp][first + j] = sums[j];
+  for (int j = 0; j < C; ++j) s_sums[warp * 64 * C + first + j] = sums[j];
   __syncthreads();
   for (int e = threadIdx.x; e < a.E4; e += kWarps * 32) {
     float v = 0.f;
-    for (int k = 0; k < kWarps; ++k) v += s_row[k][e];
+    for (int k = 0; k < kWarps; ++k) v += s_sums[k * 64 * C + e];
     a.psum[(size_t)blockIdx.x * a.E4 + e] = e < a.E ? v : 0.f;
     a.hist[(size_t)blockIdx.x * a.E4 + e] = e < a.E ? s_hist[e] : 0;
   }

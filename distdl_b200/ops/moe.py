@@ -177,7 +177,7 @@ def _choose(logits, E, k, how):
         c = c + bias.double()
     elif groups == 1 or group_score == "max":
         c = l                                               # the same order, also where scores are no longer told apart
-    c = c.masked_fill(l == -math.inf, -math.inf).masked_fill(torch.isnan(l), math.inf)
+    c = c.masked_fill((l == -math.inf) | torch.isnan(c), -math.inf).masked_fill(torch.isnan(l), math.inf)
     if score == "softmax":
         c = c.masked_fill(l == math.inf, math.inf)
     if top_groups < groups:
@@ -210,8 +210,8 @@ def route(logits: torch.Tensor, num_experts: int, k: int, capacity: int, *, scor
       group counts what its best expert does (``group_score="max"``) or its two best together (``"top2"``).
     * ``renormalize``: the weights of a token add up to ``scale``; else they are ``scale`` times the scores.
 
-    Equal scores go to the lowest expert, and scores are told apart as exact arithmetic would.  An expert with a logit of
-    -inf is never chosen; where fewer than ``k`` are left the places have id -1, slot -1 and weight 0, and a row of -inf (a
+    Equal scores go to the lowest expert, and scores are told apart as exact arithmetic would.  An expert with a logit or a
+    bias of -inf is never chosen; where fewer than ``k`` are left the places have id -1, slot -1 and weight 0, and a row of -inf (a
     padding token) routes nowhere and adds nothing to ``prob_sum``.  A NaN makes the token's weights NaN.  (With all settings
     at their defaults and up to 64 experts every logit is a finite number, and scores are told apart in fp32.)  bf16, fp16 and
     fp32 logits of up to 512 experts, with 32 choices and 32 groups at most, run on the kernels."""

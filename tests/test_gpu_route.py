@@ -189,6 +189,25 @@ def test_far_logits():
     assert ids.tolist() == [2, 0, 1, 3, 1, 3] and torch.isfinite(w).all() and torch.isfinite(prob).all()
 
 
+def test_biases_that_take_experts_out():
+    """-inf takes an expert out; a bias far below the others' leaves it to the end, and leaves the others told apart."""
+    torch.manual_seed(14)
+    logits = torch.randn(200, 40, device="cuda")
+    for low in (-math.inf, -1e9, -1e30):
+        bias = torch.randn(40, device="cuda") * 0.1
+        bias[::3] = low
+        for how in (dict(score="sigmoid"), dict(score="softmax", groups=8, top_groups=5, group_score="top2")):
+            host = dict(how, bias=bias.cpu())
+            ids = moe.route(logits, 40, 8, 200, bias=bias, **how)[2].cpu().long()
+            # (bias -inf: as the definition with the logit -inf)
+            l64 = logits.double().cpu()
+            want = definition(l64, 40, 8, 200, **host)[2] if low > -math.inf else None
+            assert want is None or torch.equal(ids, want)
+            assert low > -math.inf or not (ids[ids >= 0] % 3 == 0).any()
+    ids = moe.route(logits, 40, 30, 200, bias=bias, score="sigmoid")[2].reshape(200, 30)
+    assert (ids[:, :26] % 3 != 0).all() and (ids[:, 26:] % 3 == 0).all()
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_a_nan_shows_in_its_token_alone(score):
     logits = torch.randn(9, 24, device="cuda")
