@@ -20,6 +20,7 @@
 
 #include <cuda_fp16.h>
 
+#include <cstring>
 #include <type_traits>
 
 using namespace dd;
@@ -668,103 +669,81 @@ int dispatch_type(HeadArgs& a, int dtype, int* parts, cudaStream_t stream) {
   return DD_ERR_BAD_ARG;
 }
 
-int fill(HeadArgs& a, long long tokens, int hq, int hk, int rest, int hd, int rd, int neighbours, const double* turns,
-         float magnitude, const void* positions, int wide_positions, long long offset, long long seq) {
-  if (tokens < 0 || hq < 0 || hk < 0 || rest < 0 || hd < 1 || rd < 0 || rd > hd || rd % 2 != 0) return DD_ERR_BAD_ARG;
-  if (rd > 0 && turns == nullptr) return DD_ERR_BAD_ARG;
-  if (rd > 0 && seq < 1) return DD_ERR_BAD_ARG;
-  if (hd > 2 * kMaxPairs || tokens > 0x3fffffffLL) return DD_ERR_TOO_LARGE;
-  a.tokens = (unsigned)tokens;
-  a.seq = seq < 1 ? 1u : seq > 0x3fffffffLL ? 0x3fffffffu : (unsigned)seq;
-  a.heads[0] = hq; a.heads[1] = hk; a.heads[2] = rest;
-  a.hd = hd; a.rd = rd; a.neighbours = neighbours;
-  a.positions = positions; a.wide_positions = wide_positions; a.offset = offset;
-  a.magnitude = magnitude;
-  a.inv_hd = 1.f / (float)hd;
-  for (int i = 0; i < rd / 2; ++i) a.turns[i] = turns[i];
-  return DD_OK;
-}
-
 }  // namespace
 
 // CTAs (and rows of the backward pass's scratch) at most.
 DD_API int dd_heads_parts() { return current_sm_count() * kCtasPerSm; }
 
-// out = x with the leading `nheads` of `heads` heads rotated (sign -1: backwards); with out == x the other heads are left
-// alone, else they are copied.  Tensors [tokens, heads, hd] by token and head stride in elements; dtype 0 bf16, 1 fp16,
-// 2 fp32; turns[rd / 2]: frequencies in turns per position (host memory); positions [seq] on the device (4 or 8 bytes
-// each) of token % seq, or null for offset + token % seq.
-DD_API int dd_rotate_heads(const void* x, long long x_row, long long x_head, void* out, long long out_row, long long out_head,
-                           long long tokens, int heads, int nheads, int hd, int rd, int neighbours, const double* turns,
-                           float magnitude, float sign, const void* positions, int wide_positions, long long offset,
-                           long long seq, int dtype, void* stream) {
-  HeadArgs a = {};
-  if (nheads > heads) return DD_ERR_BAD_ARG;
-  const int r = fill(a, tokens, nheads, 0, x == out ? 0 : heads - nheads, hd, rd, neighbours, turns, magnitude, positions,
-                     wide_positions, offset, seq);
-  if (r) return r;
-  if (tokens == 0 || a.heads[0] + a.heads[2] == 0) return DD_OK;
-  if (x == nullptr || out == nullptr) return DD_ERR_BAD_ARG;
-  a.x = x; a.x_row = x_row; a.x_head = x_head;
-  a.out = out; a.out_row = out_row; a.out_head = out_head;
-  a.sign = sign;
-  int parts = 0;
-  return dispatch_type<kRotate>(a, dtype, &parts, reinterpret_cast<cudaStream_t>(stream));
-}
+// A call, packed by the caller: ctypes takes longer for thirty arguments than a launch does.  Tensors [tokens, hq + hk + rest,
+// hd] by address, token and head stride (in elements; unit stride inside a head), dtype 0 bf16, 1 fp16, 2 fp32.
+//   pass 0 (rotation)  out = x with the first hq heads turned (sign -1: backwards); the others are copied, or with out == x left
+//                      alone (hk is 0)
+//   pass 1 (norm)      out = x with the first hq heads normed with wq and turned, the next hk with wk, the others as above
+//   pass 2 (backward)  out = dx from x and dy (out of place); dwq, dwk [hd] of the weights' type (null: not wanted), or with
+//                      accumulate added to what is there, fp32; partial: dd_heads_parts() * 2 * hd floats where they are wanted
+// Weights [hd] of x's type, or fp32 with wide_weights, or null.  turns [rd / 2]: frequencies in turns per position (host
+// memory); positions [seq] on the device (4 or, wide_positions, 8 bytes each) of token % seq, or null for offset + token % seq.
+struct HeadsCall {
+  const void *x, *dy;
+  void* out;
+  const void *wq, *wk;
+  void *dwq, *dwk;
+  float* partial;
+  const void* positions;
+  const double* turns;
+  long long x_row, x_head, dy_row, dy_head, out_row, out_head, tokens, offset, seq;
+  int pass, dtype, hq, hk, rest, hd, rd, neighbours, wide_weights, wide_positions, accumulate;
+  float magnitude, sign, eps;
+};
+static_assert(sizeof(HeadsCall) == 19 * 8 + 14 * 4, "packed without holes");
 
-// out = the first hq heads of x normed with weight wq and rotated, the next hk with wk, the `rest` behind them copied (left
-// alone with out == x).  Weights [hd] of x's type, or fp32 with wide_weights, or null.
-DD_API int dd_norm_heads_fwd(const void* x, long long x_row, long long x_head, void* out, long long out_row, long long out_head,
-                             const void* wq, const void* wk, int wide_weights, float eps, long long tokens, int hq, int hk,
-                             int rest, int hd, int rd, int neighbours, const double* turns, float magnitude,
-                             const void* positions, int wide_positions, long long offset, long long seq, int dtype,
-                             void* stream) {
+DD_API int dd_heads(const void* packed, int bytes, void* stream) {
+  HeadsCall c;
+  if (packed == nullptr || bytes != (int)sizeof c) return DD_ERR_BAD_ARG;
+  memcpy(&c, packed, sizeof c);
+  const bool back = c.pass == kBackward;
+  if (c.pass < kRotate || c.pass > kBackward || (c.pass == kRotate && c.hk != 0)) return DD_ERR_BAD_ARG;
+  if (c.tokens < 0 || c.hq < 0 || c.hk < 0 || c.rest < 0 || c.hd < 1 || c.rd < 0 || c.rd > c.hd || c.rd % 2 != 0)
+    return DD_ERR_BAD_ARG;
+  if (c.rd > 0 && (c.turns == nullptr || c.seq < 1)) return DD_ERR_BAD_ARG;
+  if (c.dtype < 0 || c.dtype > 2) return DD_ERR_BAD_ARG;
+  if (c.hd > 2 * kMaxPairs || c.tokens > 0x3fffffffLL) return DD_ERR_TOO_LARGE;
+  const bool weights = back && (c.dwq != nullptr || c.dwk != nullptr);
+  if (weights && c.partial == nullptr) return DD_ERR_BAD_ARG;
   HeadArgs a = {};
-  const int r = fill(a, tokens, hq, hk, x == out ? 0 : rest, hd, rd, neighbours, turns, magnitude, positions, wide_positions,
-                     offset, seq);
-  if (r) return r;
-  if (tokens == 0 || a.heads[0] + a.heads[1] + a.heads[2] == 0) return DD_OK;
-  if (x == nullptr || out == nullptr) return DD_ERR_BAD_ARG;
-  a.x = x; a.x_row = x_row; a.x_head = x_head;
-  a.out = out; a.out_row = out_row; a.out_head = out_head;
-  a.wq = wq; a.wk = wk; a.wide_weights = wide_weights; a.eps = eps;
-  a.sign = 1.f;
-  int parts = 0;
-  return dispatch_type<kForward>(a, dtype, &parts, reinterpret_cast<cudaStream_t>(stream));
-}
-
-// Its gradients: dx [tokens, hq + hk + rest, hd] by strides, dwq / dwk [hd] (null: not wanted) of the weights' type, or with
-// accumulate added to what is there, fp32.  partial: dd_heads_parts() * 2 * hd floats of scratch, null if neither is wanted.
-DD_API int dd_norm_heads_bwd(const void* x, long long x_row, long long x_head, const void* dy, long long dy_row,
-                             long long dy_head, void* dx, long long dx_row, long long dx_head, const void* wq, const void* wk,
-                             int wide_weights, float eps, void* dwq, void* dwk, int accumulate, float* partial,
-                             long long tokens, int hq, int hk, int rest, int hd, int rd, int neighbours, const double* turns,
-                             float magnitude, const void* positions, int wide_positions, long long offset, long long seq,
-                             int dtype, void* stream) {
-  HeadArgs a = {};
-  const int r = fill(a, tokens, hq, hk, rest, hd, rd, neighbours, turns, magnitude, positions, wide_positions, offset, seq);
-  if (r) return r;
-  if ((dwq != nullptr || dwk != nullptr) && partial == nullptr) return DD_ERR_BAD_ARG;
+  a.x = c.x; a.x_row = c.x_row; a.x_head = c.x_head;
+  a.out = c.out; a.out_row = c.out_row; a.out_head = c.out_head;
+  a.tokens = (unsigned)c.tokens;
+  a.seq = c.seq < 1 ? 1u : c.seq > 0x3fffffffLL ? 0x3fffffffu : (unsigned)c.seq;
+  a.heads[0] = c.hq; a.heads[1] = c.hk; a.heads[2] = !back && c.x == c.out ? 0 : c.rest;
+  a.hd = c.hd; a.rd = c.rd; a.neighbours = c.neighbours;
+  a.positions = c.positions; a.wide_positions = c.wide_positions; a.offset = c.offset;
+  a.magnitude = c.magnitude;
+  a.inv_hd = 1.f / (float)c.hd;
+  a.sign = back ? -1.f : c.pass == kRotate ? c.sign : 1.f;
+  for (int i = 0; i < c.rd / 2; ++i) a.turns[i] = c.turns[i];
+  if (c.pass != kRotate) { a.wq = c.wq; a.wk = c.wk; a.wide_weights = c.wide_weights; a.eps = c.eps; }
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   int parts = 0;
-  if (tokens > 0 && hq + hk + rest > 0) {
-    if (x == nullptr || dy == nullptr || dx == nullptr) return DD_ERR_BAD_ARG;
-    a.x = x; a.x_row = x_row; a.x_head = x_head;
-    a.dy = dy; a.dy_row = dy_row; a.dy_head = dy_head;
-    a.out = dx; a.out_row = dx_row; a.out_head = dx_head;
-    a.wq = wq; a.wk = wk; a.wide_weights = wide_weights; a.eps = eps;
-    a.partial = dwq != nullptr || dwk != nullptr ? partial : nullptr;
-    a.sign = -1.f;
-    const int e = dispatch_type<kBackward>(a, dtype, &parts, st);
+  if (c.tokens > 0 && a.heads[0] + a.heads[1] + a.heads[2] > 0) {
+    if (c.x == nullptr || c.out == nullptr || (back && c.dy == nullptr)) return DD_ERR_BAD_ARG;
+    if (back) {
+      a.dy = c.dy; a.dy_row = c.dy_row; a.dy_head = c.dy_head;
+      a.partial = weights ? c.partial : nullptr;
+    }
+    const int e = c.pass == kRotate    ? dispatch_type<kRotate>(a, c.dtype, &parts, st)
+                  : c.pass == kForward ? dispatch_type<kForward>(a, c.dtype, &parts, st)
+                                       : dispatch_type<kBackward>(a, c.dtype, &parts, st);
     if (e) return e;
   }
-  if (dwq == nullptr && dwk == nullptr) return DD_OK;
-  const int grid = (2 * hd + 31) / 32;                        // (no tokens: parts = 0, zeros)
-  if (accumulate || wide_weights || dtype == 2)
-    heads_dw_kernel<float><<<grid, 256, 0, st>>>(partial, parts, hd, (float*)dwq, (float*)dwk, accumulate);
-  else if (dtype == 1)
-    heads_dw_kernel<__half><<<grid, 256, 0, st>>>(partial, parts, hd, (__half*)dwq, (__half*)dwk, 0);
+  if (!weights) return DD_OK;
+  const int grid = (2 * c.hd + 31) / 32;                      // (no tokens: parts = 0, zeros)
+  if (c.accumulate || c.wide_weights || c.dtype == 2)
+    heads_dw_kernel<float><<<grid, 256, 0, st>>>(c.partial, parts, c.hd, (float*)c.dwq, (float*)c.dwk, c.accumulate);
+  else if (c.dtype == 1)
+    heads_dw_kernel<__half><<<grid, 256, 0, st>>>(c.partial, parts, c.hd, (__half*)c.dwq, (__half*)c.dwk, 0);
   else
-    heads_dw_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(partial, parts, hd, (__nv_bfloat16*)dwq, (__nv_bfloat16*)dwk, 0);
+    heads_dw_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(c.partial, parts, c.hd, (__nv_bfloat16*)c.dwq,
+                                                         (__nv_bfloat16*)c.dwk, 0);
   return (int)cudaGetLastError();
 }

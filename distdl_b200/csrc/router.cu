@@ -30,6 +30,8 @@
 
 #include <cuda_fp16.h>
 
+#include <cstring>
+
 using namespace dd;
 
 namespace {
@@ -675,40 +677,58 @@ DD_API int dd_route_words(int tokens, int E) {
   return 2 * ((tokens - 1) / rows_of(tokens) + 1) * ((E + 3) / 4 * 4);
 }
 
-// logits [tokens, ld], the first E columns (dtype 0 bf16, 1 fp16, 2 fp32); bias [E] fp32 or null; ids, w, slot [tokens * k];
-// counts, prob_sum [E]; scratch: `words` words, dd_route_words or more, 16-byte aligned.
-DD_API int dd_route_fwd(const void* logits, int ld, int dtype, int tokens, int E, int k, int capacity, const float* bias,
-                        int groups, int top_groups, int group_sum, int sigmoid, int renormalize, float scale, int* ids,
-                        float* w, int* slot, int* counts, float* prob_sum, int* scratch, long long words,
-                        void* stream) {
+// A call, packed by the caller (ctypes takes longer for twenty arguments than a launch does).  logits [tokens, ld], the first E
+// columns (dtype 0 bf16, 1 fp16, 2 fp32); bias [E] fp32 or null; ids, w, slot [tokens * k]; counts, prob_sum [E]; scratch:
+// `words` words, dd_route_words or more, 16-byte aligned.
+struct RouteCall {
+  const void* logits;
+  const float* bias;
+  int* ids;
+  float* w;
+  int *slot, *counts;
+  float* prob_sum;
+  int* scratch;
+  long long words;
+  int ld, dtype, tokens, E, k, capacity, groups, top_groups, group_sum, sigmoid, renormalize;
+  float scale;
+};
+static_assert(sizeof(RouteCall) == 9 * 8 + 12 * 4, "packed without holes");
+
+DD_API int dd_route_fwd(const void* packed, int bytes, void* stream) {
+  RouteCall c;
+  if (packed == nullptr || bytes != (int)sizeof c) return DD_ERR_BAD_ARG;
+  memcpy(&c, packed, sizeof c);
   RouteArgs a = {};
   int C;
-  const int size = dtype == 2 ? 4 : 2;
-  if (dtype < 0 || dtype > 2 || !fill(a, logits, ld, size, tokens, E, k, sigmoid, renormalize, scale, &C)) return DD_ERR_BAD_ARG;
-  if (groups < 1 || groups > kMaxGroups || E % groups != 0 || top_groups < 1 || top_groups > groups) return DD_ERR_BAD_ARG;
-  if (ids == nullptr || w == nullptr || slot == nullptr || counts == nullptr || prob_sum == nullptr || scratch == nullptr)
+  const int size = c.dtype == 2 ? 4 : 2;
+  if (c.dtype < 0 || c.dtype > 2 || !fill(a, c.logits, c.ld, size, c.tokens, c.E, c.k, c.sigmoid, c.renormalize, c.scale, &C))
     return DD_ERR_BAD_ARG;
-  if (reinterpret_cast<uintptr_t>(scratch) % 16 != 0) return DD_ERR_ALIGN;
-  const int chunks = (tokens - 1) / a.rows + 1;
-  if (words < 2LL * chunks * a.E4) return DD_ERR_BAD_ARG;
-  a.bias = bias;
-  a.groups = top_groups == groups ? 1 : groups;               // (all groups: no choice among them)
-  a.top_groups = top_groups; a.size = E / groups; a.group_sum = group_sum != 0;
-  a.by_logit = bias == nullptr && !(a.groups > 1 && a.group_sum && a.size > 1);
+  if (c.groups < 1 || c.groups > kMaxGroups || c.E % c.groups != 0 || c.top_groups < 1 || c.top_groups > c.groups)
+    return DD_ERR_BAD_ARG;
+  if (c.ids == nullptr || c.w == nullptr || c.slot == nullptr || c.counts == nullptr || c.prob_sum == nullptr ||
+      c.scratch == nullptr)
+    return DD_ERR_BAD_ARG;
+  if (reinterpret_cast<uintptr_t>(c.scratch) % 16 != 0) return DD_ERR_ALIGN;
+  const int chunks = (c.tokens - 1) / a.rows + 1;
+  if (c.words < 2LL * chunks * a.E4) return DD_ERR_BAD_ARG;
+  a.bias = c.bias;
+  a.groups = c.top_groups == c.groups ? 1 : c.groups;         // (all groups: no choice among them)
+  a.top_groups = c.top_groups; a.size = c.E / c.groups; a.group_sum = c.group_sum != 0;
+  a.by_logit = c.bias == nullptr && !(a.groups > 1 && a.group_sum && a.size > 1);
   const int lanes = a.size / C;
   a.lanes = a.size % C == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
-  a.ids = ids; a.w = w;
-  a.hist = scratch;
-  a.psum = reinterpret_cast<float*>(scratch + (size_t)chunks * a.E4);
+  a.ids = c.ids; a.w = c.w;
+  a.hist = c.scratch;
+  a.psum = reinterpret_cast<float*>(c.scratch + (size_t)chunks * a.E4);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int e = dtype == 0   ? forward<__nv_bfloat16>(a, C, chunks, s)
-                : dtype == 1 ? forward<__half>(a, C, chunks, s)
-                             : forward<float>(a, C, chunks, s);
+  const int e = c.dtype == 0   ? forward<__nv_bfloat16>(a, C, chunks, s)
+                : c.dtype == 1 ? forward<__half>(a, C, chunks, s)
+                               : forward<float>(a, C, chunks, s);
   if (e) return e;
   const int per_cta = kMostRows / a.rows;
-  return launch_ahead(route_slot_kernel, dim3((chunks - 1) / per_cta + 1), dim3(kSlotThreads), 0, s, true, (const int*)ids,
-                      tokens, k, E, a.E4, capacity, (const int*)a.hist, (const float*)a.psum, chunks, a.rows, per_cta, counts,
-                      prob_sum, slot);
+  return launch_ahead(route_slot_kernel, dim3((chunks - 1) / per_cta + 1), dim3(kSlotThreads), 0, s, true, (const int*)c.ids,
+                      c.tokens, c.k, c.E, a.E4, c.capacity, (const int*)a.hist, (const float*)a.psum, chunks, a.rows, per_cta,
+                      c.counts, c.prob_sum, c.slot);
 }
 
 // dlogits [tokens, ld] from the gradients of w (dw [tokens, k], or null) and of prob_sum (dprob [E], or null).

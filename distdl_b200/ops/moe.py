@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -69,8 +70,8 @@ class _RouterFn(torch.autograd.Function):
 
 
 _native.declare("dd_route_words", [_i, _i])
-_native.declare("dd_route_fwd", [_v, _i, _i, _i, _i, _i, _i, _v, _i, _i, _i, _i, _i, _f, _v, _v, _v, _v, _v, _v,
-                                 ctypes.c_longlong, _v])
+_native.declare("dd_route_fwd", [ctypes.c_char_p, _i, _v])
+_ROUTE_CALL = struct.Struct("=8Qq11if")           # struct RouteCall of csrc/router.cu
 _native.declare("dd_route_bwd", [_v, _i, _i, _i, _i, _i, _i, _i, _f, _v, _v, _v, _v, _v, _v])
 _DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _MOST_EXPERTS, _MOST_CHOICES, _MOST_GROUPS = 512, 32, 32
@@ -88,9 +89,10 @@ def _route_forward(logits, E, k, capacity, how):
     prob_sum = torch.empty(E, dtype=torch.float32, device=dev)
     words = _native.lib().dd_route_words(T, E)
     scratch = torch.empty(words, dtype=torch.int32, device=dev)
-    call_on(logits, "dd_route_fwd", logits.data_ptr(), ld, _DTYPE[logits.dtype], T, E, k, capacity, ptr(bias), groups,
-            top_groups, int(group_score == "top2"), int(score == "sigmoid"), int(renormalize), scale, ids.data_ptr(),
-            w.data_ptr(), slot.data_ptr(), counts.data_ptr(), prob_sum.data_ptr(), scratch.data_ptr(), words)
+    call_on(logits, "dd_route_fwd", _ROUTE_CALL.pack(
+        logits.data_ptr(), ptr(bias), ids.data_ptr(), w.data_ptr(), slot.data_ptr(), counts.data_ptr(), prob_sum.data_ptr(),
+        scratch.data_ptr(), words, ld, _DTYPE[logits.dtype], T, E, k, capacity, groups, top_groups, group_score == "top2",
+        score == "sigmoid", renormalize, scale), _ROUTE_CALL.size)
     return w, prob_sum, ids, slot, counts
 
 
@@ -223,9 +225,10 @@ def route(logits: torch.Tensor, num_experts: int, k: int, capacity: int, *, scor
     if use_native(logits) and logits.dtype in _DTYPE and E <= _MOST_EXPERTS and k <= _MOST_CHOICES \
             and groups <= _MOST_GROUPS and logits.numel() and logits.shape[0] * k < 2 ** 31:
         logits = logits if logits.is_contiguous() else logits.contiguous()
+        capacity = min(int(capacity), 2 ** 31 - 1)
         if torch.is_grad_enabled() and logits.requires_grad:
-            return _RouteFn.apply(logits, E, k, int(capacity), how)
-        return _route_forward(logits, E, k, int(capacity), how)
+            return _RouteFn.apply(logits, E, k, capacity, how)
+        return _route_forward(logits, E, k, capacity, how)
     ids = _choose(logits, E, k, how)
     w, prob_sum = _route_weights(logits, E, ids, how)
     slot, counts = _slots_in_order(ids.reshape(-1), E, capacity)

@@ -5,6 +5,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 from dataclasses import dataclass, fields
 from typing import Optional
 
@@ -14,13 +15,11 @@ from .. import _native
 from ._util import call_on, main_grad_now, ptr, use_native
 from .pad import _plain
 
-_v, _i, _l, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
-_native.declare("dd_rotate_heads", [_v, _l, _l, _v, _l, _l, _l, _i, _i, _i, _i, _i, _v, _f, _f, _v, _i, _l, _l, _i, _v])
-_native.declare("dd_norm_heads_fwd", [_v, _l, _l, _v, _l, _l, _v, _v, _i, _f, _l, _i, _i, _i, _i, _i, _i, _v, _f, _v, _i, _l,
-                                      _l, _i, _v])
-_native.declare("dd_norm_heads_bwd", [_v, _l, _l, _v, _l, _l, _v, _l, _l, _v, _v, _i, _f, _v, _v, _i, _v, _l, _i, _i, _i, _i,
-                                      _i, _i, _v, _f, _v, _i, _l, _l, _i, _v])
+_native.declare("dd_heads", [ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p])
 _native.declare("dd_heads_parts", [])
+# struct HeadsCall of csrc/heads.cu: ten addresses, nine long numbers, eleven numbers, three fp32 values
+_CALL = struct.Struct("=10Q9q11i3f")
+_ROTATE, _FORWARD, _BACKWARD = 0, 1, 2
 
 _DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _SCALINGS = (None, "linear", "ntk", "yarn", "bands")
@@ -225,30 +224,26 @@ def _unit(t):
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
-def _heads(t):
-    stride = t.stride()
-    return t.data_ptr(), stride[0], stride[1]
-
-
-def _turn_args(where, head_dim):
+def _call(kind, x, out, hq, hkv, where, sign=1.0, wq=None, wk=None, eps=0.0, dy=None, dwq=None, dwk=None, partial=None,
+          accumulate=False):
+    """One call of the kernels on ``[tokens, heads, head_dim]`` tensors."""
+    tokens, heads, hd = x.shape
+    xs, os = x.stride(), out.stride()
+    ds = xs if dy is None else dy.stride()
     rotary, positions, seq, offset = where
-    if rotary is None:
-        return (0, 0, 0, 1.0), (0, 0, 0, 1)
-    place = (0, 0, offset, seq) if positions is None else (positions.data_ptr(), int(positions.dtype == torch.int64), 0, seq)
-    return rotary._plan(head_dim)[:4], place
-
-
-def _rotate(src, dst, nheads, where, sign):
-    tokens, heads, hd = src.shape
-    (dim, near, address, scale), place = _turn_args(where, hd)
-    call_on(src, "dd_rotate_heads", *_heads(src), *_heads(dst), tokens, heads, nheads, hd, dim, near, address, scale, sign,
-            *place, _DTYPE[src.dtype])
+    dim, near, address, scale = (0, 0, 0, 1.0) if rotary is None else rotary._plan(hd)[:4]
+    w = wk if wq is None else wq
+    call_on(x, "dd_heads", _CALL.pack(
+        x.data_ptr(), 0 if dy is None else dy.data_ptr(), out.data_ptr(), ptr(wq), ptr(wk), ptr(dwq), ptr(dwk), ptr(partial),
+        0 if positions is None else positions.data_ptr(), address, xs[0], xs[1], ds[0], ds[1], os[0], os[1], tokens, offset, seq,
+        kind, _DTYPE[x.dtype], hq, hkv, heads - hq - hkv, hd, dim, near, w is not None and w.dtype == torch.float32,
+        positions is not None and positions.dtype == torch.int64, accumulate, scale, sign, eps), _CALL.size)
 
 
 def _rotated_copy(qkv, nheads, where, sign):
     src = _unit(qkv)
     out = torch.empty_like(src, memory_format=torch.contiguous_format)
-    _rotate(src, out, nheads, where, sign)
+    _call(_ROTATE, src, out, nheads, 0, where, sign)
     return out
 
 
@@ -288,7 +283,7 @@ class _RopeInPlaceFn(torch.autograd.Function):
         ctx.save_for_backward(where[1])
         ctx.cfg = cfg
         t = qkv.view(layout)
-        _rotate(t, t, nheads, where, 1.0)
+        _call(_ROTATE, t, t, nheads, 0, where)
         return qkv
 
     @staticmethod
@@ -365,7 +360,7 @@ def rope_in_place(qkv, seq, nheads, rotary, offset=0, ranges=None, positions=Non
                          "of their own: use ops.rope")
     if qkv.requires_grad and torch.is_grad_enabled():
         return _RopeInPlaceFn.apply(qkv, (shape, nheads, where))
-    _rotate(read, read, nheads, where, 1.0)
+    _call(_ROTATE, read, read, nheads, 0, where)
     if not qkv.is_inference():
         torch.autograd.graph.increment_version(qkv)
     return qkv
@@ -389,19 +384,10 @@ def _plain_qk_norm_rope(qkv, hq, hkv, wq, wk, eps, where):
     return torch.cat([y.to(qkv.dtype), qkv[:, nh:]], dim=1)
 
 
-def _norm_forward(src, dst, hq, hkv, wq, wk, eps, where):
-    tokens, heads, hd = src.shape
-    (dim, near, address, scale), place = _turn_args(where, hd)
-    w = wk if wq is None else wq
-    call_on(src, "dd_norm_heads_fwd", *_heads(src), *_heads(dst), ptr(wq), ptr(wk),
-            int(w is not None and w.dtype == torch.float32), eps, tokens, hq, hkv, heads - hq - hkv, hd, dim, near, address,
-            scale, *place, _DTYPE[src.dtype])
-
-
 def _normed_copy(qkv, hq, hkv, wq, wk, eps, where):
     src = _unit(qkv)
     out = torch.empty_like(src, memory_format=torch.contiguous_format)
-    _norm_forward(src, out, hq, hkv, wq, wk, eps, where)
+    _call(_FORWARD, src, out, hq, hkv, where, 1.0, wq, wk, eps)
     return out
 
 
@@ -415,20 +401,15 @@ def _parts(device: int) -> int:
 def _norm_backward(x, dy, wq, wk, hq, hkv, eps, where, want, main=(None, None)):
     """(dx, dwq, dwk) of :func:`qk_norm_rope`; ``want``: which weights' gradients; ``main``: fp32 accumulators that they are
     added to instead (both that are wanted, or neither)."""
-    tokens, heads, hd = x.shape
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-    w = wk if wq is None else wq
     accumulate = main[0] is not None or main[1] is not None
     dwq, dwk, partial = main[0], main[1], None
     if want[0] or want[1]:
-        partial = torch.empty(_parts(x.get_device()) * 2 * hd, dtype=torch.float32, device=x.device)
+        partial = torch.empty(_parts(x.get_device()) * 2 * x.shape[2], dtype=torch.float32, device=x.device)
         if not accumulate:
             dwq = torch.empty_like(wq) if want[0] else None
             dwk = torch.empty_like(wk) if want[1] else None
-    (dim, near, address, scale), place = _turn_args(where, hd)
-    call_on(x, "dd_norm_heads_bwd", *_heads(x), *_heads(dy), *_heads(dx), ptr(wq), ptr(wk),
-            int(w is not None and w.dtype == torch.float32), eps, ptr(dwq), ptr(dwk), int(accumulate), ptr(partial), tokens, hq,
-            hkv, heads - hq - hkv, hd, dim, near, address, scale, *place, _DTYPE[x.dtype])
+    _call(_BACKWARD, x, dx, hq, hkv, where, 1.0, wq, wk, eps, dy, dwq, dwk, partial, accumulate)
     return (dx, None, None) if accumulate else (dx, dwq, dwk)
 
 
@@ -513,7 +494,7 @@ def qk_norm_rope_(qkv: torch.Tensor, seq: int, hq: int, hkv: int, q_weight=None,
     if _overlaps(qkv):
         raise ValueError("a tensor that is changed in place must not overlap itself: use ops.qk_norm_rope")
     if native and (qkv.stride(2) == 1 or qkv.shape[2] == 1):
-        _norm_forward(qkv, qkv, hq, hkv, wq, wk, float(eps), where)
+        _call(_FORWARD, qkv, qkv, hq, hkv, where, 1.0, wq, wk, float(eps))
         if not qkv.is_inference():
             torch.autograd.graph.increment_version(qkv)
         return qkv

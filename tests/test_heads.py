@@ -109,17 +109,24 @@ def test_native_entry_points_refuse_bad_sizes_without_a_launch():
     from distdl_b200 import _native
     if not _native.available():
         pytest.skip("the native library is not built")
+    from distdl_b200.ops.rotary import _CALL
     lib = _native.lib()
 
-    def rotate(tokens=4, heads=2, nheads=2, hd=16, dim=16, x=64, turns=None, seq=4):
-        return lib.dd_rotate_heads(x, 32, 16, x, 32, 16, tokens, heads, nheads, hd, dim, 0, turns, 1.0, 1.0, 0, 0, 0, seq, 0, 0)
+    def call(kind=0, tokens=4, hq=2, hk=0, rest=0, hd=16, dim=16, x=64, dy=0, out=128, turns=0, seq=4, dtype=0, dwq=0,
+             size=None):
+        packed = _CALL.pack(x, dy, out, 0, 0, dwq, 0, 0, 0, turns, 32, 16, 32, 16, 32, 16, tokens, 0, seq, kind, dtype, hq, hk,
+                            rest, hd, dim, 0, 0, 0, 0, 1.0, 1.0, 1e-6)
+        return lib.dd_heads(packed, len(packed) if size is None else size, None)
 
-    assert rotate() == 1001                       # frequencies are missing
-    assert rotate(nheads=3) == 1001
-    assert rotate(dim=0, hd=600) == 1003
-    assert rotate(dim=3) == 1001
-    assert rotate(dim=18) == 1001
-    assert rotate(tokens=-1, dim=0) == 1001
-    assert rotate(tokens=1 << 40, dim=0) == 1003
-    assert rotate(tokens=0, dim=0) == 0
-    assert rotate(dim=0, x=0) == 1001
+    assert call() == 1001                         # frequencies are missing
+    assert call(dim=0, kind=3) == 1001 and call(dim=0, size=100) == 1001 and lib.dd_heads(None, 208, None) == 1001
+    assert call(dim=0, hk=1) == 1001              # a rotation of heads of two kinds
+    assert call(dim=0, hq=-1) == 1001 and call(dim=0, rest=-1) == 1001
+    assert call(dim=0, hd=600) == 1003
+    assert call(dim=3, turns=64) == 1001 and call(dim=18, turns=64) == 1001 and call(dim=4, turns=64, seq=0) == 1001
+    assert call(tokens=-1, dim=0) == 1001
+    assert call(tokens=1 << 40, dim=0) == 1003
+    assert call(dim=0, dtype=3) == 1001
+    assert call(dim=0, x=0) == 1001 and call(dim=0, out=0) == 1001 and call(dim=0, kind=2) == 1001
+    assert call(dim=0, kind=2, dy=64, dwq=64) == 1001         # no room for the sums
+    assert call(tokens=0, dim=0) == 0

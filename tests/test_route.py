@@ -93,13 +93,15 @@ def test_native_entry_points_refuse_bad_sizes_without_a_launch():
         pytest.skip("the native library is not built")
     lib = _native.lib()
 
-    def forward(ld=16, dtype=0, tokens=4, E=16, k=2, groups=1, top=1, words=1 << 20, scratch=256, logits=256):
-        return lib.dd_route_fwd(logits, ld, dtype, tokens, E, k, 8, None, groups, top, 0, 0, 1, 1.0, 256, 256, 256, 256, 256,
-                                scratch, words, None)
+    def forward(ld=16, dtype=0, tokens=4, E=16, k=2, groups=1, top=1, words=1 << 20, scratch=256, logits=256, size=None):
+        packed = moe._ROUTE_CALL.pack(logits, 0, 256, 256, 256, 256, 256, scratch, words, ld, dtype, tokens, E, k, 8, groups,
+                                      top, 0, 0, 1, 1.0)
+        return lib.dd_route_fwd(packed, len(packed) if size is None else size, None)
 
+    assert forward(size=16) == 1001 and lib.dd_route_fwd(None, 120, None) == 1001
     assert forward(E=513, ld=600) == 1001 and forward(k=33, E=64, ld=64) == 1001 and forward(k=17) == 1001
     assert forward(ld=15) == 1001 and forward(dtype=3) == 1001 and forward(groups=3, top=1) == 1001
     assert forward(groups=4, top=5) == 1001 and forward(words=31) == 1001 and forward(scratch=260) == 1002
-    assert forward(logits=None) == 1001 and forward(tokens=0) == 1001 and forward(tokens=1 << 30, k=2) == 1001
+    assert forward(logits=0) == 1001 and forward(tokens=0) == 1001 and forward(tokens=1 << 30, k=2) == 1001
     assert lib.dd_route_bwd(256, 16, 0, 4, 16, 2, 0, 1, 1.0, 256, 256, None, None, 264, None) == 1002
     assert lib.dd_route_bwd(256, 16, 0, 4, 16, 2, 0, 1, 1.0, None, 256, None, None, 256, None) == 1001
