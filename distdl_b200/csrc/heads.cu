@@ -156,24 +156,27 @@ __device__ __forceinline__ void sin_cos_turns(float t, float* s, float* c) {
   }
 }
 
-// Sums over the lanes of a group (a power of two, the same for all of the kernel), two side by side.
+// Sums over the lanes of a group, two side by side.  GROUP: lanes of a group, 0: `group` of them (a power of two).
+template <int GROUP>
 __device__ __forceinline__ void group_sums(float& v, float& u, int group) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
-    if (group > o) {
+    if ((GROUP > 0 ? GROUP : group) > o) {
       v += __shfl_xor_sync(0xffffffffu, v, o);
       u += __shfl_xor_sync(0xffffffffu, u, o);
     }
 }
+template <int GROUP>
 __device__ __forceinline__ float group_sum(float v, int group) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
-    if (group > o) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((GROUP > 0 ? GROUP : group) > o) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// What a lane of a group holds of a head: NV vectors of VE components; FULL: every lane has all of them.
-template <typename T, int VE, int NV, int PAIRING, bool FULL>
+// What a lane of a group holds of a head: NV vectors of VE components.  GROUP: lanes of a group that all have their vectors; 0:
+// a.group lanes, some of them without.
+template <typename T, int VE, int NV, int PAIRING, int GROUP>
 struct Lane {
   static constexpr int N = NV * VE, M = N / 2;                // components, pairs of them as they are computed with
   int at[NV];                                                 // first component of each vector, -1: none
@@ -189,15 +192,15 @@ struct Lane {
         const int lanes = half / VE;                          // that hold a vector of each half; the others, what stays
         at[s] = (paired ? g + s * lanes : 2 * lanes + 2 * (g - lanes) + s) * VE;
       } else if constexpr (VE > 1) {
-        at[s] = (s * a.group + g) * VE;
+        at[s] = (s * (GROUP > 0 ? GROUP : a.group) + g) * VE;
       } else {
         const int pair = (s / 2) * a.group + g;
         at[s] = pair >= half ? 2 * pair + s % 2 : a.neighbours ? 2 * pair + s % 2 : pair + s % 2 * half;
       }
-      if (!FULL && at[s] + VE > a.hd) at[s] = -1;
+      if (GROUP == 0 && at[s] + VE > a.hd) at[s] = -1;
     }
   }
-  __device__ __forceinline__ bool has(int s) const { return FULL || at[s] >= 0; }
+  __device__ __forceinline__ bool has(int s) const { return GROUP > 0 || at[s] >= 0; }
   __device__ __forceinline__ int component(int i) const { return has(i / VE) ? at[i / VE] + i % VE : -1; }
   // kInside: the pair of components (2 i, 2 i + 1) of this lane, -1 where they stay
   __device__ __forceinline__ int pair(const HeadArgs& a, int g, int i) const {
@@ -212,9 +215,9 @@ struct Lane {
 };
 
 // Sine and cosine of a lane's pairs at a token's position, and the rotation of what it holds of a head by them.
-template <typename T, int VE, int NV, int PAIRING, bool FULL>
+template <typename T, int VE, int NV, int PAIRING, int GROUP>
 struct Angles {
-  using L = Lane<T, VE, NV, PAIRING, FULL>;
+  using L = Lane<T, VE, NV, PAIRING, GROUP>;
   static constexpr int M = L::M, A = PAIRING == kApart ? M / 2 : 1, I = PAIRING == kInside ? M : 1;
   uint64_t c2[A], s2[A], n2[A];                               // kApart: of two pairs; n2: the sines negated
   float c1[I], s1[I];                                         // kInside
@@ -331,16 +334,17 @@ __device__ __forceinline__ void copy_rest(const HeadArgs& a, const L& lane, cons
 // Forward.  Four heads' loads are in flight together and four heads are worked on side by side: that hides more than a
 // third or fourth CTA per SM or loads a step ahead would (16384 tokens, 48 heads of 128 bf16, us, rotation / norm and rotation:
 // two heads and 4 / 3 CTAs 80.7 / 87.4, two and the next two on their way 75.5 / 72.3, four 64.7 / 67.6).
-template <typename T, int VE, int NV, int PAIRING, int KIND, bool FULL>
+template <typename T, int VE, int NV, int PAIRING, int KIND, int GROUP>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_fwd_kernel(const __grid_constant__ HeadArgs a) {
-  using L = Lane<T, VE, NV, PAIRING, FULL>;
+  using L = Lane<T, VE, NV, PAIRING, GROUP>;
   constexpr int M = L::M, U = NV <= 4 ? 4 : 1;
   __shared__ double turns[kMaxPairs];
   grid_dependency_launch();
   for (int i = threadIdx.x; i < a.rd / 2; i += kThreads) turns[i] = a.turns[i];
   __syncthreads();
-  const int warp = threadIdx.x >> 5, g = threadIdx.x & (a.group - 1);
-  const int per_warp = 32 / a.group, in_warp = (threadIdx.x & 31) / a.group;
+  const int group = GROUP > 0 ? GROUP : a.group;
+  const int warp = threadIdx.x >> 5, g = threadIdx.x & (group - 1);
+  const int per_warp = 32 / group, in_warp = (threadIdx.x & 31) / group;
   const L lane(a, g);
   const unsigned stride = gridDim.x * (kThreads / 32) * per_warp;
   unsigned unit0 = (blockIdx.x * (kThreads / 32) + warp) * per_warp;      // of the kind at hand
@@ -371,14 +375,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_fwd_kernel(const _
           x += a.x_head;
         }
       };
-      Angles<T, VE, NV, PAIRING, FULL> angles;
+      Angles<T, VE, NV, PAIRING, GROUP> angles;
       auto work = [&](int h, auto heads) {
 #pragma unroll
         for (int k = 0; k < heads(); ++k) {
           uint64_t v[M];
           unpack<T, VE, NV>(raw[k], v);
           if constexpr (KIND == kNorm) {
-            const float r = rsqrtf(group_sum(dot(v, v), a.group) * a.inv_hd + a.eps);
+            const float r = rsqrtf(group_sum<GROUP>(dot(v, v), a.group) * a.inv_hd + a.eps);
             const uint64_t r2 = pack_f32x2(r, r);
 #pragma unroll
             for (int i = 0; i < M; ++i) v[i] = mul_f32x2(v[i], mul_f32x2(r2, w[i]));
@@ -416,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_fwd_kernel(const _
   copy_rest<T, VE, NV>(a, lane, a.x, a.x_row, a.x_head, unit0 + in_warp, stride);
 }
 
-// 16 bytes global -> shared by a copy of this thread's own (zeros where it is not to read).
+// 16 bytes global -> shared by a copy of this thread's own; nothing is read and zeros are written where it is not to read.
 __device__ __forceinline__ void copy_async(void* to, const void* from, bool read) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(read ? 16 : 0) : "memory");
 }
@@ -430,9 +434,9 @@ constexpr int kBwdRing = kBwdSteps * 4 * 16 * kThreads;
 // and across the units' ends, and w stays there: the registers are needed for the sums of dw and a head's values (16384
 // tokens, 48 heads of 128 bf16, us: loads into registers a head ahead 138, with w in shared memory 128, the ring 109, with two
 // heads side by side, which spill, 149).
-template <typename T, int VE, int NV, int PAIRING, bool FULL>
+template <typename T, int VE, int NV, int PAIRING, int GROUP>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const __grid_constant__ HeadArgs a) {
-  using L = Lane<T, VE, NV, PAIRING, FULL>;
+  using L = Lane<T, VE, NV, PAIRING, GROUP>;
   constexpr int N = L::N, M = L::M;
   constexpr bool RING = VE > 1;
   constexpr int R = RING ? kBwdSteps : 1;
@@ -442,8 +446,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
   __shared__ float reduced[kThreads / 32][2 * kMaxPairs];
   grid_dependency_launch();
   for (int i = threadIdx.x; i < a.rd / 2; i += kThreads) turns[i] = a.turns[i];
-  const int warp = threadIdx.x >> 5, g = threadIdx.x & (a.group - 1);
-  const int per_warp = 32 / a.group, in_warp = (threadIdx.x & 31) / a.group;
+  const int group = GROUP > 0 ? GROUP : a.group;
+  const int warp = threadIdx.x >> 5, g = threadIdx.x & (group - 1);
+  const int per_warp = 32 / group, in_warp = (threadIdx.x & 31) / group;
   const L lane(a, g);
   const unsigned stride = gridDim.x * (kThreads / 32) * per_warp;
   unsigned unit0 = (blockIdx.x * (kThreads / 32) + warp) * per_warp;      // of the kind at hand
@@ -474,8 +479,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
           const bool read = ahead_h < ahead_count && lane.has(s);
           if constexpr (RING) {
             uint8_t* to = ring + ((slot * 2 * NV + s) * kThreads + threadIdx.x) * 16;
-            copy_async(to, read ? x + lane.at[s] : reinterpret_cast<const T*>(a.x), read);
-            copy_async(to + NV * kThreads * 16, read ? dy + lane.at[s] : reinterpret_cast<const T*>(a.x), read);
+            copy_async(to, x + lane.at[s], read);
+            copy_async(to + NV * kThreads * 16, dy + lane.at[s], read);
           } else {
             clear(rx[s]);
             clear(rd[s]);
@@ -495,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
     for (; unit0 < units; unit0 += stride) {
       const Unit u(a, kind, unit0 + in_warp, unit0 + in_warp < units);
       T* out = reinterpret_cast<T*>(a.out) + (long long)u.token * a.out_row + u.head * a.out_head;
-      Angles<T, VE, NV, PAIRING, FULL> angles;
+      Angles<T, VE, NV, PAIRING, GROUP> angles;
       angles.set(a, turns, lane, g, u.token);
       for (int h = 0; h < chunk; ++h) {
         fetch(slot == 0 ? R - 1 : slot - 1);
@@ -513,17 +518,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
         unpack<T, VE, NV>(rx, v);
         unpack<T, VE, NV>(rd, d);
         angles.rotate(a, lane, g, d);                       // (a.sign: backwards)
+        if constexpr (VE > 1) {
 #pragma unroll
-        for (int i = 0; i < M; ++i) {
-          if constexpr (VE > 1) {
-            const float2 w = *reinterpret_cast<const float2*>(&weights[lane.has(2 * i / VE) ? lane.at[2 * i / VE] + 2 * i % VE : 0]);
+          for (int i = 0; i < M; i += 2) {
+            const float4 w = *reinterpret_cast<const float4*>(&weights[lane.has(2 * i / VE) ? lane.at[2 * i / VE] + 2 * i % VE : 0]);
             gw[i] = mul_f32x2(d[i], pack_f32x2(w.x, w.y));
-          } else {
-            gw[i] = mul_f32x2(d[i], pack_f32x2(weights[max(lane.at[2 * i], 0)], weights[max(lane.at[2 * i + 1], 0)]));
+            gw[i + 1] = mul_f32x2(d[i + 1], pack_f32x2(w.z, w.w));
           }
+        } else {
+#pragma unroll
+          for (int i = 0; i < M; ++i)
+            gw[i] = mul_f32x2(d[i], pack_f32x2(weights[max(lane.at[2 * i], 0)], weights[max(lane.at[2 * i + 1], 0)]));
         }
         float q = dot(v, v), p = dot(gw, v);
-        group_sums(q, p, a.group);
+        group_sums<GROUP>(q, p, a.group);
         const float r = rsqrtf(q * a.inv_hd + a.eps);
         const float mean = p * r * a.inv_hd;                // of g w u
         const uint64_t r2 = pack_f32x2(r, r), m2 = pack_f32x2(-mean * r, -mean * r);
@@ -551,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
       for (int i = 0; i < N; ++i) {
         const float2 f = unpack_f32x2(sums[i / 2]);
         float v = i % 2 ? f.y : f.x;
-        for (int o = a.group; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        for (int o = group; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         if (in_warp == 0 && lane.component(i) >= 0) reduced[warp][lane.component(i)] = v;
       }
     }
@@ -568,24 +576,27 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
   copy_rest<T, VE, NV>(a, lane, a.dy, a.dy_row, a.dy_head, unit0 + in_warp, stride);
 }
 
-// dw[c] = sum over the CTAs of partial[cta][which][c], always in the same order: a warp per 32 columns of CTAs' rows, the
-// eight warps of a block take every eighth row.
+// dw[c] = sum over the CTAs of partial[cta][which][c], always in the same order: a block per 32 columns, its 32 warps take
+// every 32nd row.
 template <typename W>
-__global__ void __launch_bounds__(256) heads_dw_kernel(const float* __restrict__ partial, int parts, int hd, W* __restrict__ dwq,
-                                                       W* __restrict__ dwk, int accumulate) {
-  __shared__ float red[8][33];
+__global__ void __launch_bounds__(1024) heads_dw_kernel(const float* partial, int parts, int hd, W* dwq, W* dwk,
+                                                        int accumulate) {
+  __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;                       // of the two weights' 2 * hd
   float v = 0.f;
+  grid_dependency_wait();                                     // (launched ahead of the end of the kernel before it)
+  grid_dependency_launch();
   if (c < 2 * hd) {
-#pragma unroll 8
-    for (int p = row; p < parts; p += 8) v += partial[(size_t)p * 2 * hd + c];
+#pragma unroll 10
+    for (int p = row; p < parts; p += 32) v += partial[(size_t)p * 2 * hd + c];
   }
   red[row][lane] = v;
   __syncthreads();
   if (row == 0 && c < 2 * hd) {
     v = 0.f;
-    for (int k = 0; k < 8; ++k) v += red[k][lane];
+#pragma unroll
+    for (int k = 0; k < 32; ++k) v += red[k][lane];
     W* dst = c < hd ? dwq : dwk;
     if (dst != nullptr) {
       dst += c < hd ? c : c - hd;
@@ -600,10 +611,10 @@ constexpr int kChunkHeads = 16;
 
 enum Pass { kRotate = 0, kForward = 1, kBackward = 2 };
 
-template <typename T, int VE, int NV, int PAIRING, bool FULL, int PASS>
+template <typename T, int VE, int NV, int PAIRING, int GROUP, int PASS>
 int launch(const HeadArgs& a, int ctas, cudaStream_t stream) {
   if constexpr (PASS == kBackward) {
-    auto* kernel = heads_bwd_kernel<T, VE, NV, PAIRING, FULL>;
+    auto* kernel = heads_bwd_kernel<T, VE, NV, PAIRING, GROUP>;
     const int smem = VE > 1 ? kBwdRing : 0;
     static bool configured[64] = {false};
     int dev = 0;
@@ -615,7 +626,7 @@ int launch(const HeadArgs& a, int ctas, cudaStream_t stream) {
     }
     kernel<<<ctas, kThreads, smem, stream>>>(a);
   } else {
-    heads_fwd_kernel<T, VE, NV, PAIRING, PASS == kRotate ? kRope : kNorm, FULL><<<ctas, kThreads, 0, stream>>>(a);
+    heads_fwd_kernel<T, VE, NV, PAIRING, PASS == kRotate ? kRope : kNorm, GROUP><<<ctas, kThreads, 0, stream>>>(a);
   }
   return (int)cudaGetLastError();
 }
@@ -652,13 +663,24 @@ int dispatch(HeadArgs& a, int* parts, cudaStream_t stream) {
   const int ctas = (int)(want < most ? want : most);
   *parts = ctas;
   if (!vectors) {
-    if (a.hd <= 128) return launch<T, 1, 4, kInside, false, PASS>(a, ctas, stream);
-    return launch<T, 1, 16, kInside, false, PASS>(a, ctas, stream);
+    if (a.hd <= 128) return launch<T, 1, 4, kInside, 0, PASS>(a, ctas, stream);
+    return launch<T, 1, 16, kInside, 0, PASS>(a, ctas, stream);
   }
-  const bool full = a.hd == 2 * VE * a.group;
-  if (a.neighbours)
-    return full ? launch<T, VE, 2, kInside, true, PASS>(a, ctas, stream) : launch<T, VE, 2, kInside, false, PASS>(a, ctas, stream);
-  return full ? launch<T, VE, 2, kApart, true, PASS>(a, ctas, stream) : launch<T, VE, 2, kApart, false, PASS>(a, ctas, stream);
+  // groups of 4 to 32 lanes that all have their vectors know their size beforehand: shuffles and addresses without questions
+  // (16384 tokens, 48 heads of 128 bf16, backward: 108 -> 98 us)
+  const int full = a.hd == 2 * VE * a.group ? a.group : 0;
+  if (a.neighbours) {
+    if (full == 4) return launch<T, VE, 2, kInside, 4, PASS>(a, ctas, stream);
+    if (full == 8) return launch<T, VE, 2, kInside, 8, PASS>(a, ctas, stream);
+    if (full == 16) return launch<T, VE, 2, kInside, 16, PASS>(a, ctas, stream);
+    if (full == 32) return launch<T, VE, 2, kInside, 32, PASS>(a, ctas, stream);
+    return launch<T, VE, 2, kInside, 0, PASS>(a, ctas, stream);
+  }
+  if (full == 4) return launch<T, VE, 2, kApart, 4, PASS>(a, ctas, stream);
+  if (full == 8) return launch<T, VE, 2, kApart, 8, PASS>(a, ctas, stream);
+  if (full == 16) return launch<T, VE, 2, kApart, 16, PASS>(a, ctas, stream);
+  if (full == 32) return launch<T, VE, 2, kApart, 32, PASS>(a, ctas, stream);
+  return launch<T, VE, 2, kApart, 0, PASS>(a, ctas, stream);
 }
 
 template <int PASS>
@@ -738,12 +760,12 @@ DD_API int dd_heads(const void* packed, int bytes, void* stream) {
   }
   if (!weights) return DD_OK;
   const int grid = (2 * c.hd + 31) / 32;                      // (no tokens: parts = 0, zeros)
-  if (c.accumulate || c.wide_weights || c.dtype == 2)
-    heads_dw_kernel<float><<<grid, 256, 0, st>>>(c.partial, parts, c.hd, (float*)c.dwq, (float*)c.dwk, c.accumulate);
-  else if (c.dtype == 1)
-    heads_dw_kernel<__half><<<grid, 256, 0, st>>>(c.partial, parts, c.hd, (__half*)c.dwq, (__half*)c.dwk, 0);
-  else
-    heads_dw_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(c.partial, parts, c.hd, (__nv_bfloat16*)c.dwq,
-                                                         (__nv_bfloat16*)c.dwk, 0);
-  return (int)cudaGetLastError();
+  auto add = [&](auto* dwq, auto* dwk, int accumulate) {
+    using W = std::remove_pointer_t<decltype(dwq)>;
+    return launch_ahead(heads_dw_kernel<W>, dim3(grid), dim3(1024), 0, st, true, (const float*)c.partial, parts, c.hd, dwq, dwk,
+                        accumulate);
+  };
+  if (c.accumulate || c.wide_weights || c.dtype == 2) return add((float*)c.dwq, (float*)c.dwk, c.accumulate);
+  if (c.dtype == 1) return add((__half*)c.dwq, (__half*)c.dwk, 0);
+  return add((__nv_bfloat16*)c.dwq, (__nv_bfloat16*)c.dwk, 0);
 }
