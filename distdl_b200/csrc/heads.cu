@@ -13,8 +13,10 @@
 //    every position below 2^31, where 32 bits are off by radians), then sin and cos in 32 bits, once per lane for all heads of
 //    a chunk.  The frequencies travel as arguments of the kernel: no table, no copy, nothing to capture or to keep;
 //  * the backward pass recomputes r from x, which it needs anyway.
-// A unit of work is a token's chunk of heads of one kind (query / key / rest); units are dealt to the groups of a grid of two
-// CTAs per SM, kind by kind, so that the lanes of a warp do the same and what belongs to a kind is held once.
+// A unit of work is a token's chunk of heads of one kind (query / key / rest).  Units are dealt to the warps of a grid of two
+// CTAs per SM, kind by kind, so that what belongs to a kind is held once; the heads of a unit to the groups of the warp in turn,
+// so that a warp reads and writes them as they lie in memory (a group with 16 heads for itself, its neighbours with the next
+// token's, 16384 tokens, 48 heads of 128 bf16: rotation 68.4 us, backward 107.9; with four heads 64.6 and 102.5).
 #include "common.cuh"
 #include "runtime.cuh"
 
@@ -52,8 +54,9 @@ struct HeadArgs {
   long long offset;
   unsigned tokens, seq;
   int heads[3];               // query, key and other heads (those are copied; none in place)
-  int chunk[3], chunks[3];    // heads per unit, units per token
+  int chunk[3], chunks[3];    // heads per unit (whole rounds of a warp's groups), units per token
   int hd, rd, group;          // group: lanes per head (a power of two)
+  int queries;                // forward: of the heads of the first kind, those that take wq
   int wide_positions, wide_weights, neighbours;
   float magnitude, sign, eps, inv_hd;
   double turns[kMaxPairs];    // frequency of each pair in turns per position
@@ -293,14 +296,32 @@ __device__ __forceinline__ float weight_of(const HeadArgs& a, int kind, int c) {
   return a.wide_weights ? reinterpret_cast<const float*>(w)[c] : to_f(reinterpret_cast<const T*>(w)[c]);
 }
 
-// A unit of work: heads [first, first + count) of a token, of one kind.
+// The weights of a lane's components, from shared memory.
+template <int VE, int NV, typename L>
+__device__ __forceinline__ void weights_of(const float* weights, const L& lane, uint64_t (&w)[NV * VE / 2]) {
+  if constexpr (VE > 1) {
+#pragma unroll
+    for (int i = 0; i < NV * VE / 2; i += 2) {
+      const float4 f = *reinterpret_cast<const float4*>(&weights[lane.has(2 * i / VE) ? lane.at[2 * i / VE] + 2 * i % VE : 0]);
+      w[i] = pack_f32x2(f.x, f.y);
+      w[i + 1] = pack_f32x2(f.z, f.w);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV / 2; ++i)
+      w[i] = pack_f32x2(weights[max(lane.at[2 * i], 0)], weights[max(lane.at[2 * i + 1], 0)]);
+  }
+}
+
+// A unit of work of a warp: of its heads the group `in_warp` has every per_warp-th, from `head` on, `count` of them.
 struct Unit {
   unsigned token;
   int head, count;
-  __device__ __forceinline__ Unit(const HeadArgs& a, int kind, unsigned unit, bool live) {
-    token = live ? unit / (unsigned)a.chunks[kind] : 0u;
-    const int first = live ? (int)(unit - token * (unsigned)a.chunks[kind]) * a.chunk[kind] : 0;
-    count = live ? min(a.chunk[kind], a.heads[kind] - first) : 0;
+  __device__ __forceinline__ Unit(const HeadArgs& a, int kind, unsigned unit, int in_warp, int per_warp) {
+    token = unit / (unsigned)a.chunks[kind];
+    const int first = (int)(unit - token * (unsigned)a.chunks[kind]) * a.chunk[kind] + in_warp;
+    const int end = min(first - in_warp + a.chunk[kind], a.heads[kind]);
+    count = first < end ? (end - first + per_warp - 1) / per_warp : 0;
     head = first + (kind > 0 ? a.heads[0] : 0) + (kind > 1 ? a.heads[1] : 0);
   }
 };
@@ -308,10 +329,11 @@ struct Unit {
 // The heads behind queries and keys, copied (forward: of x, backward: of dy).
 template <typename T, int VE, int NV, typename L>
 __device__ __forceinline__ void copy_rest(const HeadArgs& a, const L& lane, const void* from, long long row, long long head,
-                                          unsigned unit, unsigned stride) {
+                                          unsigned unit, unsigned stride, int in_warp, int per_warp) {
   const unsigned units = a.tokens * (unsigned)a.chunks[2];
+  const long long step = head * per_warp, out_step = a.out_head * per_warp;
   for (; unit < units; unit += stride) {
-    const Unit u(a, 2, unit, true);
+    const Unit u(a, 2, unit, in_warp, per_warp);
     const T* src = reinterpret_cast<const T*>(from) + (long long)u.token * row + u.head * head;
     T* out = reinterpret_cast<T*>(a.out) + (long long)u.token * a.out_row + u.head * a.out_head;
     constexpr int R = NV <= 4 ? 4 : 1;
@@ -321,103 +343,107 @@ __device__ __forceinline__ void copy_rest(const HeadArgs& a, const L& lane, cons
       for (int k = 0; k < R; ++k)
 #pragma unroll
         for (int s = 0; s < NV; ++s)
-          if (h + k < u.count && lane.has(s)) r[k][s] = load_pack<T, VE>(src + (h + k) * head + lane.at[s]);
+          if (h + k < u.count && lane.has(s)) r[k][s] = load_pack<T, VE>(src + (h + k) * step + lane.at[s]);
 #pragma unroll
       for (int k = 0; k < R; ++k)
 #pragma unroll
         for (int s = 0; s < NV; ++s)
-          if (h + k < u.count && lane.has(s)) store_pack<T, VE>(out + (h + k) * a.out_head + lane.at[s], r[k][s]);
+          if (h + k < u.count && lane.has(s)) store_pack<T, VE>(out + (h + k) * out_step + lane.at[s], r[k][s]);
     }
   }
 }
 
 // Forward.  Four heads' loads are in flight together and four heads are worked on side by side: that hides more than a
 // third or fourth CTA per SM or loads a step ahead would (16384 tokens, 48 heads of 128 bf16, us, rotation / norm and rotation:
-// two heads and 4 / 3 CTAs 80.7 / 87.4, two and the next two on their way 75.5 / 72.3, four 64.7 / 67.6).
+// two heads and 4 / 3 CTAs 80.7 / 87.4, two and the next two on their way 75.5 / 72.3, four 64.7 / 67.6).  Query and key heads
+// are one kind here, which share their angles; their weights are in shared memory.
 template <typename T, int VE, int NV, int PAIRING, int KIND, int GROUP>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_fwd_kernel(const __grid_constant__ HeadArgs a) {
   using L = Lane<T, VE, NV, PAIRING, GROUP>;
   constexpr int M = L::M, U = NV <= 4 ? 4 : 1;
   __shared__ double turns[kMaxPairs];
+  __shared__ __align__(16) float weights[KIND == kNorm ? 2 : 1][KIND == kNorm ? 2 * kMaxPairs : 4];
   grid_dependency_launch();
   for (int i = threadIdx.x; i < a.rd / 2; i += kThreads) turns[i] = a.turns[i];
+  if constexpr (KIND == kNorm) {
+    for (int c = threadIdx.x; c < 2 * a.hd; c += kThreads)
+      weights[c >= a.hd][c >= a.hd ? c - a.hd : c] = weight_of<T>(a, c >= a.hd, c >= a.hd ? c - a.hd : c);
+  }
   __syncthreads();
   const int group = GROUP > 0 ? GROUP : a.group;
   const int warp = threadIdx.x >> 5, g = threadIdx.x & (group - 1);
   const int per_warp = 32 / group, in_warp = (threadIdx.x & 31) / group;
   const L lane(a, g);
-  const unsigned stride = gridDim.x * (kThreads / 32) * per_warp;
-  unsigned unit0 = (blockIdx.x * (kThreads / 32) + warp) * per_warp;      // of the kind at hand
-#pragma unroll 1
-  for (int kind = 0; kind < 2; ++kind) {
-    const unsigned units = a.tokens * (unsigned)a.chunks[kind];
-    uint64_t w[KIND == kNorm ? M : 1];
-    if (KIND == kNorm && unit0 < units) {
+  const unsigned stride = gridDim.x * (kThreads / 32), units = a.tokens * (unsigned)a.chunks[0];
+  const long long x_step = a.x_head * per_warp, out_step = a.out_head * per_warp;
+  unsigned unit = blockIdx.x * (kThreads / 32) + warp;
+  for (; unit < units; unit += stride) {
+    // (every lane of the warp takes part in every step: a group whose heads have ended works on none)
+    const Unit u(a, 0, unit, in_warp, per_warp);
+    const int most = __shfl_sync(0xffffffffu, u.count, 0);    // (no group has more than the first)
+    const T* x = reinterpret_cast<const T*>(a.x) + (long long)u.token * a.x_row + u.head * a.x_head;
+    T* out = reinterpret_cast<T*>(a.out) + (long long)u.token * a.out_row + u.head * a.out_head;
+    Pack<T, VE> raw[U][NV];
+    auto fetch = [&](int h, auto heads) {
 #pragma unroll
-      for (int i = 0; i < M; ++i)
-        w[i] = pack_f32x2(weight_of<T>(a, kind, lane.component(2 * i)), weight_of<T>(a, kind, lane.component(2 * i + 1)));
-    }
-    for (; unit0 < units; unit0 += stride) {
-      // (every lane of the warp takes part in every step: a group without a unit works on none of its heads)
-      const Unit u(a, kind, unit0 + in_warp, unit0 + in_warp < units);
-      const int most = __reduce_max_sync(0xffffffffu, u.count);
-      const T* x = reinterpret_cast<const T*>(a.x) + (long long)u.token * a.x_row + u.head * a.x_head;
-      T* out = reinterpret_cast<T*>(a.out) + (long long)u.token * a.out_row + u.head * a.out_head;
-      Pack<T, VE> raw[U][NV];
-      auto fetch = [&](int h, auto heads) {
+      for (int k = 0; k < heads(); ++k) {
 #pragma unroll
-        for (int k = 0; k < heads(); ++k) {
-#pragma unroll
-          for (int s = 0; s < NV; ++s) {
-            if (h + k < u.count && lane.has(s)) raw[k][s] = load_pack<T, VE>(x + lane.at[s]);
-            else clear(raw[k][s]);
-          }
-          x += a.x_head;
+        for (int s = 0; s < NV; ++s) {
+          if (h + k < u.count && lane.has(s)) raw[k][s] = load_pack<T, VE>(x + lane.at[s]);
+          else clear(raw[k][s]);
         }
-      };
-      Angles<T, VE, NV, PAIRING, GROUP> angles;
-      auto work = [&](int h, auto heads) {
+        x += x_step;
+      }
+    };
+    Angles<T, VE, NV, PAIRING, GROUP> angles;
+    auto work = [&](int h, auto heads) {
 #pragma unroll
-        for (int k = 0; k < heads(); ++k) {
-          uint64_t v[M];
-          unpack<T, VE, NV>(raw[k], v);
-          if constexpr (KIND == kNorm) {
-            const float r = rsqrtf(group_sum<GROUP>(dot(v, v), a.group) * a.inv_hd + a.eps);
-            const uint64_t r2 = pack_f32x2(r, r);
+      for (int k = 0; k < heads(); ++k) {
+        uint64_t v[M];
+        unpack<T, VE, NV>(raw[k], v);
+        if constexpr (KIND == kNorm) {
+          const float r = rsqrtf(group_sum<GROUP>(dot(v, v), a.group) * a.inv_hd + a.eps);
+          const uint64_t r2 = pack_f32x2(r, r);
+          uint64_t w[M];
+          weights_of<VE, NV>(weights[u.head + (h + k) * per_warp >= a.queries], lane, w);
 #pragma unroll
-            for (int i = 0; i < M; ++i) v[i] = mul_f32x2(v[i], mul_f32x2(r2, w[i]));
-          }
-          angles.rotate(a, lane, g, v);
-          if (h + k < u.count) {
-            Pack<T, VE> res[NV];
-            pack<T, VE, NV>(v, res);
-#pragma unroll
-            for (int s = 0; s < NV; ++s)
-              if (lane.has(s)) store_pack<T, VE>(out + lane.at[s], res[s]);
-          }
-          out += a.out_head;
+          for (int i = 0; i < M; ++i) v[i] = mul_f32x2(v[i], mul_f32x2(r2, w[i]));
         }
-      };
-      // U heads at a time, the last ones of a unit (few tokens: its only one) singly
-      const std::integral_constant<int, U> many;
-      const std::integral_constant<int, 1> one;
-      int h = 0;
-      if (most >= U) fetch(0, many);
-      else fetch(0, one);
-      angles.set(a, turns, lane, g, u.token);                 // while the first heads are on their way
-      for (; h + U <= most; h += U) {
-        if (h > 0) fetch(h, many);
-        work(h, many);
+        angles.rotate(a, lane, g, v);
+        if (h + k < u.count) {
+          Pack<T, VE> res[NV];
+          pack<T, VE, NV>(v, res);
+#pragma unroll
+          for (int s = 0; s < NV; ++s)
+            if (lane.has(s)) store_pack<T, VE>(out + lane.at[s], res[s]);
+        }
+        out += out_step;
       }
-      for (; h < most; ++h) {
-        if (h > 0) fetch(h, one);
-        work(h, one);
-      }
+    };
+    // U heads at a time, the last ones of a unit (few tokens: its only one) in twos and singly
+    const std::integral_constant<int, U> many;
+    const std::integral_constant<int, (U > 1 ? 2 : 1)> two;
+    const std::integral_constant<int, 1> one;
+    int h = 0;
+    if (most >= U) fetch(0, many);
+    else if (most >= 2) fetch(0, two);
+    else fetch(0, one);
+    angles.set(a, turns, lane, g, u.token);                   // while the first heads are on their way
+    for (; h + U <= most; h += U) {
+      if (h > 0) fetch(h, many);
+      work(h, many);
     }
-    // the deal goes on where the last kind's ended (its units padded to whole warps, so that every group keeps its place)
-    unit0 -= (units + per_warp - 1) / per_warp * per_warp;
+    if (U > 2 && h + 2 <= most) {
+      if (h > 0) fetch(h, two);
+      work(h, two);
+      h += 2;
+    }
+    if (h < most) {
+      if (h > 0) fetch(h, one);
+      work(h, one);
+    }
   }
-  copy_rest<T, VE, NV>(a, lane, a.x, a.x_row, a.x_head, unit0 + in_warp, stride);
+  copy_rest<T, VE, NV>(a, lane, a.x, a.x_row, a.x_head, unit - units, stride, in_warp, per_warp);
 }
 
 // 16 bytes global -> shared by a copy of this thread's own; nothing is read and zeros are written where it is not to read.
@@ -450,26 +476,27 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
   const int warp = threadIdx.x >> 5, g = threadIdx.x & (group - 1);
   const int per_warp = 32 / group, in_warp = (threadIdx.x & 31) / group;
   const L lane(a, g);
-  const unsigned stride = gridDim.x * (kThreads / 32) * per_warp;
-  unsigned unit0 = (blockIdx.x * (kThreads / 32) + warp) * per_warp;      // of the kind at hand
+  const unsigned stride = gridDim.x * (kThreads / 32);
+  unsigned unit = blockIdx.x * (kThreads / 32) + warp;        // of the kind at hand
 #pragma unroll 1
   for (int kind = 0; kind < 2; ++kind) {
     const unsigned units = a.tokens * (unsigned)a.chunks[kind];
-    const int chunk = a.chunk[kind];
+    const int rounds = a.chunk[kind] / per_warp;              // of a unit, the same for all of them
+    const long long x_step = a.x_head * per_warp, dy_step = a.dy_head * per_warp, out_step = a.out_head * per_warp;
     for (int c = threadIdx.x; c < a.hd; c += kThreads) weights[c] = weight_of<T>(a, kind, c);
     __syncthreads();
     uint64_t sums[M] = {};
 
     Pack<T, VE> rx[NV], rd[NV];
     // the copies' place in the units, ahead of the work's
-    unsigned ahead = unit0;
+    unsigned ahead = unit;
     int ahead_h = 0, ahead_count = 0;
     const T* x = nullptr;
     const T* dy = nullptr;
     auto fetch = [&](int slot) {
       if (ahead < units) {
         if (ahead_h == 0) {
-          const Unit u(a, kind, ahead + in_warp, ahead + in_warp < units);
+          const Unit u(a, kind, ahead, in_warp, per_warp);
           ahead_count = u.count;
           x = reinterpret_cast<const T*>(a.x) + (long long)u.token * a.x_row + u.head * a.x_head;
           dy = reinterpret_cast<const T*>(a.dy) + (long long)u.token * a.dy_row + u.head * a.dy_head;
@@ -487,9 +514,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
             if (read) { rx[s] = load_pack<T, VE>(x + lane.at[s]); rd[s] = load_pack<T, VE>(dy + lane.at[s]); }
           }
         }
-        x += a.x_head;
-        dy += a.dy_head;
-        if (++ahead_h == chunk) { ahead_h = 0; ahead += stride; }
+        x += x_step;
+        dy += dy_step;
+        if (++ahead_h == rounds) { ahead_h = 0; ahead += stride; }
       }
       if constexpr (RING) copy_commit();
     };
@@ -497,12 +524,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
     for (int i = 0; i < R - 1; ++i) fetch(i);
 
     int slot = 0;
-    for (; unit0 < units; unit0 += stride) {
-      const Unit u(a, kind, unit0 + in_warp, unit0 + in_warp < units);
+    for (; unit < units; unit += stride) {
+      const Unit u(a, kind, unit, in_warp, per_warp);
       T* out = reinterpret_cast<T*>(a.out) + (long long)u.token * a.out_row + u.head * a.out_head;
       Angles<T, VE, NV, PAIRING, GROUP> angles;
       angles.set(a, turns, lane, g, u.token);
-      for (int h = 0; h < chunk; ++h) {
+      for (int h = 0; h < rounds; ++h) {
         fetch(slot == 0 ? R - 1 : slot - 1);
         if constexpr (RING) {
           copy_wait<R - 1>();
@@ -518,18 +545,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
         unpack<T, VE, NV>(rx, v);
         unpack<T, VE, NV>(rd, d);
         angles.rotate(a, lane, g, d);                       // (a.sign: backwards)
-        if constexpr (VE > 1) {
+        weights_of<VE, NV>(weights, lane, gw);
 #pragma unroll
-          for (int i = 0; i < M; i += 2) {
-            const float4 w = *reinterpret_cast<const float4*>(&weights[lane.has(2 * i / VE) ? lane.at[2 * i / VE] + 2 * i % VE : 0]);
-            gw[i] = mul_f32x2(d[i], pack_f32x2(w.x, w.y));
-            gw[i + 1] = mul_f32x2(d[i + 1], pack_f32x2(w.z, w.w));
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < M; ++i)
-            gw[i] = mul_f32x2(d[i], pack_f32x2(weights[max(lane.at[2 * i], 0)], weights[max(lane.at[2 * i + 1], 0)]));
-        }
+        for (int i = 0; i < M; ++i) gw[i] = mul_f32x2(d[i], gw[i]);
         float q = dot(v, v), p = dot(gw, v);
         group_sums<GROUP>(q, p, a.group);
         const float r = rsqrtf(q * a.inv_hd + a.eps);
@@ -548,11 +566,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
           for (int s = 0; s < NV; ++s)
             if (lane.has(s)) store_pack<T, VE>(out + lane.at[s], res[s]);
         }
-        out += a.out_head;
+        out += out_step;
       }
     }
     if constexpr (RING) copy_wait<0>();                       // (empty groups: the ring is free for the next kind)
-    unit0 -= (units + per_warp - 1) / per_warp * per_warp;    // as in the forward pass
+    unit -= units;                                            // as in the forward pass
     if (a.partial != nullptr) {
       // the lanes that hold the same components: over the warp by shuffles, over the warps in their order
 #pragma unroll
@@ -573,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
       __syncthreads();
     }
   }
-  copy_rest<T, VE, NV>(a, lane, a.dy, a.dy_row, a.dy_head, unit0 + in_warp, stride);
+  copy_rest<T, VE, NV>(a, lane, a.dy, a.dy_row, a.dy_head, unit, stride, in_warp, per_warp);
 }
 
 // dw[c] = sum over the CTAs of partial[cta][which][c], always in the same order: a block per 32 columns, its 32 warps take
@@ -605,9 +623,10 @@ __global__ void __launch_bounds__(1024) heads_dw_kernel(const float* partial, in
   }
 }
 
-// Heads per unit at most.  More of them share a lane's angles, fewer give more units: as many as leave every group of the
-// grid two units.
-constexpr int kChunkHeads = 16;
+// Heads of a group per unit at most.  More of them share a lane's angles, fewer give more units (as many as leave every warp of
+// the grid two) and keep what the warps are at closer together in memory, which three streams want most (us, as above, 16 / 8 /
+// 4 heads: rotation 65.7 / 71.7 / 70.4, backward 106.4 / 106.6 / 97.0).
+constexpr int kMostRounds = 16, kMostRoundsBackward = 4;
 
 enum Pass { kRotate = 0, kForward = 1, kBackward = 2 };
 
@@ -647,19 +666,20 @@ int dispatch(HeadArgs& a, int* parts, cudaStream_t stream) {
   a.group = 32;
   if (vectors)
     for (a.group = 1; a.group * 2 * VE < a.hd; a.group *= 2) {}
-  const int most = current_sm_count() * kCtasPerSm, groups_per_cta = kThreads / a.group;
+  const int most = current_sm_count() * kCtasPerSm, warps = kThreads / 32, per_warp = 32 / a.group;
   long long units;
-  for (int chunk = kChunkHeads;; chunk /= 2) {
+  for (int rounds = PASS == kBackward ? kMostRoundsBackward : kMostRounds;; rounds /= 2) {
     units = 0;
     for (int k = 0; k < 3; ++k) {
-      a.chunks[k] = (a.heads[k] + chunk - 1) / chunk;
-      a.chunk[k] = a.chunks[k] > 0 ? (a.heads[k] + a.chunks[k] - 1) / a.chunks[k] : 1;
+      a.chunk[k] = rounds * per_warp;
+      if (a.chunk[k] > a.heads[k]) a.chunk[k] = (a.heads[k] + per_warp - 1) / per_warp * per_warp;
+      a.chunks[k] = a.heads[k] > 0 ? (a.heads[k] + a.chunk[k] - 1) / a.chunk[k] : 0;
       units += (long long)a.tokens * a.chunks[k];
     }
-    if (chunk == 1 || units >= 2LL * most * groups_per_cta) break;
+    if (rounds == 1 || units >= 2LL * most * warps) break;
   }
   if (units > 0x3fffffffLL) return DD_ERR_TOO_LARGE;
-  const long long want = (units + groups_per_cta - 1) / groups_per_cta;
+  const long long want = (units + warps - 1) / warps;
   const int ctas = (int)(want < most ? want : most);
   *parts = ctas;
   if (!vectors) {
@@ -737,7 +757,10 @@ DD_API int dd_heads(const void* packed, int bytes, void* stream) {
   a.out = c.out; a.out_row = c.out_row; a.out_head = c.out_head;
   a.tokens = (unsigned)c.tokens;
   a.seq = c.seq < 1 ? 1u : c.seq > 0x3fffffffLL ? 0x3fffffffu : (unsigned)c.seq;
-  a.heads[0] = c.hq; a.heads[1] = c.hk; a.heads[2] = !back && c.x == c.out ? 0 : c.rest;
+  a.heads[0] = back ? c.hq : c.hq + c.hk;
+  a.heads[1] = back ? c.hk : 0;
+  a.heads[2] = !back && c.x == c.out ? 0 : c.rest;
+  a.queries = c.hq;
   a.hd = c.hd; a.rd = c.rd; a.neighbours = c.neighbours;
   a.positions = c.positions; a.wide_positions = c.wide_positions; a.offset = c.offset;
   a.magnitude = c.magnitude;
