@@ -336,7 +336,7 @@ __device__ __forceinline__ void copy_rest(const HeadArgs& a, const L& lane, cons
     const Unit u(a, 2, unit, in_warp, per_warp);
     const T* src = reinterpret_cast<const T*>(from) + (long long)u.token * row + u.head * head;
     T* out = reinterpret_cast<T*>(a.out) + (long long)u.token * a.out_row + u.head * a.out_head;
-    constexpr int R = NV <= 4 ? 4 : 1;
+    constexpr int R = VE > 1 ? 4 : 2;
     for (int h = 0; h < u.count; h += R) {
       Pack<T, VE> r[R][NV];
 #pragma unroll
@@ -360,7 +360,7 @@ __device__ __forceinline__ void copy_rest(const HeadArgs& a, const L& lane, cons
 template <typename T, int VE, int NV, int PAIRING, int KIND, int GROUP>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_fwd_kernel(const __grid_constant__ HeadArgs a) {
   using L = Lane<T, VE, NV, PAIRING, GROUP>;
-  constexpr int M = L::M, U = NV <= 4 ? 4 : 1;
+  constexpr int M = L::M, U = VE > 1 ? 4 : 1;
   __shared__ double turns[kMaxPairs];
   __shared__ __align__(16) float weights[KIND == kNorm ? 2 : 1][KIND == kNorm ? 2 * kMaxPairs : 4];
   grid_dependency_launch();
@@ -659,13 +659,11 @@ int dispatch(HeadArgs& a, int* parts, cudaStream_t stream) {
   constexpr int VE = 16 / sizeof(T);
   const int size = sizeof(T);
   // whole vectors need heads of whole vectors at 16-byte addresses, two vectors per lane of a warp, and pairs that lie inside
-  // a vector or whole vectors apart; else a warp per head and single components
+  // a vector or whole vectors apart; else single components, sixteen per lane
   const bool vectors = a.hd % VE == 0 && a.hd <= 64 * VE && (a.neighbours || a.rd % (2 * VE) == 0) &&
                        aligned(a.x, a.x_row, a.x_head, size) && aligned(a.dy, a.dy_row, a.dy_head, size) &&
                        aligned(a.out, a.out_row, a.out_head, size);
-  a.group = 32;
-  if (vectors)
-    for (a.group = 1; a.group * 2 * VE < a.hd; a.group *= 2) {}
+  for (a.group = 1; a.group * (vectors ? 2 * VE : 16) < a.hd; a.group *= 2) {}
   const int most = current_sm_count() * kCtasPerSm, warps = kThreads / 32, per_warp = 32 / a.group;
   long long units;
   for (int rounds = PASS == kBackward ? kMostRoundsBackward : kMostRounds;; rounds /= 2) {
@@ -682,10 +680,7 @@ int dispatch(HeadArgs& a, int* parts, cudaStream_t stream) {
   const long long want = (units + warps - 1) / warps;
   const int ctas = (int)(want < most ? want : most);
   *parts = ctas;
-  if (!vectors) {
-    if (a.hd <= 128) return launch<T, 1, 4, kInside, 0, PASS>(a, ctas, stream);
-    return launch<T, 1, 16, kInside, 0, PASS>(a, ctas, stream);
-  }
+  if (!vectors) return launch<T, 1, 16, kInside, 0, PASS>(a, ctas, stream);
   // groups of 4 to 32 lanes that all have their vectors know their size beforehand: shuffles and addresses without questions
   // (16384 tokens, 48 heads of 128 bf16, backward: 108 -> 98 us)
   const int full = a.hd == 2 * VE * a.group ? a.group : 0;
