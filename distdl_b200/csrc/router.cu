@@ -202,11 +202,15 @@ __device__ __forceinline__ int choose(const RouteArgs& a, unsigned (&key)[C], in
       __syncwarp();
     }
     const int g = best_of_groups<int>(a, values, 0, b0, b1, step);
-    const int value = a.group_sum ? b0 + b1 : b0;
-    const bool in = among_best(a, value, g, step);
+    // value (24 bits) over what favours the lower number: the best groups one by one, as the experts below
+    unsigned group = g < a.groups ? (unsigned)(a.group_sum ? b0 + b1 : b0) << 5 | (unsigned)(31 - g) : 0u, worst = 0u;
+    bool in = false;
+    for (int i = 0; i < a.top_groups; ++i) {
+      worst = __reduce_max_sync(0xffffffffu, group);
+      if (group == worst) { in = g < a.groups; group = 0u; }
+    }
     if (near >= 0) {
-      const int least = (int)__reduce_min_sync(0xffffffffu, in ? (unsigned)value : 0x7fffffffu);
-      const int most = (int)__reduce_max_sync(0xffffffffu, !in && g < a.groups ? (unsigned)value : 0u);
+      const int least = (int)(worst >> 5), most = (int)(__reduce_max_sync(0xffffffffu, group) >> 5);
       // (of a group with one expert only its value itself would have to be known)
       close = (most > 0 && least - most <= (a.group_sum ? 2 * near : near)) ||
               __any_sync(0xffffffffu, g < a.groups && a.group_sum && a.size > 1 && b0 > 0 && b1 == 0);

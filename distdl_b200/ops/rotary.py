@@ -253,7 +253,8 @@ class _RopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, cfg):
         nheads, where, sign = cfg
-        ctx.save_for_backward(where[1])
+        if where[1] is not None:
+            ctx.save_for_backward(where[1])
         ctx.cfg = cfg
         return _rotated_copy(qkv, nheads, where, sign)
 
@@ -264,7 +265,8 @@ class _RopeFn(torch.autograd.Function):
 
 
 def _turned_back(ctx, d, nheads, where, sign):
-    where = (where[0], ctx.saved_tensors[0], *where[2:])
+    if where[1] is not None:
+        where = (where[0], ctx.saved_tensors[0], *where[2:])     # (which says whether they have been changed since)
     if not _plain(d):                       # under a function transform: elementary operations
         return _plain_rope(d, nheads, where, sign)
     if torch.is_grad_enabled():             # differentiated itself
@@ -280,7 +282,8 @@ class _RopeInPlaceFn(torch.autograd.Function):
     def forward(ctx, qkv, cfg):
         layout, nheads, where = cfg
         ctx.mark_dirty(qkv)
-        ctx.save_for_backward(where[1])
+        if where[1] is not None:
+            ctx.save_for_backward(where[1])
         ctx.cfg = cfg
         t = qkv.view(layout)
         _call(_ROTATE, t, t, nheads, 0, where)
