@@ -2,7 +2,7 @@
 under a profiler:
 
     python -m distdl_b200.utils.profile_case gemm|gemm_wgrad|ag_gemm|gemm_rs|attn_fwd|attn_bwd|rmsnorm|rmsnorm_bwd|
-        add_rmsnorm|router|adamw|xent [launches]
+        add_rmsnorm|router|route|rope|qk_norm|qk_norm_bwd|clip|adamw|xent [launches]
 
 Inputs are larger than the 126 MB L2 where that matters for the DRAM figures
 but stay well under a few GB.
@@ -79,6 +79,26 @@ def main():
         from distdl_b200.ops import moe
         logits = torch.randn(1 << 20, 8, device=dev, dtype=torch.bfloat16)
         fn = lambda: moe.route(logits, 8, 2, 1 << 19)  # noqa: E731
+    elif what == "route":
+        logits = torch.randn(65536, 512, device=dev, dtype=torch.bfloat16)
+        bias = torch.randn(512, device=dev) * 0.05
+        fn = lambda: ops.moe.route(logits, 512, 8, 2048, score="sigmoid", bias=bias, groups=8, top_groups=4,  # noqa: E731
+                                   group_score="top2")
+    elif what in ("rope", "qk_norm", "qk_norm_bwd"):
+        qkv = torch.randn(16384, 48, 128, device=dev, dtype=torch.bfloat16, requires_grad=what == "qk_norm_bwd")
+        wq, wk = (torch.ones(128, device=dev, dtype=torch.bfloat16, requires_grad=what == "qk_norm_bwd") for _ in range(2))
+        rotary = ops.Rotary()
+        if what == "rope":
+            fn = lambda: ops.rope(qkv, 16384, 40, rotary=rotary)  # noqa: E731
+        elif what == "qk_norm":
+            fn = lambda: ops.qk_norm_rope(qkv, 16384, 32, 8, wq, wk, rotary=rotary)  # noqa: E731
+        else:
+            y = ops.qk_norm_rope(qkv, 16384, 32, 8, wq, wk, rotary=rotary)
+            dy = torch.randn_like(y)
+            fn = lambda: torch.autograd.grad(y, (qkv, wq, wk), dy, retain_graph=True)  # noqa: E731
+    elif what == "clip":
+        grads = [torch.randn(n, device=dev) for n in (1 << 26, 1 << 24, 4096)]
+        fn = lambda: ops.clip_grad_norm_(grads, 1e-3)  # noqa: E731
     elif what == "adamw":
         m = 64 * 1024 * 1024
         p, a, b, g = (torch.zeros(m, device=dev) for _ in range(4))
