@@ -4,6 +4,7 @@ from __future__ import annotations
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native
 
@@ -12,6 +13,19 @@ def stream_ptr(t: torch.Tensor = None) -> int:
     """Raw handle of the current CUDA stream (kernels launch on torch's stream).  Asked for at every
     launch: 0.3 us this way, 5 us through a ``torch.cuda.Stream`` object."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+_modes, _transforms, _tracing = (torch._C._len_torch_dispatch_stack, torch._C._are_functorch_transforms_active,
+                                 torch._C._is_tracing)
+_tensor_types = (torch.Tensor, torch.nn.Parameter)
+
+
+def ordinary(t: torch.Tensor) -> bool:
+    """Whether a kernel may stand for elementary operations on ``t`` in a forward pass: a tensor itself, outside dispatch
+    modes, function transforms, forward-mode derivatives and tracing (what is asked here takes 0.4 us; a backward pass,
+    whose gradients may be batched, asks ``pad._plain``)."""
+    return type(t) in _tensor_types and not _modes() and not _transforms() and forward_ad._current_level < 0 \
+        and not _tracing()
 
 
 def call_on(t: torch.Tensor, name: str, *args) -> None:

@@ -11,7 +11,7 @@ import struct
 import torch
 
 from .. import _native
-from ._util import call_on, ptr, stream_ptr, use_native
+from ._util import call_on, ordinary, ptr, stream_ptr, use_native
 from .pad import _plain
 
 _v, _i, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
@@ -223,7 +223,7 @@ def route(logits: torch.Tensor, num_experts: int, k: int, capacity: int, *, scor
         return _route_plain_softmax(logits, E, k, capacity)
     how = _route_check(logits, E, k, score, bias, groups, top_groups, group_score, renormalize, scale)
     if use_native(logits) and logits.dtype in _DTYPE and E <= _MOST_EXPERTS and k <= _MOST_CHOICES \
-            and groups <= _MOST_GROUPS and logits.numel() and logits.shape[0] * k < 2 ** 31:
+            and groups <= _MOST_GROUPS and logits.numel() and logits.shape[0] * k < 2 ** 31 and ordinary(logits):
         logits = logits if logits.is_contiguous() else logits.contiguous()
         capacity = min(int(capacity), 2 ** 31 - 1)
         if torch.is_grad_enabled() and logits.requires_grad:

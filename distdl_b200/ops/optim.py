@@ -8,7 +8,7 @@ import functools
 import torch
 
 from .. import _native
-from ._util import call_on, ptr, stream_ptr, use_native
+from ._util import call_on, ordinary, ptr, stream_ptr, use_native
 
 _native.declare("dd_grad_norm_parts", [ctypes.c_int])
 _native.declare("dd_grad_norm", [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
@@ -99,7 +99,7 @@ def _tensors(tensors):
             if not t.is_floating_point():
                 raise ValueError(f"gradients are floating-point tensors, not {t.dtype}")
         return None
-    if not use_native(tensors[0]) or not all([t.is_contiguous() or _dense(t) for t in tensors]):
+    if not use_native(tensors[0]) or not ordinary(tensors[0]) or not all([t.is_contiguous() or _dense(t) for t in tensors]):
         return None
     return (array.array("Q", [t.data_ptr() for t in tensors]), array.array("q", [t.numel() for t in tensors]),
             array.array("B", codes))

@@ -12,7 +12,7 @@ from typing import Optional
 import torch
 
 from .. import _native
-from ._util import call_on, main_grad_now, ptr, use_native
+from ._util import call_on, main_grad_now, ordinary, ptr, use_native
 from .pad import _plain
 
 _native.declare("dd_heads", [ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p])
@@ -89,12 +89,13 @@ class Rotary:
         kernels, kept with the settings (the array that holds the frequencies as its last entry)."""
         plans = self.__dict__.get("_plans")
         if plans is None:
-            plans = self.__dict__["_plans"] = {}
+            plans = self.__dict__.setdefault("_plans", {})
         plan = plans.get(head_dim)
         if plan is None:
             dim = self.rotated(head_dim)
             arr = (ctypes.c_double * max(1, dim // 2))(*(f / (2 * math.pi) for f in _frequencies(self, dim)))
-            plan = plans[head_dim] = (dim, int(self.interleaved), ctypes.addressof(arr), self.scale, arr)
+            # (the first of several threads' stays: its address may be in use)
+            plan = plans.setdefault(head_dim, (dim, int(self.interleaved), ctypes.addressof(arr), self.scale, arr))
         return plan
 
     def __getstate__(self):                 # (copies and pickles hold the settings; addresses are this process's)
@@ -147,8 +148,9 @@ def _positions_of_ranges(ranges, device) -> torch.Tensor:
     key = (tuple((int(a), int(n)) for a, n in ranges), str(device))
     p = _range_positions.get(key)
     if p is None:
-        p = torch.cat([torch.arange(a, a + n, dtype=torch.int64) for a, n in key[0]]).to(device)
-        _range_positions[key] = p
+        p = torch.cat([torch.arange(a, a + n, dtype=torch.int64, device=device) for a, n in key[0]])
+        if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
+            _range_positions[key] = p       # (what a captured graph makes is the graph's own)
     return p
 
 
@@ -216,7 +218,7 @@ def _plain_rope(qkv, nheads, where, sign=1.0):
 
 
 def _native_ok(qkv):
-    return use_native(qkv) and qkv.dtype in _DTYPE and 1 <= qkv.shape[2] <= 512
+    return use_native(qkv) and qkv.dtype in _DTYPE and 1 <= qkv.shape[2] <= 512 and ordinary(qkv)
 
 
 def _unit(t):
@@ -362,6 +364,8 @@ def rope_in_place(qkv, seq, nheads, rotary, offset=0, ranges=None, positions=Non
         raise ValueError("a tensor that is turned in place must have its heads' components next to one another in memory "
                          "of their own: use ops.rope")
     if qkv.requires_grad and torch.is_grad_enabled():
+        if qkv.is_leaf:
+            raise RuntimeError("a leaf that requires a gradient cannot be turned in place: use ops.rope, or torch.no_grad()")
         return _RopeInPlaceFn.apply(qkv, (shape, nheads, where))
     _call(_ROTATE, read, read, nheads, 0, where)
     if not qkv.is_inference():
@@ -444,8 +448,8 @@ class _QKNormRopeFn(torch.autograd.Function):
             # gathered weights collect their gradient in fp32 beside them
             main = [main_grad_now(getattr(r, "main_grad", None), getattr(r, "main_grad_owner", None), ctx, k) if n else None
                     for k, r, n in ((1, ctx.refs[0], want[0]), (2, ctx.refs[1], want[1]))]
-            if any(m is None for m, n in zip(main, want) if n):
-                main = (None, None)
+            if any(m is None for m, n in zip(main, want) if n) or main[0] is main[1]:
+                main = (None, None)         # (one weight for both kinds: autograd adds)
         return (*_norm_backward(_unit(qkv), _unit(dy), wq, wk, hq, hkv, eps, where, want, main), None)
 
 

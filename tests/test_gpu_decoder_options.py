@@ -67,6 +67,22 @@ def test_training_step_with_an_optimizer_of_torchs(family):
         assert int(mlp.last_dropped) >= 0 and torch.isfinite(mlp.aux_loss)
 
 
+def test_recomputed_blocks_give_the_same_gradients():
+    """A block that recomputes its forward pass works on the same values: the same kernels, the same order of sums."""
+    tokens = torch.randint(0, 1000, (2, 257), device="cuda")
+    seen = []
+    for policy in ("none", "full"):
+        model = decoder("whole")
+        model.cfg.activation_policy = policy
+        model.loss(tokens[:, :-1], tokens[:, 1:]).backward()
+        model.release_gathered()
+        seen.append({n: p.grad.clone() for n, p in model.named_parameters() if p.grad is not None})
+    assert seen[0].keys() == seen[1].keys() and any("q_norm" in n for n in seen[0])
+    for n in seen[0]:
+        if "embed" not in n:                                  # (its rows are added by atomics)
+            assert torch.equal(seen[0][n], seen[1][n]), n
+
+
 def test_trainer_and_generation():
     from distdl_b200.parallel import SyntheticTokens, Trainer
     model = decoder("moe")

@@ -374,6 +374,65 @@ def test_on_another_stream_and_captured_in_graphs():
         assert all(torch.equal(a, b) for a, b in zip(want, out))
 
 
+def test_one_weight_for_queries_and_keys():
+    """Its gradient is the sum of both, also where it is collected beside the weight."""
+    x = torch.randn(200, 6, 128, device="cuda", dtype=BF16)
+    w = torch.ones(128, device="cuda", requires_grad=True)
+    dy = torch.randn_like(x)
+    both = [torch.ones(128, device="cuda", requires_grad=True) for _ in range(2)]
+    want = sum(torch.autograd.grad(ops.qk_norm_rope(x, 200, 3, 3, *both, rotary=ops.Rotary()), both, dy))
+    assert torch.equal(torch.autograd.grad(ops.qk_norm_rope(x, 200, 3, 3, w, w, rotary=ops.Rotary()), w, dy)[0], want)
+    w.main_grad = torch.zeros(128, device="cuda")
+    ops.qk_norm_rope(x, 200, 3, 3, w, w, rotary=ops.Rotary()).backward(dy)
+    assert torch.equal(w.grad + w.main_grad, want)
+
+
+def test_differentiated_twice_and_forwards():
+    """The gradient of a gradient, and forward-mode derivatives, by elementary operations."""
+    torch.manual_seed(7)
+    r = ops.Rotary(theta=100.0)
+    x = torch.randn(3, 3, 16, device="cuda", dtype=torch.float32, requires_grad=True)
+    w = (1 + 0.1 * torch.randn(16, device="cuda")).requires_grad_()
+    dy = torch.randn(3, 3, 16, device="cuda")
+
+    def twice(x, w):
+        y = ops.qk_norm_rope(x, 3, 2, 1, w, w, rotary=r)
+        g, = torch.autograd.grad(y, x, dy.to(y.dtype), create_graph=True)
+        return torch.autograd.grad(g.square().sum(), (x, w))
+
+    wide = twice(x.detach().double().requires_grad_(), w.detach().double().requires_grad_())
+    for a, b in zip(twice(x, w), wide):
+        assert torch.allclose(a.double(), b, rtol=1e-4, atol=1e-4 * b.abs().max().item())
+    import torch.autograd.forward_ad as fwd
+    t = torch.randn_like(x)
+    with torch.no_grad(), fwd.dual_level():
+        out = fwd.unpack_dual(ops.rope(fwd.make_dual(x.detach(), t), 3, 3, rotary=r))
+        assert torch.allclose(out.tangent, ops.rope(t, 3, 3, rotary=r), atol=1e-5)
+    many = torch.func.vmap(lambda z: ops.rope(z, 3, 3, rotary=r))(torch.stack([x.detach(), t]))
+    assert torch.allclose(many[1], ops.rope(t, 3, 3, rotary=r), atol=1e-5)
+
+
+def test_a_leaf_is_not_turned_in_place():
+    x = torch.randn(4, 3, 64, device="cuda", requires_grad=True)
+    keep = x.detach().clone()
+    with pytest.raises(RuntimeError):
+        ops.rope_(x, 4, 3, rotary=ops.Rotary())
+    assert torch.equal(x, keep)
+
+
+def test_ranges_first_met_in_a_graph():
+    x = torch.randn(7, 2, 64, device="cuda")
+    ranges = ((11, 3), (501, 4))
+    r = ops.Rotary()
+    ops.rope(x, 7, 2, rotary=r)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.rope(x, 7, 2, rotary=r, ranges=ranges)
+    eager = ops.rope(x, 7, 2, rotary=r, ranges=ranges)
+    graph.replay()
+    assert torch.equal(y, eager)
+
+
 def test_offsets_beyond_32_bits():
     """Tokens whose elements lie more than 2^31 apart."""
     big = torch.empty((1 << 31) + (1 << 12), device="cuda", dtype=BF16)
