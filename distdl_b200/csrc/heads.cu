@@ -9,9 +9,9 @@
 // Bandwidth bounds them: a head is read and written once, with 16 bytes per access.  So nothing else travels:
 //  * a group of lanes (8 for 128 bf16 components) holds a head in registers, two vectors per lane, and a lane that holds one
 //    component of a pair also holds the other (the vectors lie half the rotated part apart, or the pairs lie inside a vector);
-//  * the angles are computed, not read: position times frequency in turns in 64 bits, reduced to half a turn (exact for
-//    every position below 2^31, where 32 bits are off by radians), then sin and cos in 32 bits, once per lane for all heads of
-//    a chunk.  The frequencies travel as arguments of the kernel: no table, no copy, nothing to capture or to keep;
+//  * the angles are computed, not read: position times frequency in turns in 64 bits, reduced to half a turn (within 10^-6
+//    radians for every position below 2^31, where 32 bits are off by whole turns), then sin and cos in 32 bits, once per lane for
+//    all heads of a chunk.  The frequencies travel as arguments of the kernel: no table, no copy, nothing to capture or to keep;
 //  * the backward pass recomputes r from x, which it needs anyway.
 // A unit of work is a token's chunk of heads of one kind (query / key / rest).  Units are dealt to the warps of a grid of two
 // CTAs per SM, kind by kind, so that what belongs to a kind is held once; the heads of a unit to the groups of the warp in turn,
@@ -446,9 +446,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_fwd_kernel(const _
   copy_rest<T, VE, NV>(a, lane, a.x, a.x_row, a.x_head, unit - units, stride, in_warp, per_warp);
 }
 
-// 16 bytes global -> shared by a copy of this thread's own; nothing is read and zeros are written where it is not to read.
-__device__ __forceinline__ void copy_async(void* to, const void* from, bool read) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(read ? 16 : 0) : "memory");
+// 16 bytes global -> shared by a copy of this thread's own.
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
@@ -506,8 +506,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
           const bool read = ahead_h < ahead_count && lane.has(s);
           if constexpr (RING) {
             uint8_t* to = ring + ((slot * 2 * NV + s) * kThreads + threadIdx.x) * 16;
-            copy_async(to, x + lane.at[s], read);
-            copy_async(to + NV * kThreads * 16, dy + lane.at[s], read);
+            if (read) {
+              copy_async(to, x + lane.at[s]);
+              copy_async(to + NV * kThreads * 16, dy + lane.at[s]);
+            } else {
+              *reinterpret_cast<uint4*>(to) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(to + NV * kThreads * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
           } else {
             clear(rx[s]);
             clear(rd[s]);
