@@ -20,9 +20,10 @@
 // exponential shows in the experts.
 //
 // A warp works on a token, its lanes on C consecutive experts each, which they sort; the k best are then the largest of the
-// lanes' first ones, k times, one warp-wide integer maximum each.  Some 500 instructions per token of 256 experts bound it
-// above some thousand tokens (with the experts unsorted and the winner's place looked for by ballot and shuffle 1 130 to
-// 1 920, 16384 tokens 34 to 66 us), a latency below.  Slots follow in a second kernel (route_slot_kernel): a pair's
+// lanes' first ones, k times, one warp-wide integer maximum each.  Above some thousand tokens instructions that follow from one
+// another bound it, 650 (softmax, no bias) to 1 050 (sigmoid, bias, 8 groups) per token of 256 experts: 16384 tokens 19 to 32 us
+// (with the experts unsorted and the winner's place looked for by ballot and shuffle 1 130 to 1 920, 34 to 66 us); below, a
+// latency.  Slots follow in a second kernel (route_slot_kernel): a pair's
 // slot is its rank in pair order among the pairs of its expert, so nothing depends on how CTAs are scheduled; sums of p are
 // formed per chunk of tokens and then over the chunks, always in the same order.
 #include "common.cuh"
@@ -379,7 +380,7 @@ struct Scores {
 template <typename T, int C>
 __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(const __grid_constant__ RouteArgs a) {
   __shared__ int s_hist[kMaxExperts];
-  __shared__ __align__(16) double s_row[kWarps][32 * C];   // a warp's values by expert; at the end its sums of p
+  __shared__ __align__(16) double s_row[kWarps][32 * C];      // a warp's values by expert; at the end its sums of p
   grid_dependency_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < a.E; e += kWarps * 32) s_hist[e] = 0;

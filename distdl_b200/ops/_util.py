@@ -17,15 +17,20 @@ def stream_ptr(t: torch.Tensor = None) -> int:
 
 _modes, _transforms, _tracing = (torch._C._len_torch_dispatch_stack, torch._C._are_functorch_transforms_active,
                                  torch._C._is_tracing)
+_batched = torch._C._functorch.is_legacy_batchedtensor
 _tensor_types = (torch.Tensor, torch.nn.Parameter)
 
 
 def ordinary(t: torch.Tensor) -> bool:
     """Whether a kernel may stand for elementary operations on ``t`` in a forward pass: a tensor itself, outside dispatch
-    modes, function transforms, forward-mode derivatives and tracing (what is asked here takes 0.4 us; a backward pass,
-    whose gradients may be batched, asks ``pad._plain``)."""
+    modes, function transforms, forward-mode derivatives and tracing."""
     return type(t) in _tensor_types and not _modes() and not _transforms() and forward_ad._current_level < 0 \
         and not _tracing()
+
+
+def ordinary_gradient(t: torch.Tensor) -> bool:
+    """The same in a backward pass, whose gradients may be batched."""
+    return ordinary(t) and not _batched(t)
 
 
 def call_on(t: torch.Tensor, name: str, *args) -> None:

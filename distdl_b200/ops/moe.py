@@ -11,8 +11,7 @@ import struct
 import torch
 
 from .. import _native
-from ._util import call_on, ordinary, ptr, stream_ptr, use_native
-from .pad import _plain
+from ._util import call_on, ordinary, ordinary_gradient, ptr, stream_ptr, use_native
 
 _v, _i, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
 _native.declare("dd_moe_assign", [_v, _i, _i, _i, _v, _v, _v])
@@ -112,7 +111,7 @@ class _RouteFn(torch.autograd.Function):
     def backward(ctx, dw, dprob, _dids, _dslot, _dcounts):
         logits, ids, w = ctx.saved_tensors
         E, k, how = ctx.cfg
-        if torch.is_grad_enabled() or not all(g is None or _plain(g) for g in (dw, dprob)):
+        if torch.is_grad_enabled() or not all([g is None or ordinary_gradient(g) for g in (dw, dprob)]):
             # differentiated itself, or under a function transform: elementary operations, with the experts as they are
             with torch.enable_grad():
                 outs = _route_weights(logits, E, ids.reshape(-1, k), how)
@@ -121,9 +120,11 @@ class _RouteFn(torch.autograd.Function):
             return d, None, None, None, None
         if dw is None and dprob is None:
             return None, None, None, None, None
-        dw, dprob = (g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) else g.float().contiguous()
-                     for g in (dw, dprob))
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        if dw is not None and (dw.dtype != torch.float32 or not dw.is_contiguous()):
+            dw = dw.float().contiguous()
+        if dprob is not None and (dprob.dtype != torch.float32 or not dprob.is_contiguous()):
+            dprob = dprob.float().contiguous()
+        dlogits = torch.empty_like(logits)
         call_on(logits, "dd_route_bwd", logits.data_ptr(), logits.shape[1], _DTYPE[logits.dtype], logits.shape[0], E, k,
                 int(how[0] == "sigmoid"), int(how[5]), how[6], ids.data_ptr(), w.data_ptr(), ptr(dw), ptr(dprob),
                 dlogits.data_ptr())

@@ -12,8 +12,7 @@ from typing import Optional
 import torch
 
 from .. import _native
-from ._util import call_on, main_grad_now, ordinary, ptr, use_native
-from .pad import _plain
+from ._util import call_on, main_grad_now, ordinary, ordinary_gradient, ptr, use_native
 
 _native.declare("dd_heads", [ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p])
 _native.declare("dd_heads_parts", [])
@@ -269,7 +268,7 @@ class _RopeFn(torch.autograd.Function):
 def _turned_back(ctx, d, nheads, where, sign):
     if where[1] is not None:
         where = (where[0], ctx.saved_tensors[0], *where[2:])     # (which says whether they have been changed since)
-    if not _plain(d):                       # under a function transform: elementary operations
+    if not ordinary_gradient(d):            # under a function transform: elementary operations
         return _plain_rope(d, nheads, where, sign)
     if torch.is_grad_enabled():             # differentiated itself
         return _RopeFn.apply(d, (nheads, where, sign))
@@ -435,7 +434,7 @@ class _QKNormRopeFn(torch.autograd.Function):
         hq, hkv, eps, where = ctx.cfg
         where = (where[0], positions, *where[2:])
         need = ctx.needs_input_grad
-        if torch.is_grad_enabled() or not _plain(dy):
+        if torch.is_grad_enabled() or not ordinary_gradient(dy):
             # differentiated itself, or under a function transform: elementary operations
             leaves = [t for t, n in zip((qkv, wq, wk), need) if n]
             with torch.enable_grad():
@@ -444,7 +443,7 @@ class _QKNormRopeFn(torch.autograd.Function):
             return (*(next(got) if n else None for n in need[:3]), None)
         want = need[1:3]
         main = (None, None)
-        if want[0] or want[1]:
+        if hasattr(ctx.refs[0], "main_grad") or hasattr(ctx.refs[1], "main_grad"):
             # gathered weights collect their gradient in fp32 beside them
             main = [main_grad_now(getattr(r, "main_grad", None), getattr(r, "main_grad_owner", None), ctx, k) if n else None
                     for k, r, n in ((1, ctx.refs[0], want[0]), (2, ctx.refs[1], want[1]))]
