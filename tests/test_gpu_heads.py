@@ -412,6 +412,48 @@ def test_differentiated_twice_and_forwards():
     assert torch.allclose(many[1], ops.rope(t, 3, 3, rotary=r), atol=1e-5)
 
 
+def test_in_inference_mode_and_without_heads_to_turn():
+    r = ops.Rotary(theta=10000.0)
+    with torch.inference_mode():
+        x = torch.randn(6, 5, 64, device="cuda", dtype=BF16)
+        y = ops.qk_norm_rope(x, 6, 3, 1, rotary=r)
+        z = ops.rope(x, 6, 4, rotary=r)
+        assert torch.equal(ops.rope_(x.clone(), 6, 4, rotary=r), z)
+        assert torch.equal(ops.qk_norm_rope_(x, 6, 3, 1, rotary=r), y)
+    x = torch.randn(6, 5, 64, device="cuda", dtype=BF16, requires_grad=True)
+    w = [torch.ones(64, device="cuda", dtype=BF16, requires_grad=True) for _ in range(2)]
+    y = ops.qk_norm_rope(x, 6, 0, 0, *w, rotary=r)
+    dy = torch.randn_like(y)
+    grads = torch.autograd.grad(y, (x, *w), dy)
+    assert torch.equal(y, x) and torch.equal(grads[0], dy) and not grads[1].any() and not grads[2].any()
+    empty = ops.qk_norm_rope(x[:0], 6, 3, 1, *w, rotary=r)
+    grads = torch.autograd.grad(empty, (x, *w), empty.detach(), allow_unused=True)
+    assert empty.shape == (0, 5, 64) and not grads[0].any() and not grads[1].any() and not grads[2].any()
+    assert torch.equal(ops.rope_(x.detach(), 6, 5, rotary=ops.Rotary(dim=0)), x)
+
+
+def test_only_what_is_asked_for_gets_a_gradient():
+    r = ops.Rotary()
+    x = torch.randn(30, 6, 128, device="cuda", dtype=BF16, requires_grad=True)
+    wq, wk = (torch.ones(128, device="cuda", dtype=BF16) for _ in range(2))
+    dy = torch.randn_like(x)
+    dx, = torch.autograd.grad(ops.qk_norm_rope(x, 30, 3, 2, wq, wk, rotary=r), x, dy)
+    wk.requires_grad_()
+    only, = torch.autograd.grad(ops.qk_norm_rope(x.detach(), 30, 3, 2, wq, wk, rotary=r), wk, dy)
+    every = torch.autograd.grad(ops.qk_norm_rope(x, 30, 3, 2, wq.requires_grad_(), wk, rotary=r), (x, wq, wk), dy)
+    assert torch.equal(every[0], dx) and torch.equal(every[2], only)
+
+
+def test_positions_changed_before_the_backward_pass_are_noticed():
+    x = torch.randn(4, 2, 64, device="cuda", requires_grad=True)
+    pos = torch.arange(4, device="cuda")
+    for y in (ops.rope(x, 4, 2, rotary=ops.Rotary(), positions=pos),
+              ops.qk_norm_rope(x, 4, 1, 1, rotary=ops.Rotary(), positions=pos)):
+        pos += 1
+        with pytest.raises(RuntimeError):
+            y.sum().backward()
+
+
 def test_a_leaf_is_not_turned_in_place():
     x = torch.randn(4, 3, 64, device="cuda", requires_grad=True)
     keep = x.detach().clone()

@@ -239,6 +239,29 @@ def test_padding_columns_views_and_addresses():
     check(odd, 61, 4, 20, score="sigmoid")
 
 
+def test_no_room_and_all_experts():
+    torch.manual_seed(15)
+    logits = torch.randn(20, 12, device="cuda")
+    w, prob, ids, slot, counts = moe.route(logits, 12, 12, 0, score="sigmoid")
+    assert (slot == -1).all() and (counts == 20).all() and (ids.reshape(20, 12).sort(1).values == torch.arange(
+        12, device="cuda")).all()
+    check(logits, 12, 12, 1 << 40, score="sigmoid")
+    with torch.inference_mode():
+        moe.route(torch.randn(20, 12, device="cuda"), 12, 3, 4, score="sigmoid")
+
+
+def test_results_changed_in_place_do_not_disturb_the_gradient():
+    logits = torch.randn(20, 12, device="cuda", requires_grad=True)
+    w, prob, ids, slot, counts = moe.route(logits, 12, 3, 4, score="sigmoid")
+    want, = torch.autograd.grad(w.square().sum(), logits, retain_graph=True)
+    counts += 1
+    slot.fill_(-1)
+    assert torch.equal(torch.autograd.grad(w.square().sum(), logits, retain_graph=True)[0], want)
+    ids += 1                                                  # (these the gradient needs)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(w.square().sum(), logits)
+
+
 def test_no_tokens():
     w, prob, ids, slot, counts = moe.route(torch.zeros(0, 128, device="cuda"), 128, 4, 8, score="sigmoid")
     assert w.shape == (0, 4) and ids.numel() == 0 and (prob == 0).all() and (counts == 0).all()
