@@ -224,26 +224,29 @@ __device__ __forceinline__ int choose(const RouteArgs& a, unsigned (&key)[C], in
   } else {
     sort_falling<C>(key);
   }
-  // the k best one by one
-  int chosen = -1;
-  unsigned was = 0u;
-  const int rounds = a.k + (near >= 0 ? 1 : 0);               // (one more: the first that is left out must not be close)
-  for (int i = 0; i < rounds; ++i) {
+  // the k best one by one: lane i keeps the i-th key
+  unsigned mine = 0u;
+  for (int i = 0; i < a.k; ++i) {
     const unsigned top = __reduce_max_sync(0xffffffffu, key[0]);
-    if (top == 0u) break;
-    const int e = 511 - (int)(top & 511u);
-    if (i > 0 && (int)(was >> 9) - (int)(top >> 9) <= near) {
-      const int f = 511 - (int)(was & 511u);                  // two alike in logit and bias are alike, and in order
-      close |= to_f(from[f]) != to_f(from[e]) || (a.bias != nullptr && a.bias[f] != a.bias[e]);
-    }
-    was = top;
-    if (lane == i && i < a.k) chosen = e;
+    if (lane == i) mine = top;
     if (key[0] == top) {
 #pragma unroll
       for (int j = 0; j + 1 < C; ++j) key[j] = key[j + 1];
       key[C - 1] = 0u;
     }
   }
+  if (near >= 0) {                                            // none may be close to the next, the first left out included
+    unsigned next = __shfl_down_sync(0xffffffffu, mine, 1);
+    const unsigned out = __reduce_max_sync(0xffffffffu, key[0]);
+    if (lane == a.k - 1) next = out;
+    if (lane < a.k && next != 0u && (int)(mine >> 9) - (int)(next >> 9) <= near) {
+      const int e = 511 - (int)(mine & 511u), f = 511 - (int)(next & 511u);
+      // (two alike in logit and bias are alike, and in order)
+      close |= to_f(from[f]) != to_f(from[e]) || (a.bias != nullptr && a.bias[f] != a.bias[e]);
+    }
+    close = __any_sync(0xffffffffu, close);
+  }
+  const int chosen = lane < a.k && mine != 0u ? 511 - (int)(mine & 511u) : -1;
   return chosen;
 }
 
@@ -380,17 +383,16 @@ struct Scores {
 template <typename T, int C>
 __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(const __grid_constant__ RouteArgs a) {
   __shared__ int s_hist[kMaxExperts];
+  __shared__ __align__(16) float s_bias[32 * C];
   __shared__ __align__(16) double s_row[kWarps][32 * C];      // a warp's values by expert; at the end its sums of p
   grid_dependency_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < a.E; e += kWarps * 32) s_hist[e] = 0;
+  for (int e = threadIdx.x; e < 32 * C; e += kWarps * 32) s_bias[e] = a.bias != nullptr && e < a.E ? a.bias[e] : 0.f;
   __syncthreads();
   const int first = lane * C;
   const int left = min(max(a.E - first, 0), C);               // experts of this lane
   const bool exact = a.by_logit && sizeof(T) == 2;            // the logits fit into a key's value
-  float bias[C];
-#pragma unroll
-  for (int j = 0; j < C; ++j) bias[j] = a.bias != nullptr && j < left ? a.bias[first + j] : 0.f;
   float sums[C];
 #pragma unroll
   for (int j = 0; j < C; ++j) sums[j] = 0.f;
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
       const float back = a.by_logit ? 0.f : a.sigmoid ? __expf(fminf(top_l, 0.f)) : s.inv;
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        v[j] = a.by_logit ? l[j] : s.part[j] * back + bias[j];
+        v[j] = a.by_logit ? l[j] : s.part[j] * back + s_bias[first + j];
         if (!(l[j] > -INFINITY && v[j] > -INFINITY)) v[j] = -INFINITY;     // (a bias of -inf takes an expert out, too)
         else { hi = fmaxf(hi, v[j]); lo = fminf(lo, v[j]); }
       }
@@ -430,7 +432,8 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
       near = (int)fminf(off * steps + 3.f, 8388607.f);
 #pragma unroll
       for (int j = 0; j < C; ++j)
-        key[j] = v[j] > -INFINITY ? (unsigned)((int)(fmaxf(v[j] - lo, 0.f) * steps) + 1) << 9 | (511 - first - j) : 0u;
+        // (2^23 + a whole number: the number is the mantissa, and the shift drops the rest)
+        key[j] = v[j] > -INFINITY ? (__float_as_uint(fmaf(fmaxf(v[j] - lo, 0.f), steps, 8388609.f)) << 9) + (511 - first - j) : 0u;
     }
     if (nan) {
 #pragma unroll

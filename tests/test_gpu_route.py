@@ -154,6 +154,19 @@ def test_nearly_equal_scores_are_told_apart(score):
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("k", [1, 2, 8, 31, 32])
+def test_the_first_left_out_is_told_apart(score, k):
+    # k - 1 experts far above the others; of two that are an ulp of fp32 apart the later is the better one
+    g = torch.Generator().manual_seed(k)
+    logits = torch.randn(32, 80, generator=g)
+    place = torch.stack([torch.randperm(80, generator=g) for _ in range(32)])
+    two = place[:, k - 1:k + 1].sort(1).values
+    logits.scatter_(1, place[:, :k - 1], 6.0 + torch.rand(32, k - 1, generator=g))
+    logits.scatter_(1, two, torch.tensor([4.0, 4.0 + 2.0 ** -21]).expand(32, 2))
+    check(logits.cuda(), 80, k, 32, grads=False, score=score, bias=torch.zeros(80).cuda())
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("grouped", [False, True])
 @pytest.mark.parametrize("bias", [False, True])
 def test_masked_experts_and_padding_tokens(score, grouped, bias):
