@@ -365,10 +365,7 @@ struct Scores {
       for (int j = 0; j < C; ++j) part[j] = __expf(l[j] - shift);
     } else if (top >= 0.f) {
 #pragma unroll
-      for (int j = 0; j < C; ++j) {
-        const float e = __expf(-fabsf(l[j]));
-        part[j] = __fdividef(l[j] > 0.f ? 1.f : e, 1.f + e);
-      }
+      for (int j = 0; j < C; ++j) part[j] = __fdividef(1.f, 1.f + __expf(-l[j]));   // (e^88: 0, as e^-88)
     } else {
       const float shift = none ? 0.f : top;
 #pragma unroll
@@ -419,11 +416,12 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
 #pragma unroll
       for (int j = 0; j < C; ++j) {
         v[j] = a.by_logit ? l[j] : s.part[j] * back + s_bias[first + j];
-        if (!(l[j] > -INFINITY && v[j] > -INFINITY)) v[j] = -INFINITY;     // (a bias of -inf takes an expert out, too)
-        else { hi = fmaxf(hi, v[j]); lo = fminf(lo, v[j]); }
+        if (!(l[j] > -INFINITY)) v[j] = -INFINITY;            // (a bias of -inf takes an expert out, too)
+        hi = fmaxf(hi, v[j]);
+        lo = fminf(lo, v[j]);
       }
       hi = top_of_warp(hi);
-      // (values far below the largest are not told apart: should they decide, they are close)
+      // (values far below the largest, -inf among them, are not told apart: should they decide, they are close)
       lo = fmaxf(low_of_warp(lo), hi - (a.by_logit ? 64.f : 8.f));
       const float range = hi - lo, steps = range > 1e-25f ? __fdividef(kSteps, range) : 0.f;
       // scores: sigmoid 4e-7 off at most (its slope times the exponential's error, a division), softmax 4e-6 of the largest,
