@@ -74,6 +74,12 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __
 // C values of one lane in memory, moved in pieces of up to 16 bytes.
 template <typename T, int C> struct alignas(C * sizeof(T) < 16 ? C * sizeof(T) : 16) Row { T v[C]; };
 
+// Where a value of each expert stands in shared memory, so that the lanes' loads of up to 16 bytes lie side by side.
+template <int C> __device__ __forceinline__ int place_of(int lane, int j) {
+  constexpr int V = C < 4 ? C : 4;
+  return lane * V + j / V * 32 * V + j % V;
+}
+
 template <typename T, int C>
 __device__ __forceinline__ void load_row(const T* p, bool vectors, int left, float (&l)[C]) {
   if (vectors && left >= C) {
@@ -385,7 +391,7 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
   grid_dependency_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < a.E; e += kWarps * 32) s_hist[e] = 0;
-  for (int e = threadIdx.x; e < 32 * C; e += kWarps * 32) s_bias[e] = a.bias != nullptr && e < a.E ? a.bias[e] : 0.f;
+  for (int e = threadIdx.x; e < 32 * C; e += kWarps * 32) s_bias[place_of<C>(e / C, e % C)] = a.bias != nullptr && e < a.E ? a.bias[e] : 0.f;
   __syncthreads();
   const int first = lane * C;
   const int left = min(max(a.E - first, 0), C);               // experts of this lane
@@ -415,7 +421,7 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
       const float back = a.by_logit ? 0.f : a.sigmoid ? __expf(fminf(top_l, 0.f)) : s.inv;
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        v[j] = a.by_logit ? l[j] : s.part[j] * back + s_bias[first + j];
+        v[j] = a.by_logit ? l[j] : s.part[j] * back + s_bias[place_of<C>(lane, j)];
         if (!(l[j] > -INFINITY)) v[j] = -INFINITY;            // (a bias of -inf takes an expert out, too)
         hi = fmaxf(hi, v[j]);
         lo = fminf(lo, v[j]);
@@ -609,11 +615,11 @@ route_bwd_kernel(const __grid_constant__ RouteArgs a, const float* __restrict__ 
     const float w = next_w, g = id >= 0 ? next_g : 0.f;
     if (kAhead && a.tokens - t > stride) fetch(t + stride);
 #pragma unroll
-    for (int j = 0; j < C; ++j) s_row[warp][first + j] = 0.f;
+    for (int j = 0; j < C; ++j) s_row[warp][place_of<C>(lane, j)] = 0.f;
     const float wd = warp_sum(id >= 0 ? w * g : 0.f);         // scale * D
     const float grad = a.renormalize ? w * (g - __fdividef(wd, a.scale)) : w * g;
     __syncwarp();
-    if (id >= 0 && id < a.E) s_row[warp][id] = grad;
+    if (id >= 0 && id < a.E) s_row[warp][place_of<C>(id / C, id % C)] = grad;
     unsigned bad = 0u;
     bool nan;
     const float top_l = top_logit<C>(l, a.sigmoid, bad, nan);
@@ -629,7 +635,7 @@ route_bwd_kernel(const __grid_constant__ RouteArgs a, const float* __restrict__ 
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       const float f = a.sigmoid ? __fdividef(1.f, 1.f + __expf(l[j])) : 1.f;
-      const float v = f * (s_row[warp][first + j] + p[j] * (coef[j] - pq - all));
+      const float v = f * (s_row[warp][place_of<C>(lane, j)] + p[j] * (coef[j] - pq - all));
       out.v[j] = from_f<T>(j >= left ? 0.f : nan ? __int_as_float(0x7fffffff) : v);
     }
     T* to = dlogits + (size_t)t * a.ld;
