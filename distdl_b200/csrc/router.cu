@@ -189,11 +189,56 @@ __device__ __forceinline__ void clear_others(const RouteArgs& a, V (&v)[C], V no
   }
 }
 
-// The choice of one token from the keys of its experts: lane i gets the i-th expert, -1 where there is none.  `close` is set
-// where values within `near` of one another (near < 0: all values are exact) decide and are not those of experts alike in logit
-// and bias.
+// What an expert is chosen by, in 64 bits (softmax scores: choose_in_64_bits).  T: of the logits.
+template <typename T>
+__device__ __forceinline__ double value_in_64_bits(const RouteArgs& a, const T* from, int e) {
+  const double l = to_f(from[e]);
+  return (a.by_logit ? l : 1.0 / (1.0 + exp(-l))) + (a.bias != nullptr ? (double)a.bias[e] : 0.0);
+}
+// Whether this lane's group is among the best, in 64 bits: of a lane's sorted keys those that can be one of its group's two best
+// (its best), their value >= least.  (What decides few tokens is kept short: others wait at the end for the one that is fetching
+// instructions.  With all experts in 64 bits 16384 tokens took 34 us, with those that matter 29.)
 template <typename T, int C>
-__device__ __forceinline__ int choose(const RouteArgs& a, unsigned (&key)[C], int first, int left, int near, bool& close,
+__device__ __noinline__ bool groups_in_64_bits(const RouteArgs& a, const unsigned* key, int least, const T* from) {
+  double b0 = -INFINITY, b1 = -INFINITY;
+#pragma unroll 1
+  for (int j = 0; j < C; ++j) {
+    const bool in = key[j] != 0u && (int)(key[j] >> 9) >= least;
+    if (!__any_sync(0xffffffffu, in)) break;
+    const double v = in ? value_in_64_bits<T>(a, from, 511 - (int)(key[j] & 511u)) : -INFINITY;
+    b1 = fmax(b1, fmin(b0, v));
+    b0 = fmax(b0, v);
+  }
+  int step;
+  const int g = best_of_groups<double>(a, nullptr, -INFINITY, b0, b1, step);
+  return among_best(a, a.group_sum && b1 > -INFINITY ? b0 + b1 : b0, g, step);
+}
+// The first k of n candidates, the i-th key in lane i (0: none), in the order of 64 bits.
+template <typename T>
+__device__ __noinline__ int order_in_64_bits(const RouteArgs& a, unsigned mine, int n, const T* from) {
+  const int lane = threadIdx.x & 31, e = mine != 0u ? 511 - (int)(mine & 511u) : kMaxExperts;
+  const double c = mine != 0u ? value_in_64_bits<T>(a, from, e) : -INFINITY;
+  int place = 0;
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) {
+    const double other = __shfl_sync(0xffffffffu, c, i);
+    const int f = __shfl_sync(0xffffffffu, e, i);
+    place += other > c || (other == c && f < e);
+  }
+  int chosen = -1;
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) {
+    const int f = __shfl_sync(0xffffffffu, e, i);
+    if (__shfl_sync(0xffffffffu, place, i) == lane && f < kMaxExperts) chosen = f;
+  }
+  return lane < a.k ? chosen : -1;
+}
+
+// The choice of one token from the keys of its experts: lane i gets the i-th expert, -1 where there is none.  `close` is set
+// where values within `near` of one another (near < 0: all values are exact) decide, are not those of experts alike in logit
+// and bias, and are not decided here (`here`: where they can be).
+template <typename T, int C>
+__device__ __forceinline__ int choose(const RouteArgs& a, unsigned (&key)[C], int first, int left, int near, bool here, bool& close,
                                       int* values, const T* from) {
   const int lane = threadIdx.x & 31;
   if (a.groups > 1) {
@@ -221,6 +266,13 @@ __device__ __forceinline__ int choose(const RouteArgs& a, unsigned (&key)[C], in
       // (of a group with one expert only its value itself would have to be known)
       close = (most > 0 && least - most <= (a.group_sum ? 2 * near : near)) ||
               __any_sync(0xffffffffu, g < a.groups && a.group_sum && a.size > 1 && b0 > 0 && b1 == 0);
+      if (close && here && a.lanes > 0) {
+        unsigned sorted[C];
+#pragma unroll
+        for (int j = 0; j < C; ++j) sorted[j] = key[j];
+        in = groups_in_64_bits<T, C>(a, sorted, (a.group_sum ? b1 : b0) - near, from);
+        close = false;
+      }
     }
     clear_others<unsigned, C>(a, key, 0u, in, first, left, step);
     if (a.lanes == 0) {
@@ -243,14 +295,33 @@ __device__ __forceinline__ int choose(const RouteArgs& a, unsigned (&key)[C], in
   }
   if (near >= 0) {                                            // none may be close to the next, the first left out included
     unsigned next = __shfl_down_sync(0xffffffffu, mine, 1);
-    const unsigned out = __reduce_max_sync(0xffffffffu, key[0]);
+    unsigned out = __reduce_max_sync(0xffffffffu, key[0]);
     if (lane == a.k - 1) next = out;
+    bool alike = true;
     if (lane < a.k && next != 0u && (int)(mine >> 9) - (int)(next >> 9) <= near) {
       const int e = 511 - (int)(mine & 511u), f = 511 - (int)(next & 511u);
       // (two alike in logit and bias are alike, and in order)
-      close |= to_f(from[f]) != to_f(from[e]) || (a.bias != nullptr && a.bias[f] != a.bias[e]);
+      alike = to_f(from[f]) == to_f(from[e]) && (a.bias == nullptr || a.bias[f] == a.bias[e]);
     }
-    close = __any_sync(0xffffffffu, close);
+    if (__any_sync(0xffffffffu, !alike)) {
+      if (!here || close) { close = true; return -1; }
+      // all that may be among the k best: up to the first that is not close to the one before it
+      int n = a.k;
+      unsigned last = __shfl_sync(0xffffffffu, mine, a.k - 1);
+      while (out != 0u && (int)(last >> 9) - (int)(out >> 9) <= near) {
+        if (n == 32) { close = true; return -1; }
+        if (lane == n) mine = out;
+        ++n;
+        last = out;
+        if (key[0] == out) {
+#pragma unroll
+          for (int j = 0; j + 1 < C; ++j) key[j] = key[j + 1];
+          key[C - 1] = 0u;
+        }
+        out = __reduce_max_sync(0xffffffffu, key[0]);
+      }
+      return order_in_64_bits<T>(a, mine, n, from);
+    }
   }
   const int chosen = lane < a.k && mine != 0u ? 511 - (int)(mine & 511u) : -1;
   return chosen;
@@ -445,7 +516,8 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
         if ((bad >> j) & 1u) key[j] = kBad | (511 - first - j);
     }
     bool close = false;
-    int chosen = choose<T, C>(a, key, first, left, near, close, reinterpret_cast<int*>(s_row[warp]), from);
+    int chosen = choose<T, C>(a, key, first, left, near, !nan && (a.by_logit || a.sigmoid), close,
+                              reinterpret_cast<int*>(s_row[warp]), from);
     if (close) {                                              // (the same on every lane)
       float again[C];
 #pragma unroll
