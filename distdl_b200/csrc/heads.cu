@@ -8,7 +8,8 @@
 //
 // Bandwidth bounds them: a head is read and written once, with 16 bytes per access.  So nothing else travels:
 //  * a group of lanes (8 for 128 bf16 components) holds a head in registers, two vectors per lane, and a lane that holds one
-//    component of a pair also holds the other (the vectors lie half the rotated part apart, or the pairs lie inside a vector);
+//    component of a pair also holds the other (the vectors lie half the rotated part apart, or the pairs lie inside a vector; where
+//    that half is not whole vectors, the others come from their lanes through shared memory);
 //  * the angles are computed, not read: position times frequency in turns in 64 bits, reduced to half a turn (within 10^-6
 //    radians for every position below 2^31, where 32 bits are off by whole turns), then sin and cos in 32 bits, once per lane for
 //    all heads of a chunk.  The frequencies travel as arguments of the kernel: no table, no copy, nothing to capture or to keep;
@@ -38,6 +39,7 @@ enum Kind { kRope = 0, kNorm = 1 };
 enum Pairing {
   kApart = 0,     // halves that are whole vectors: at the same place of its two vectors
   kInside = 1,    // next to one another in a vector; with single components, any pair of components that it holds
+  kCrossed = 2,   // halves that are not whole vectors: one in its vectors, the other in another lane's, by way of shared memory
 };
 
 struct HeadArgs {
@@ -217,12 +219,56 @@ struct Lane {
   }
 };
 
+// kCrossed: a warp's heads in shared memory, as they came, and where a lane finds the partners of its components there: byte
+// offsets, two to a word; for components that stay that of a zero.  Heads are a word more than their length apart, for the banks.
+constexpr int kCrossing = 32 * 2 * 4 + 32;                    // words of a warp; then the zero
+template <typename T, int VE, int NV, int PAIRING, int GROUP>
+struct Partners {
+  using L = Lane<T, VE, NV, PAIRING, GROUP>;
+  static constexpr int M = PAIRING == kCrossed ? L::M : 1;
+  uint32_t from[M];
+  uint32_t *warp, *own;                                       // the warp's heads, and this lane's
+
+  __device__ __forceinline__ Partners(const HeadArgs& a, const L& lane, int in_warp, uint32_t* words) : warp(words) {
+    if constexpr (PAIRING == kCrossed) {
+      static_assert(NV == 2 && VE * sizeof(T) == 16, "kCrossing");
+      const int start = in_warp * (a.hd * (int)sizeof(T) / 4 + 1);
+      own = words + start;
+      auto of = [&](int c) {
+        if (c < 0 || c >= a.rd) return kCrossing * 4;
+        return start * 4 + (c < lane.half ? c + lane.half : c - lane.half) * (int)sizeof(T);
+      };
+#pragma unroll
+      for (int i = 0; i < M; ++i) from[i] = (uint32_t)of(lane.component(2 * i)) | (uint32_t)of(lane.component(2 * i + 1)) << 16;
+    }
+  }
+  // u: the partners of r
+  __device__ __forceinline__ void cross(const L& lane, const Pack<T, VE> (&r)[NV], uint64_t (&u)[L::M]) const {
+    if constexpr (PAIRING == kCrossed) {
+      __syncwarp();                                           // (the head before has been read)
+#pragma unroll
+      for (int s = 0; s < NV; ++s)
+        if (lane.has(s)) {
+          uint32_t* to = own + lane.at[s] * (int)sizeof(T) / 4;
+          to[0] = r[s].v.x; to[1] = r[s].v.y; to[2] = r[s].v.z; to[3] = r[s].v.w;
+        }
+      __syncwarp();
+      const uint8_t* base = reinterpret_cast<const uint8_t*>(warp);
+#pragma unroll
+      for (int i = 0; i < M; ++i)
+        u[i] = pack_f32x2(to_f(*reinterpret_cast<const T*>(base + (from[i] & 0xffffu))),
+                          to_f(*reinterpret_cast<const T*>(base + (from[i] >> 16))));
+    }
+  }
+};
+
 // Sine and cosine of a lane's pairs at a token's position, and the rotation of what it holds of a head by them.
 template <typename T, int VE, int NV, int PAIRING, int GROUP>
 struct Angles {
   using L = Lane<T, VE, NV, PAIRING, GROUP>;
-  static constexpr int M = L::M, A = PAIRING == kApart ? M / 2 : 1, I = PAIRING == kInside ? M : 1;
-  uint64_t c2[A], s2[A], n2[A];                               // kApart: of two pairs; n2: the sines negated
+  static constexpr int M = L::M, A = PAIRING == kApart ? M / 2 : PAIRING == kCrossed ? M : 1, I = PAIRING == kInside ? M : 1;
+  // of two pairs (kApart; n2: the sines negated) or two components (kCrossed; s2 with the sign that they take their partner with)
+  uint64_t c2[A], s2[A], n2[A];
   float c1[I], s1[I];                                         // kInside
 
   __device__ __forceinline__ void set(const HeadArgs& a, const double* turns, const L& lane, int g, unsigned token) {
@@ -250,6 +296,21 @@ struct Angles {
         s2[i] = pack_f32x2(s[0], s[1]);
         n2[i] = pack_f32x2(-s[0], -s[1]);
       }
+    } else if constexpr (PAIRING == kCrossed) {
+#pragma unroll
+      for (int i = 0; i < A; ++i) {
+        float c[2] = {1.f, 1.f}, s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int at = lane.component(2 * i + e);
+          if (at >= 0 && at < a.rd) {
+            angle(at < lane.half ? at : at - lane.half, &c[e], &s[e]);
+            if (at < lane.half) s[e] = -s[e];
+          }
+        }
+        c2[i] = pack_f32x2(c[0], c[1]);
+        s2[i] = pack_f32x2(s[0], s[1]);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < I; ++i) {
@@ -258,8 +319,12 @@ struct Angles {
       }
     }
   }
-  __device__ __forceinline__ void rotate(const HeadArgs& a, const L& lane, int g, uint64_t (&v)[M]) const {
-    if constexpr (PAIRING == kApart) {
+  // u: the partners (kCrossed)
+  __device__ __forceinline__ void rotate(const HeadArgs& a, const L& lane, int g, uint64_t (&v)[M], const uint64_t (&u)[M]) const {
+    if constexpr (PAIRING == kCrossed) {
+#pragma unroll
+      for (int i = 0; i < A; ++i) v[i] = fma_f32x2(v[i], c2[i], mul_f32x2(u[i], s2[i]));
+    } else if constexpr (PAIRING == kApart) {
       if (lane.paired) {
 #pragma unroll
         for (int i = 0; i < A; ++i) {
@@ -360,20 +425,32 @@ __device__ __forceinline__ void copy_rest(const HeadArgs& a, const L& lane, cons
 template <typename T, int VE, int NV, int PAIRING, int KIND, int GROUP>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_fwd_kernel(const __grid_constant__ HeadArgs a) {
   using L = Lane<T, VE, NV, PAIRING, GROUP>;
-  constexpr int M = L::M, U = VE > 1 ? 4 : 1;
+  constexpr bool CROSSED = PAIRING == kCrossed;
+  constexpr int M = L::M, U = CROSSED ? 2 : VE > 1 ? 4 : 1;
   __shared__ double turns[kMaxPairs];
   __shared__ __align__(16) float weights[KIND == kNorm ? 2 : 1][KIND == kNorm ? 2 * kMaxPairs : 4];
+  // kCrossed: the weights of the components' partners
+  __shared__ __align__(16) float opposite[CROSSED && KIND == kNorm ? 2 : 1][CROSSED && KIND == kNorm ? 2 * kMaxPairs : 4];
+  __shared__ uint32_t crossing[CROSSED ? kThreads / 32 : 1][CROSSED ? kCrossing + 1 : 1];
   grid_dependency_launch();
   for (int i = threadIdx.x; i < a.rd / 2; i += kThreads) turns[i] = a.turns[i];
   if constexpr (KIND == kNorm) {
     for (int c = threadIdx.x; c < 2 * a.hd; c += kThreads)
       weights[c >= a.hd][c >= a.hd ? c - a.hd : c] = weight_of<T>(a, c >= a.hd, c >= a.hd ? c - a.hd : c);
+    if constexpr (CROSSED) {
+      for (int i = threadIdx.x; i < 2 * a.hd; i += kThreads) {
+        const int which = i >= a.hd, c = which ? i - a.hd : i, half = a.rd / 2;
+        opposite[which][c] = weight_of<T>(a, which, c < half ? c + half : c < a.rd ? c - half : c);
+      }
+    }
   }
+  if (CROSSED && threadIdx.x < kThreads / 32) crossing[threadIdx.x][kCrossing] = 0u;
   __syncthreads();
   const int group = GROUP > 0 ? GROUP : a.group;
   const int warp = threadIdx.x >> 5, g = threadIdx.x & (group - 1);
   const int per_warp = 32 / group, in_warp = (threadIdx.x & 31) / group;
   const L lane(a, g);
+  const Partners<T, VE, NV, PAIRING, GROUP> partners(a, lane, in_warp, crossing[CROSSED ? warp : 0]);
   const unsigned stride = gridDim.x * (kThreads / 32), units = a.tokens * (unsigned)a.chunks[0];
   const long long x_step = a.x_head * per_warp, out_step = a.out_head * per_warp;
   unsigned unit = blockIdx.x * (kThreads / 32) + warp;
@@ -399,17 +476,24 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_fwd_kernel(const _
     auto work = [&](int h, auto heads) {
 #pragma unroll
       for (int k = 0; k < heads(); ++k) {
-        uint64_t v[M];
+        uint64_t v[M], other[M];
         unpack<T, VE, NV>(raw[k], v);
+        partners.cross(lane, raw[k], other);
         if constexpr (KIND == kNorm) {
           const float r = rsqrtf(group_sum<GROUP>(dot(v, v), a.group) * a.inv_hd + a.eps);
           const uint64_t r2 = pack_f32x2(r, r);
+          const int which = u.head + (h + k) * per_warp >= a.queries;
           uint64_t w[M];
-          weights_of<VE, NV>(weights[u.head + (h + k) * per_warp >= a.queries], lane, w);
+          weights_of<VE, NV>(weights[which], lane, w);
 #pragma unroll
           for (int i = 0; i < M; ++i) v[i] = mul_f32x2(v[i], mul_f32x2(r2, w[i]));
+          if constexpr (CROSSED) {
+            weights_of<VE, NV>(opposite[which], lane, w);
+#pragma unroll
+            for (int i = 0; i < M; ++i) other[i] = mul_f32x2(other[i], mul_f32x2(r2, w[i]));
+          }
         }
-        angles.rotate(a, lane, g, v);
+        angles.rotate(a, lane, g, v, other);
         if (h + k < u.count) {
           Pack<T, VE> res[NV];
           pack<T, VE, NV>(v, res);
@@ -466,16 +550,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
   constexpr int N = L::N, M = L::M;
   constexpr bool RING = VE > 1;
   constexpr int R = RING ? kBwdSteps : 1;
+  constexpr bool CROSSED = PAIRING == kCrossed;
   extern __shared__ __align__(16) uint8_t ring[];             // [R][2 NV][kThreads] vectors
   __shared__ double turns[kMaxPairs];
   __shared__ __align__(16) float weights[2 * kMaxPairs];
   __shared__ float reduced[kThreads / 32][2 * kMaxPairs];
+  __shared__ uint32_t crossing[CROSSED ? kThreads / 32 : 1][CROSSED ? kCrossing + 1 : 1];
   grid_dependency_launch();
   for (int i = threadIdx.x; i < a.rd / 2; i += kThreads) turns[i] = a.turns[i];
+  if (CROSSED && threadIdx.x < kThreads / 32) crossing[threadIdx.x][kCrossing] = 0u;
   const int group = GROUP > 0 ? GROUP : a.group;
   const int warp = threadIdx.x >> 5, g = threadIdx.x & (group - 1);
   const int per_warp = 32 / group, in_warp = (threadIdx.x & 31) / group;
   const L lane(a, g);
+  const Partners<T, VE, NV, PAIRING, GROUP> partners(a, lane, in_warp, crossing[CROSSED ? warp : 0]);
   const unsigned stride = gridDim.x * (kThreads / 32);
   unsigned unit = blockIdx.x * (kThreads / 32) + warp;        // of the kind at hand
 #pragma unroll 1
@@ -547,9 +635,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_bwd_kernel(const _
           slot = slot == R - 1 ? 0 : slot + 1;
         }
         uint64_t v[M], d[M], gw[M];
+        partners.cross(lane, rd, gw);
         unpack<T, VE, NV>(rx, v);
         unpack<T, VE, NV>(rd, d);
-        angles.rotate(a, lane, g, d);                       // (a.sign: backwards)
+        angles.rotate(a, lane, g, d, gw);                     // (a.sign: backwards)
         weights_of<VE, NV>(weights, lane, gw);
 #pragma unroll
         for (int i = 0; i < M; ++i) gw[i] = mul_f32x2(d[i], gw[i]);
@@ -666,15 +755,18 @@ int dispatch(HeadArgs& a, int* parts, cudaStream_t stream) {
   // in place nothing but what turns is touched (3062 tokens, 32 heads of 80 fp16, 32 of them turned: 8.7 -> 6.7 us)
   if (PASS == kRotate && a.x == a.out && a.rd < a.hd) a.hd = a.hd % VE == 0 ? (a.rd + VE - 1) / VE * VE : a.rd;
   if (a.hd == 0) return DD_OK;
-  // whole vectors need heads of whole vectors at 16-byte addresses, two vectors per lane of a warp, and pairs that lie inside
-  // a vector or whole vectors apart; else single components, sixteen per lane
-  const bool vectors = a.hd % VE == 0 && a.hd <= 64 * VE && (a.neighbours || a.rd % (2 * VE) == 0) &&
-                       aligned(a.x, a.x_row, a.x_head, size) && aligned(a.dy, a.dy_row, a.dy_head, size) &&
-                       aligned(a.out, a.out_row, a.out_head, size);
+  // whole vectors need heads of whole vectors at 16-byte addresses and two vectors per lane of a warp; else single components,
+  // sixteen per lane
+  const bool vectors = a.hd % VE == 0 && a.hd <= 64 * VE && aligned(a.x, a.x_row, a.x_head, size) &&
+                       aligned(a.dy, a.dy_row, a.dy_head, size) && aligned(a.out, a.out_row, a.out_head, size);
+  // halves that are not whole vectors (rd / 2 = 25, say): partners by way of shared memory, 16384 tokens, 48 heads of 128 bf16 of
+  // which 50 components turn, us, rotation / in place / norm and rotation / backward: 77 / 39 / 96 / 174 (4 heads per unit 188),
+  // single components 131 / 93 / 137 / 272
+  const bool crossed = vectors && !a.neighbours && a.rd % (2 * VE) != 0;
   for (a.group = 1; a.group * (vectors ? 2 * VE : 16) < a.hd; a.group *= 2) {}
   const int most = current_sm_count() * kCtasPerSm, warps = kThreads / 32, per_warp = 32 / a.group;
   long long units;
-  for (int rounds = PASS == kBackward ? kMostRoundsBackward : kMostRounds;; rounds /= 2) {
+  for (int rounds = PASS == kBackward && !crossed ? kMostRoundsBackward : kMostRounds;; rounds /= 2) {
     units = 0;
     for (int k = 0; k < 3; ++k) {
       a.chunk[k] = rounds * per_warp;
@@ -690,7 +782,7 @@ int dispatch(HeadArgs& a, int* parts, cudaStream_t stream) {
   *parts = ctas;
   if (!vectors) return launch<T, 1, 16, kInside, 0, PASS>(a, ctas, stream);
   // groups of 4 to 32 lanes that all have their vectors know their size beforehand: shuffles and addresses without questions
-  // (16384 tokens, 48 heads of 128 bf16, backward: 108 -> 98 us)
+  // (backward 108 -> 98 us when it was added; 96 now)
   const int full = a.hd == 2 * VE * a.group ? a.group : 0;
   if (a.neighbours) {
     if (full == 4) return launch<T, VE, 2, kInside, 4, PASS>(a, ctas, stream);
@@ -699,6 +791,7 @@ int dispatch(HeadArgs& a, int* parts, cudaStream_t stream) {
     if (full == 32) return launch<T, VE, 2, kInside, 32, PASS>(a, ctas, stream);
     return launch<T, VE, 2, kInside, 0, PASS>(a, ctas, stream);
   }
+  if (crossed) return launch<T, VE, 2, kCrossed, 0, PASS>(a, ctas, stream);
   if (full == 4) return launch<T, VE, 2, kApart, 4, PASS>(a, ctas, stream);
   if (full == 8) return launch<T, VE, 2, kApart, 8, PASS>(a, ctas, stream);
   if (full == 16) return launch<T, VE, 2, kApart, 16, PASS>(a, ctas, stream);

@@ -486,3 +486,50 @@ def test_offsets_beyond_32_bits():
     y = ops.qk_norm_rope(keep, 2, 1, 1, rotary=r)
     ops.qk_norm_rope_(x, 2, 1, 1, rotary=r)
     assert torch.equal(x, y)
+
+
+HALVES = [(128, 50), (128, 2), (128, 126), (64, 34), (256, 24), (512, 510), (512, 4), (40, 38), (8, 6), (16, 10), (24, 4)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("hd,dim", HALVES)
+def test_halves_that_are_not_whole_vectors(hd, dim, dtype):
+    if dtype == FP32 and hd == 512:
+        hd, dim = 256, dim // 4 * 2                           # (the most that a warp holds as vectors)
+    torch.manual_seed(hd + dim)
+    r = ops.Rotary(theta=10000.0, dim=dim)
+    x = torch.randn(70, 9, hd, device="cuda").to(dtype).requires_grad_()
+    z = angles(r, hd, torch.arange(70, device="cuda") % 35 + 5)
+    y = ops.rope(x, 35, 7, rotary=r, offset=5)
+    assert_turned(y, x, z, r, 7, dtype)
+    dy = torch.randn_like(y)
+    assert_turned(torch.autograd.grad(y, x, dy)[0], dy, z.conj(), r, 7, dtype)
+    flat = x.detach().clone()
+    assert torch.equal(ops.rope_(flat, 35, 7, rotary=r, offset=5), y)
+    w = [(1 + 0.2 * torch.randn(hd, device="cuda")).to(dtype) for _ in range(2)]
+    y, _ = run_norm(x.detach() * 2, *w, 4, 3, r, 35, offset=5)
+    flat = x.detach() * 2
+    assert torch.equal(ops.qk_norm_rope_(flat, 35, 4, 3, *[t.detach() for t in w], rotary=r, offset=5), y)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_many_heads_with_halves_that_are_not_whole_vectors(dtype):
+    torch.manual_seed(2)
+    r = ops.Rotary(dim=50)
+    x = torch.randn(900, 30, 128, device="cuda").to(dtype)
+    assert_turned(ops.rope(x, 900, 29, rotary=r), x, angles(r, 128, torch.arange(900, device="cuda")), r, 29, dtype)
+    w = [(1 + 0.2 * torch.randn(128, device="cuda")).to(dtype) for _ in range(2)]
+    run_norm(x, *w, 19, 5, r, 300)
+
+
+@pytest.mark.parametrize("dim", [50, 32])
+def test_what_stays_is_a_copy_whatever_it_is(dim):
+    x = torch.randn(11, 5, 128, device="cuda", dtype=BF16)
+    r = ops.Rotary(dim=dim)
+    clean = ops.rope(x, 11, 4, rotary=r)
+    for k, v in enumerate((float("inf"), float("nan"), -float("inf"))):
+        x[:, :, dim + k::7] = v
+    for y in (ops.rope(x, 11, 4, rotary=r), ops.rope_(x.clone(), 11, 4, rotary=r)):
+        assert torch.equal(y[..., :dim], torch.cat([clean[:, :4], x[:, 4:]], 1)[..., :dim])
+        # (of a NaN the bits behind its first are not kept by a conversion)
+        torch.testing.assert_close(y[..., dim:], x[..., dim:], rtol=0.0, atol=0.0, equal_nan=True)
