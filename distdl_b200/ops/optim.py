@@ -174,7 +174,5 @@ def clip_grad_norm_(tensors, max_norm: float, norm: torch.Tensor = None) -> torc
     if not given:
         norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
     _grad_norm(tensors, lists, norm, None, max_norm, given, True)
-    if any([t.is_inference() for t in tensors]):
-        tensors = [t for t in tensors if not t.is_inference()]
-    torch.autograd.graph.increment_version(tensors)
+    torch.autograd.graph.increment_version(tensors)           # (passes over tensors of inference mode)
     return norm

@@ -367,8 +367,7 @@ def rope_in_place(qkv, seq, nheads, rotary, offset=0, ranges=None, positions=Non
             raise RuntimeError("a leaf that requires a gradient cannot be turned in place: use ops.rope, or torch.no_grad()")
         return _RopeInPlaceFn.apply(qkv, (shape, nheads, where))
     _call(_ROTATE, read, read, nheads, 0, where)
-    if not qkv.is_inference():
-        torch.autograd.graph.increment_version(qkv)
+    torch.autograd.graph.increment_version(qkv)               # (passes over tensors of inference mode)
     return qkv
 
 
@@ -501,8 +500,7 @@ def qk_norm_rope_(qkv: torch.Tensor, seq: int, hq: int, hkv: int, q_weight=None,
         raise ValueError("a tensor that is changed in place must not overlap itself: use ops.qk_norm_rope")
     if native and (qkv.stride(2) == 1 or qkv.shape[2] == 1):
         _call(_FORWARD, qkv, qkv, hq, hkv, where, 1.0, wq, wk, float(eps))
-        if not qkv.is_inference():
-            torch.autograd.graph.increment_version(qkv)
+        torch.autograd.graph.increment_version(qkv)
         return qkv
     with torch.no_grad():
         qkv.copy_(_plain_qk_norm_rope(qkv, hq, hkv, wq, wk, eps, where))

@@ -161,3 +161,16 @@ def test_a_tensor_of_more_than_32_bits():
     want = math.sqrt(50 * 4 + 7)
     assert abs(ops.clip_grad_norm_([g], 1.0).item() - want) < 1e-5
     assert abs(g[-1].item() - 2 / want) <= 2.0 ** -8 * 2 / want and g[1 << 30] == 0
+
+
+def test_gradients_of_inference_mode_among_others():
+    ours = torch.randn(1000, device="cuda")
+    keep = ours.clone()
+    with torch.inference_mode():
+        other = torch.randn(77, device="cuda")
+        want = math.sqrt(ours.double().square().sum().item() + other.double().square().sum().item())
+        assert abs(ops.clip_grad_norm_([other, ours], 1.0).item() - want) <= 2.0 ** -23 * want
+    version = ours._version
+    ops.clip_grad_norm_([other, ours], 0.5)
+    assert ours._version > version
+    assert torch.allclose(ours, keep * (0.5 / want), rtol=1e-5, atol=0)
