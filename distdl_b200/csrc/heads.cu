@@ -420,13 +420,14 @@ __device__ __forceinline__ void copy_rest(const HeadArgs& a, const L& lane, cons
 
 // Forward.  Four heads' loads are in flight together and four heads are worked on side by side: that hides more than a
 // third or fourth CTA per SM or loads a step ahead would (16384 tokens, 48 heads of 128 bf16, us, rotation / norm and rotation:
-// two heads and 4 / 3 CTAs 80.7 / 87.4, two and the next two on their way 75.5 / 72.3, four 64.7 / 67.6).  Query and key heads
+// two heads and 4 / 3 CTAs 80.7 / 87.4, two and the next two on their way 75.5 / 72.3, four 64.7 / 67.6; with partners from other
+// lanes two 77.1 / 95.7, four 71.5 / 105.5, which spill with the norm: two there).  Query and key heads
 // are one kind here, which share their angles; their weights are in shared memory.
 template <typename T, int VE, int NV, int PAIRING, int KIND, int GROUP>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) heads_fwd_kernel(const __grid_constant__ HeadArgs a) {
   using L = Lane<T, VE, NV, PAIRING, GROUP>;
   constexpr bool CROSSED = PAIRING == kCrossed;
-  constexpr int M = L::M, U = CROSSED ? 2 : VE > 1 ? 4 : 1;
+  constexpr int M = L::M, U = CROSSED && KIND == kNorm ? 2 : VE > 1 ? 4 : 1;
   __shared__ double turns[kMaxPairs];
   __shared__ __align__(16) float weights[KIND == kNorm ? 2 : 1][KIND == kNorm ? 2 * kMaxPairs : 4];
   // kCrossed: the weights of the components' partners
@@ -760,7 +761,7 @@ int dispatch(HeadArgs& a, int* parts, cudaStream_t stream) {
   const bool vectors = a.hd % VE == 0 && a.hd <= 64 * VE && aligned(a.x, a.x_row, a.x_head, size) &&
                        aligned(a.dy, a.dy_row, a.dy_head, size) && aligned(a.out, a.out_row, a.out_head, size);
   // halves that are not whole vectors (rd / 2 = 25, say): partners by way of shared memory, 16384 tokens, 48 heads of 128 bf16 of
-  // which 50 components turn, us, rotation / in place / norm and rotation / backward: 77 / 39 / 96 / 174 (4 heads per unit 188),
+  // which 50 components turn, us, rotation / in place / norm and rotation / backward: 72 / 39 / 96 / 174 (4 heads per unit 188),
   // single components 131 / 93 / 137 / 272
   const bool crossed = vectors && !a.neighbours && a.rd % (2 * VE) != 0;
   for (a.group = 1; a.group * (vectors ? 2 * VE : 16) < a.hd; a.group *= 2) {}
