@@ -462,7 +462,8 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
   grid_dependency_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < a.E; e += kWarps * 32) s_hist[e] = 0;
-  for (int e = threadIdx.x; e < 32 * C; e += kWarps * 32) s_bias[place_of<C>(e / C, e % C)] = a.bias != nullptr && e < a.E ? a.bias[e] : 0.f;
+  for (int e = threadIdx.x; e < 32 * C; e += kWarps * 32)
+    s_bias[place_of<C>(e / C, e % C)] = a.bias != nullptr && e < a.E ? a.bias[e] : 0.f;
   __syncthreads();
   const int first = lane * C;
   const int left = min(max(a.E - first, 0), C);               // experts of this lane
@@ -657,7 +658,8 @@ route_slot_kernel(const int* ids, int tokens, int k, int E, int E4, int capacity
 //   dl_e = f_e (G_e + p_e (q_e - sum p q)),  f = 1 (softmax) or 1 - s_e (sigmoid)
 template <typename T, int C>
 __global__ void __launch_bounds__(kWarps * 32)
-route_bwd_kernel(const __grid_constant__ RouteArgs a, const float* __restrict__ dw, const float* __restrict__ dprob, T* __restrict__ dlogits) {
+route_bwd_kernel(const __grid_constant__ RouteArgs a, const float* __restrict__ dw, const float* __restrict__ dprob,
+                 T* __restrict__ dlogits) {
   __shared__ __align__(16) float s_row[kWarps][32 * C];
   grid_dependency_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
