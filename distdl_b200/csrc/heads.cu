@@ -51,10 +51,11 @@ struct HeadArgs {
   long long out_row, out_head;
   const void* wq;             // [hd] or null (ones)
   const void* wk;
-  const void* positions;      // [seq] of 4 or 8 bytes, of token % seq, or null: offset + token % seq
+  const void* positions;      // [seq] of 4 or 8 bytes, of token % seq, or null: offset + token % seq, and `jump` more from the
+                              // place `split` on (a sequence of two ranges of positions)
   float* partial;             // backward: [gridDim.x][2][hd], or null
-  long long offset;
-  unsigned tokens, seq;
+  long long offset, jump;
+  unsigned tokens, seq, split;
   int heads[3];               // query, key and other heads (those are copied; none in place)
   int chunk[3], chunks[3];    // heads per unit (whole rounds of a warp's groups), units per token
   int hd, rd, group;          // group: lanes per head (a power of two)
@@ -273,9 +274,10 @@ struct Angles {
 
   __device__ __forceinline__ void set(const HeadArgs& a, const double* turns, const L& lane, int g, unsigned token) {
     long long pos;
-    if (a.positions == nullptr) pos = a.offset + token % a.seq;
-    else if (a.wide_positions) pos = reinterpret_cast<const long long*>(a.positions)[token % a.seq];
-    else pos = reinterpret_cast<const int*>(a.positions)[token % a.seq];
+    const unsigned at = token % a.seq;
+    if (a.positions == nullptr) pos = a.offset + at + (at >= a.split ? a.jump : 0);
+    else if (a.wide_positions) pos = reinterpret_cast<const long long*>(a.positions)[at];
+    else pos = reinterpret_cast<const int*>(a.positions)[at];
     const double place = (double)pos;
     auto angle = [&](int pair, float* c, float* s) {
       double t = place * turns[pair];
@@ -822,6 +824,8 @@ DD_API int dd_heads_parts() { return current_sm_count() * kCtasPerSm; }
 //                      accumulate added to what is there, fp32; partial: dd_heads_parts() * 2 * hd floats where they are wanted
 // Weights [hd] of x's type, or fp32 with wide_weights, or null.  turns [rd / 2]: frequencies in turns per position (host
 // memory); positions [seq] on the device (4 or, wide_positions, 8 bytes each) of token % seq, or null for offset + token % seq.
+// Where a second range of positions follows the first in every sequence, two more numbers stand behind the call: the place it begins
+// at, and what is added to its positions.
 struct HeadsCall {
   const void *x, *dy;
   void* out;
@@ -835,11 +839,16 @@ struct HeadsCall {
   float magnitude, sign, eps;
 };
 static_assert(sizeof(HeadsCall) == 19 * 8 + 14 * 4, "packed without holes");
+struct SecondRange { long long split, jump; };
 
 DD_API int dd_heads(const void* packed, int bytes, void* stream) {
   HeadsCall c;
-  if (packed == nullptr || bytes != (int)sizeof c) return DD_ERR_BAD_ARG;
+  SecondRange second = {0x7fffffffLL, 0};
+  const bool two = bytes == (int)(sizeof c + sizeof second);
+  if (packed == nullptr || (bytes != (int)sizeof c && !two)) return DD_ERR_BAD_ARG;
   memcpy(&c, packed, sizeof c);
+  if (two) memcpy(&second, static_cast<const char*>(packed) + sizeof c, sizeof second);
+  if (second.split < 0) return DD_ERR_BAD_ARG;
   const bool back = c.pass == kBackward;
   if (c.pass < kRotate || c.pass > kBackward || (c.pass == kRotate && c.hk != 0)) return DD_ERR_BAD_ARG;
   if (c.tokens < 0 || c.hq < 0 || c.hk < 0 || c.rest < 0 || c.hd < 1 || c.rd < 0 || c.rd > c.hd || c.rd % 2 != 0)
@@ -860,6 +869,7 @@ DD_API int dd_heads(const void* packed, int bytes, void* stream) {
   a.queries = c.hq;
   a.hd = c.hd; a.rd = c.rd; a.neighbours = c.neighbours;
   a.positions = c.positions; a.wide_positions = c.wide_positions; a.offset = c.offset;
+  a.split = second.split > 0x7fffffffLL ? 0x7fffffffu : (unsigned)second.split; a.jump = second.jump;
   a.magnitude = c.magnitude;
   a.inv_hd = 1.f / (float)c.hd;
   a.sign = back ? -1.f : c.pass == kRotate ? c.sign : 1.f;

@@ -18,6 +18,7 @@ _native.declare("dd_heads", [ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p])
 _native.declare("dd_heads_parts", [])
 # struct HeadsCall of csrc/heads.cu: ten addresses, nine long numbers, eleven numbers, three fp32 values
 _CALL = struct.Struct("=10Q9q11i3f")
+_SECOND = struct.Struct("=2q")                  # and what may follow it
 _ROTATE, _FORWARD, _BACKWARD = 0, 1, 2
 
 _DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -139,36 +140,51 @@ def _frequencies(rotary: Rotary, dim: int) -> tuple:
     return tuple(out)
 
 
-_range_positions = {}
-
-
-def _positions_of_ranges(ranges, device) -> torch.Tensor:
-    """Positions of a local sequence made of several ranges ``((start, length), ...)``, kept per device."""
-    key = (tuple((int(a), int(n)) for a, n in ranges), str(device))
-    p = _range_positions.get(key)
-    if p is None:
-        p = torch.cat([torch.arange(a, a + n, dtype=torch.int64, device=device) for a, n in key[0]])
-        if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
-            _range_positions[key] = p       # (what a captured graph makes is the graph's own)
-    return p
+def _place_of_ranges(ranges, tokens, seq, device):
+    """(positions or None, offset, second) of a local sequence made of several ranges ``((start, length), ...)``: up to two of
+    them travel with the call, ``second = (first place of the second, what its positions are ahead of the first's)``; of more
+    the positions are listed on the device.  Nothing is kept: what one call makes belongs to its stream, mode and graph."""
+    runs = []
+    for a, n in ranges:
+        a, n = int(a), int(n)
+        if n < 0:
+            raise ValueError(f"a range of positions has a length that is not negative, not {n}")
+        if n and runs and runs[-1][0] + runs[-1][1] == a:
+            runs[-1] = (runs[-1][0], runs[-1][1] + n)
+        elif n:
+            runs.append((a, n))
+    n = sum(r[1] for r in runs)
+    if n != seq:
+        raise ValueError(f"the ranges hold {n} positions, a sequence has {seq} tokens")
+    if tokens % max(1, n) or (n == 0 and tokens):
+        raise ValueError(f"{tokens} tokens are not whole sequences of {n}")
+    if len(runs) > 2:
+        return torch.cat([torch.arange(a, a + m, dtype=torch.int64, device=device) for a, m in runs]), 0, None
+    if not runs:
+        return None, 0, None
+    (a, n), second = runs[0], None
+    if len(runs) == 2:
+        second = (n, runs[1][0] - n - a)
+    return None, a, second
 
 
 def _where(qkv, rotary, seq, offset, ranges, positions):
-    """The arguments that say how ``qkv [tokens, heads, head_dim]`` is turned: (rotary, positions or None, seq, offset)."""
+    """The arguments that say how ``qkv [tokens, heads, head_dim]`` is turned: (rotary, positions or None, seq, offset,
+    second): the position of a token of place ``i`` (its index modulo ``seq``) is ``positions[i]``, or ``offset + i``, and from
+    the place ``second[0]`` on ``second[1]`` more."""
     if rotary is None:
-        return None, None, 1, 0
+        return None, None, 1, 0, None
     if not isinstance(rotary, Rotary):
         raise TypeError(f"rotary must be an ops.Rotary, not {type(rotary).__name__}")
     if ranges is not None:
         if positions is not None or offset:
             raise ValueError("give positions, ranges or an offset, not several of them")
-        positions = _positions_of_ranges(ranges, qkv.device)
-        if positions.numel() != seq:
-            raise ValueError(f"the ranges hold {positions.numel()} positions, a sequence has {seq} tokens")
+        positions, offset, second = _place_of_ranges(ranges, qkv.shape[0], seq, qkv.device)
+        return rotary, positions, max(1, int(seq)), offset, second
     if positions is None:
         if seq < 1:
             raise ValueError(f"a sequence has at least one token, not {seq}")
-        return rotary, None, int(seq), int(offset)
+        return rotary, None, int(seq), int(offset), None
     if offset:
         raise ValueError("give positions or an offset, not both")
     if positions.dtype not in (torch.int64, torch.int32):
@@ -181,14 +197,20 @@ def _where(qkv, rotary, seq, offset, ranges, positions):
                          f"sequence")
     if positions.dim() != 1 or not positions.is_contiguous():
         positions = positions.reshape(-1).contiguous()
-    return rotary, positions, max(1, n), 0
+    return rotary, positions, max(1, n), 0, None
 
 
-def _angles(qkv, rotary, positions, seq, offset):
+def _angles(qkv, where):
     """(cos, sin) [tokens, 1, dim / 2] times the magnitude, fp32 from 64 bits (plain path)."""
+    rotary, positions, seq, offset, second = where
     f = torch.tensor(rotary.frequencies(qkv.shape[2]), dtype=torch.float64, device=qkv.device)
     at = torch.arange(qkv.shape[0], device=qkv.device) % seq
-    at = at + offset if positions is None else positions[at]
+    if positions is not None:
+        at = positions[at]
+    elif second is not None:
+        at = torch.where(at < second[0], at, at + second[1]) + offset
+    else:
+        at = at + offset
     angle = (at.double().unsqueeze(1) * f).unsqueeze(1)
     wide = torch.float64 if qkv.dtype == torch.float64 else torch.float32
     return (rotary.scale * angle.cos()).to(wide), (rotary.scale * angle.sin()).to(wide)
@@ -209,8 +231,8 @@ def _wide(x):
 
 
 def _plain_rope(qkv, nheads, where, sign=1.0):
-    rotary, positions, seq, offset = where
-    cos, sin = _angles(qkv, rotary, positions, seq, offset)
+    rotary = where[0]
+    cos, sin = _angles(qkv, where)
     sin = sign * sin
     y = _rotated(_wide(qkv[:, :nheads]), cos, sin, rotary.rotated(qkv.shape[2]), rotary.interleaved)
     return torch.cat([y.to(qkv.dtype), qkv[:, nheads:]], dim=1)
@@ -231,14 +253,17 @@ def _call(kind, x, out, hq, hkv, where, sign=1.0, wq=None, wk=None, eps=0.0, dy=
     tokens, heads, hd = x.shape
     xs, os = x.stride(), out.stride()
     ds = xs if dy is None else dy.stride()
-    rotary, positions, seq, offset = where
+    rotary, positions, seq, offset, second = where
     dim, near, address, scale = (0, 0, 0, 1.0) if rotary is None else rotary._plan(hd)[:4]
     w = wk if wq is None else wq
-    call_on(x, "dd_heads", _CALL.pack(
+    call = _CALL.pack(
         x.data_ptr(), 0 if dy is None else dy.data_ptr(), out.data_ptr(), ptr(wq), ptr(wk), ptr(dwq), ptr(dwk), ptr(partial),
         0 if positions is None else positions.data_ptr(), address, xs[0], xs[1], ds[0], ds[1], os[0], os[1], tokens, offset, seq,
         kind, _DTYPE[x.dtype], hq, hkv, heads - hq - hkv, hd, dim, near, w is not None and w.dtype == torch.float32,
-        positions is not None and positions.dtype == torch.int64, accumulate, scale, sign, eps), _CALL.size)
+        positions is not None and positions.dtype == torch.int64, accumulate, scale, sign, eps)
+    if second is not None:
+        call += _SECOND.pack(*second)
+    call_on(x, "dd_heads", call, len(call))
 
 
 def _rotated_copy(qkv, nheads, where, sign):
@@ -382,9 +407,9 @@ def _plain_qk_norm_rope(qkv, hq, hkv, wq, wk, eps, where):
     u = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps)
     parts = [u[:, :hq] if wq is None else u[:, :hq] * wq.to(x.dtype), u[:, hq:] if wk is None else u[:, hq:] * wk.to(x.dtype)]
     y = torch.cat(parts, dim=1)
-    rotary, positions, seq, offset = where
+    rotary = where[0]
     if rotary is not None:
-        cos, sin = _angles(qkv, rotary, positions, seq, offset)
+        cos, sin = _angles(qkv, where)
         y = _rotated(y, cos, sin, rotary.rotated(qkv.shape[2]), rotary.interleaved)
     return torch.cat([y.to(qkv.dtype), qkv[:, nh:]], dim=1)
 
