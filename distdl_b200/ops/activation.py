@@ -7,7 +7,7 @@ from __future__ import annotations
 import torch
 
 from .. import _native
-from ._util import stream_ptr, use_native
+from ._util import _modes, stream_ptr, use_native
 
 
 class _SwiGLUFn(torch.autograd.Function):
@@ -72,16 +72,27 @@ def gelu(x: torch.Tensor) -> torch.Tensor:
 _rope_cache = {}
 
 
-def rope_table(seq: int, head_dim: int, theta: float, device) -> torch.Tensor:
-    """[seq, head_dim/2, 2] fp32 table of (cos, sin)."""
-    key = (seq, head_dim, theta, str(device))
+def _host_table(seq, head_dim, theta):
+    inv = 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.float64, device="cpu") / head_dim))
+    ang = torch.outer(torch.arange(seq, dtype=torch.float64, device="cpu"), inv)
+    return torch.stack([ang.cos(), ang.sin()], dim=-1).float()
+
+
+def _kept_table(key, make, device):
+    """The table of ``key``, copied from the host when it is first asked for: the copy has ended when this returns, so that
+    every stream may read it.  Under a dispatch mode (fake tensors, say) tables are made for the call alone."""
+    if _modes():
+        return make().to(device).contiguous()
     t = _rope_cache.get(key)
     if t is None:
-        inv = 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.float64) / head_dim))
-        ang = torch.outer(torch.arange(seq, dtype=torch.float64), inv)
-        t = torch.stack([ang.cos(), ang.sin()], dim=-1).float().to(device).contiguous()
-        _rope_cache[key] = t
+        with torch.inference_mode(False):
+            t = _rope_cache[key] = make().to(device).contiguous()
     return t
+
+
+def rope_table(seq: int, head_dim: int, theta: float, device) -> torch.Tensor:
+    """[seq, head_dim/2, 2] fp32 table of (cos, sin)."""
+    return _kept_table((seq, head_dim, theta, str(device)), lambda: _host_table(seq, head_dim, theta), device)
 
 
 class _RopeFn(torch.autograd.Function):
@@ -107,13 +118,16 @@ class _RopeFn(torch.autograd.Function):
 
 def rope_table_ranges(ranges, head_dim: int, theta: float, device) -> torch.Tensor:
     """Table for a local sequence made of several position ranges ``((start, length), ...)``."""
-    key = (tuple(ranges), head_dim, theta, str(device))
-    t = _rope_cache.get(key)
-    if t is None:
-        full = rope_table(max(a + n for a, n in ranges), head_dim, theta, device)
-        t = torch.cat([full[a:a + n] for a, n in ranges]).contiguous()
-        _rope_cache[key] = t
-    return t
+    key, last = (tuple(ranges), head_dim, theta, str(device)), max(a + n for a, n in ranges)
+    if key not in _rope_cache and torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+        full = rope_table(last, head_dim, theta, device)      # (a piece of the graph's own)
+        return torch.cat([full[a:a + n] for a, n in ranges])
+
+    def make():
+        full = _host_table(last, head_dim, theta)
+        return torch.cat([full[a:a + n] for a, n in ranges])
+
+    return _kept_table(key, make, device)
 
 
 def rope_(qkv: torch.Tensor, seq: int, nheads: int, theta: float = 500000.0, offset: int = 0,

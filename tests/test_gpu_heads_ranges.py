@@ -57,3 +57,33 @@ def test_ranges_are_the_positions_that_they_list(ranges, where, hd, dtype):
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(held, want))
     assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("where", ["another stream", "graph"])
+def test_tables_of_ranges_first_met_elsewhere(where):
+    theta, ranges = (811.0, ((4, 30), (500, 40))) if where == "graph" else (812.0, ((4, 30), (500, 40)))
+    x = torch.randn(140, 4, 64, device="cuda", dtype=torch.bfloat16)
+    rotary = ops.Rotary(theta=theta)
+    want = ops.rope(x, 70, 3, rotary=rotary, positions=listed(ranges))
+    if where == "graph":
+        ops.rope_(x.clone(), 70, 3, theta=theta, offset=470)      # (the table that holds these positions)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = ops.rope_(x.clone(), 70, 3, theta=theta, ranges=ranges)
+        got = ops.rope_(x.clone(), 70, 3, theta=theta, ranges=ranges)
+        graph.replay()
+        assert torch.equal(held, got)
+    else:
+        side = torch.cuda.Stream()
+        busy = torch.randn(4096, 4096, device="cuda")
+        y = x.clone()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                busy = busy @ busy * 1e-3
+            ops.rope_(y, 70, 3, theta=theta, ranges=ranges)
+        got = ops.rope_(x.clone(), 70, 3, theta=theta, ranges=ranges)
+        torch.cuda.synchronize()
+    # one rounding to bf16 of either, and a table of fp32 (2^-24) against angles of 64 bits
+    assert ((got.float() - want.float()).abs() <= 2 * 2.0 ** -8 * want.float().abs() + 2.0 ** -16 * x.float().abs().max()).all()

@@ -52,6 +52,20 @@ def test_ranges_first_met_under_fake_tensors(ranges):
     assert torch.equal(ops.rope(x, 7, 3, rotary=r, ranges=ranges), ops.rope(x, 7, 3, rotary=r, positions=listed(ranges)))
 
 
+@pytest.mark.parametrize("place", [dict(), dict(offset=3), dict(ranges=((0, 3), (40, 4)))], ids=str)
+def test_tables_first_made_under_fake_tensors_or_in_inference_mode(place):
+    x = torch.randn(14, 4, 16)
+    for theta, mode in ((701.0, FakeTensorMode()), (702.0, torch.inference_mode())):
+        with mode:
+            ops.rope_(torch.randn(14, 4, 16), 7, 3, theta=theta, **place)
+        y = x.clone().requires_grad_()
+        out = ops.rope_(y * 1, 7, 3, theta=theta, **place)
+        out.sum().backward()
+        assert torch.allclose(out, ops.rope(x, 7, 3, rotary=ops.Rotary(theta=theta), **place), atol=1e-5)
+        with FakeTensorMode():
+            ops.rope_(torch.randn(14, 4, 16), 7, 3, theta=theta, **place)
+
+
 def test_ranges_that_are_refused():
     x, r = torch.randn(14, 4, 16), ops.Rotary()
     for ranges, tokens in ((((0, 6),), 14), (((0, 8), (3, -1)), 14), (((0, 7),), 13), ((), 14)):
