@@ -294,20 +294,25 @@ __device__ __forceinline__ int choose(const RouteArgs& a, unsigned (&key)[C], in
     }
   }
   if (near >= 0) {                                            // none may be close to the next, the first left out included
-    unsigned next = __shfl_down_sync(0xffffffffu, mine, 1);
-    unsigned out = __reduce_max_sync(0xffffffffu, key[0]);
-    if (lane == a.k - 1) next = out;
+    const unsigned next = __shfl_down_sync(0xffffffffu, mine, 1);
+    unsigned out = __reduce_max_sync(0xffffffffu, key[0]), last = __shfl_sync(0xffffffffu, mine, a.k - 1);
+    // (two alike in logit and bias are alike, and in order)
+    auto same = [&](unsigned x, unsigned y) {
+      const int e = 511 - (int)(x & 511u), f = 511 - (int)(y & 511u);
+      return to_f(from[f]) == to_f(from[e]) && (a.bias == nullptr || a.bias[f] == a.bias[e]);
+    };
     bool alike = true;
-    if (lane < a.k && next != 0u && (int)(mine >> 9) - (int)(next >> 9) <= near) {
-      const int e = 511 - (int)(mine & 511u), f = 511 - (int)(next & 511u);
-      // (two alike in logit and bias are alike, and in order)
-      alike = to_f(from[f]) == to_f(from[e]) && (a.bias == nullptr || a.bias[f] == a.bias[e]);
+    if (lane < a.k - 1 && next != 0u && (int)(mine >> 9) - (int)(next >> 9) <= near) alike = same(mine, next);
+    // of those left out all that are close, not the next one alone: behind some that are alike there may be others
+    if (out != 0u && (int)(last >> 9) - (int)(out >> 9) <= near) {
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+        if (key[j] != 0u && (int)(last >> 9) - (int)(key[j] >> 9) <= near) alike = alike && same(last, key[j]);
     }
     if (__any_sync(0xffffffffu, !alike)) {
       if (!here || close) { close = true; return -1; }
       // all that may be among the k best: up to the first that is not close to the one before it
       int n = a.k;
-      unsigned last = __shfl_sync(0xffffffffu, mine, a.k - 1);
       while (out != 0u && (int)(last >> 9) - (int)(out >> 9) <= near) {
         if (n == 32) { close = true; return -1; }
         if (lane == n) mine = out;
