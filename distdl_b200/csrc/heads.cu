@@ -51,17 +51,20 @@ struct HeadArgs {
   long long out_row, out_head;
   const void* wq;             // [hd] or null (ones)
   const void* wk;
-  const void* positions;      // [seq] of 4 or 8 bytes, of token % seq, or null: offset + token % seq, and `jump` more from the
-                              // place `split` on (a sequence of two ranges of positions)
+  const void* positions;      // [seq] of 4 or 8 bytes, of token % seq, or null: offset + token % seq, from the place
+                              // `split` on offset_behind + token % seq (a sequence of two ranges of positions)
   float* partial;             // backward: [gridDim.x][2][hd], or null
-  long long offset, jump;
-  unsigned tokens, seq, split;
+  long long offset;
+  unsigned tokens, seq;
   int heads[3];               // query, key and other heads (those are copied; none in place)
   int chunk[3], chunks[3];    // heads per unit (whole rounds of a warp's groups), units per token
   int hd, rd, group;          // group: lanes per head (a power of two)
   int queries;                // forward: of the heads of the first kind, those that take wq
   int wide_positions, wide_weights, neighbours;
   float magnitude, sign, eps, inv_hd;
+  unsigned split;             // (behind the others: between them kCrossed spills more in the backward pass:
+                              // 16384 tokens, 48 heads, 50 of 128 turned, forward and backward 271 -> 284 us)
+  long long offset_behind;
   double turns[kMaxPairs];    // frequency of each pair in turns per position
 };
 
@@ -275,7 +278,7 @@ struct Angles {
   __device__ __forceinline__ void set(const HeadArgs& a, const double* turns, const L& lane, int g, unsigned token) {
     long long pos;
     const unsigned at = token % a.seq;
-    if (a.positions == nullptr) pos = a.offset + at + (at >= a.split ? a.jump : 0);
+    if (a.positions == nullptr) pos = (at < a.split ? a.offset : a.offset_behind) + at;
     else if (a.wide_positions) pos = reinterpret_cast<const long long*>(a.positions)[at];
     else pos = reinterpret_cast<const int*>(a.positions)[at];
     const double place = (double)pos;
@@ -869,7 +872,7 @@ DD_API int dd_heads(const void* packed, int bytes, void* stream) {
   a.queries = c.hq;
   a.hd = c.hd; a.rd = c.rd; a.neighbours = c.neighbours;
   a.positions = c.positions; a.wide_positions = c.wide_positions; a.offset = c.offset;
-  a.split = second.split > 0x7fffffffLL ? 0x7fffffffu : (unsigned)second.split; a.jump = second.jump;
+  a.split = second.split > 0x7fffffffLL ? 0x7fffffffu : (unsigned)second.split; a.offset_behind = c.offset + second.jump;
   a.magnitude = c.magnitude;
   a.inv_hd = 1.f / (float)c.hd;
   a.sign = back ? -1.f : c.pass == kRotate ? c.sign : 1.f;
