@@ -158,11 +158,38 @@ __global__ void moe_pair_dot_kernel(const __nv_bfloat16* __restrict__ a, const _
 // Outputs per pair (t, c): ids, w; hist[chunk][e] for moe_slot_kernel, which follows and
 // turns the histograms into slots (arrival order at the expert = pair index order, -1 beyond
 // the capacity).  prob_sum[e] ends as sum_t p[t, e] and must be zero on entry.
+// The choice is by the logits themselves, the lower expert first where they are equal.  An expert of -inf is never chosen: the
+// places of a token that has none left get -1 and weight 0, and a token of -inf alone adds nothing.  A NaN or +inf makes the
+// token's weights, its p and its gradient NaN, and counts as the best.
 // A latency, not a bandwidth: a few KB per CTA.  The probabilities of a warp's tokens are added by shuffles and
 // the warps' sums in order: adding them one by one with shared-memory atomics (a compare-and-swap loop of all
 // tokens on the same E words) took most of the time; 64 tokens, 8 experts: 34 -> 3.4 us, 4096 tokens:
 // 58 -> 3.8 us.
 // ---------------------------------------------------------------------------
+// A token's logits, -inf where there is no expert and +inf for a NaN, and the largest of them.
+template <int EMAX>
+__device__ __forceinline__ float router_logits(const __nv_bfloat16* __restrict__ logits, int E, float (&l)[EMAX]) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < EMAX; ++e) {
+    const float v = e < E ? __bfloat162float(logits[e]) : -INFINITY;
+    l[e] = v == v ? v : INFINITY;
+    m = fmaxf(m, l[e]);
+  }
+  return m;
+}
+// The probabilities in their place: 0 where there is no expert at all, NaN where a logit is no number.
+template <int EMAX>
+__device__ __forceinline__ void router_probs(float m, float (&p)[EMAX]) {
+  const float shift = m == -INFINITY ? 0.f : m;
+  float z = 0.f;
+#pragma unroll
+  for (int e = 0; e < EMAX; ++e) { p[e] = __expf(p[e] - shift); z += p[e]; }
+  const float inv = m == -INFINITY ? 0.f : m == INFINITY ? __int_as_float(0x7fffffff) : 1.f / z;
+#pragma unroll
+  for (int e = 0; e < EMAX; ++e) p[e] *= inv;
+}
+
 template <int EMAX>
 __global__ void __launch_bounds__(256)
 moe_router_fwd_kernel(const __nv_bfloat16* __restrict__ logits, int ld, int tokens, int E, int k, int capacity,
@@ -175,38 +202,29 @@ moe_router_fwd_kernel(const __nv_bfloat16* __restrict__ logits, int ld, int toke
   const int t = blockIdx.x * blockDim.x + threadIdx.x;
   float p[EMAX];
   if (t < tokens) {
-    float m = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < EMAX; ++e) {
-      p[e] = e < E ? __bfloat162float(logits[(size_t)t * ld + e]) : -INFINITY;
-      m = fmaxf(m, p[e]);
-    }
-    float z = 0.f;
-#pragma unroll
-    for (int e = 0; e < EMAX; ++e) { p[e] = e < E ? __expf(p[e] - m) : 0.f; z += p[e]; }
-    const float inv = 1.f / z;
-#pragma unroll
-    for (int e = 0; e < EMAX; ++e) p[e] *= inv;
+    const float m = router_logits<EMAX>(logits + (size_t)t * ld, E, p);
     unsigned long long taken = 0ull;
     float wsel[8];
     int isel[8];
     float zs = 0.f;
     for (int c = 0; c < k; ++c) {
-      float best = -1.f;
-      int bi = 0;
+      float best = -INFINITY;
+      int bi = -1;
 #pragma unroll
       for (int e = 0; e < EMAX; ++e)
-        if (e < E && !((taken >> e) & 1ull) && p[e] > best) { best = p[e]; bi = e; }
-      taken |= 1ull << bi;
-      wsel[c] = best; isel[c] = bi; zs += best;
+        if (!((taken >> e) & 1ull) && p[e] > best) { best = p[e]; bi = e; }
+      if (bi >= 0) taken |= 1ull << bi;
+      wsel[c] = bi >= 0 ? __expf(best - m) : 0.f;             // (+inf: NaN)
+      isel[c] = bi; zs += wsel[c];
     }
     const float invs = 1.f / zs;
     for (int c = 0; c < k; ++c) {
       const int pr = t * k + c;
       ids[pr] = isel[c];
-      w[pr] = wsel[c] * invs;
-      atomicAdd(&s_hist[isel[c]], 1);
+      w[pr] = isel[c] < 0 ? 0.f : wsel[c] * invs;
+      if (isel[c] >= 0) atomicAdd(&s_hist[isel[c]], 1);
     }
+    router_probs<EMAX>(m, p);
   } else {
 #pragma unroll
     for (int e = 0; e < EMAX; ++e) p[e] = 0.f;
@@ -236,30 +254,22 @@ moe_router_bwd_kernel(const __nv_bfloat16* __restrict__ logits, int ld, int toke
   const int t = blockIdx.x * blockDim.x + threadIdx.x;
   if (t >= tokens) return;
   float p[EMAX];
-  float m = -INFINITY;
-#pragma unroll
-  for (int e = 0; e < EMAX; ++e) {
-    p[e] = e < E ? __bfloat162float(logits[(size_t)t * ld + e]) : -INFINITY;
-    m = fmaxf(m, p[e]);
-  }
-  float z = 0.f;
-#pragma unroll
-  for (int e = 0; e < EMAX; ++e) { p[e] = e < E ? __expf(p[e] - m) : 0.f; z += p[e]; }
-  const float inv = 1.f / z;
+  const float m = router_logits<EMAX>(logits + (size_t)t * ld, E, p);
+  router_probs<EMAX>(m, p);
   float cp = 0.f;
 #pragma unroll
-  for (int e = 0; e < EMAX; ++e) {
-    p[e] *= inv;
+  for (int e = 0; e < EMAX; ++e)
     if (e < E && coef != nullptr) cp += coef[e] * p[e];
-  }
   float g[EMAX];
 #pragma unroll
   for (int e = 0; e < EMAX; ++e) g[e] = (e < E && coef != nullptr) ? p[e] * (coef[e] - cp) : 0.f;
   if (dw != nullptr) {
     float wd = 0.f;
-    for (int c = 0; c < k; ++c) wd += w[t * k + c] * dw[t * k + c];
+    for (int c = 0; c < k; ++c)
+      if (ids[t * k + c] >= 0) wd += w[t * k + c] * dw[t * k + c];
     for (int c = 0; c < k; ++c) {
       const int i = ids[t * k + c];
+      if (i < 0) continue;
       const float add = w[t * k + c] * (dw[t * k + c] - wd);
 #pragma unroll
       for (int e = 0; e < EMAX; ++e)
@@ -271,6 +281,7 @@ moe_router_bwd_kernel(const __nv_bfloat16* __restrict__ logits, int ld, int toke
 #pragma unroll
     for (int q = 0; q < EMAX; ++q)
       if (q == e) v = g[q];
+    if (m == INFINITY && e < E) v = __int_as_float(0x7fffffff);
     dlogits[(size_t)t * ld + e] = __float2bfloat16(v);
   }
 }

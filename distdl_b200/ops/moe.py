@@ -215,13 +215,12 @@ def route(logits: torch.Tensor, num_experts: int, k: int, capacity: int, *, scor
 
     Equal scores go to the lowest expert, and scores are told apart as exact arithmetic would.  An expert with a logit or a
     bias of -inf is never chosen; where fewer than ``k`` are left the places have id -1, slot -1 and weight 0, and a row of -inf (a
-    padding token) routes nowhere and adds nothing to ``prob_sum``.  A NaN makes the token's weights NaN.  (With all settings
-    at their defaults and up to 64 experts every logit is a finite number, and scores are told apart in fp32.)  bf16, fp16 and
+    padding token) routes nowhere and adds nothing to ``prob_sum``.  A NaN makes the token's weights NaN.  bf16, fp16 and
     fp32 logits of up to 512 experts, with 32 choices and 32 groups at most, run on the kernels."""
     E = num_experts
-    if score == "softmax" and bias is None and groups == 1 and renormalize and scale == 1.0 \
-            and (E <= 64 or not use_native(logits)):
-        return _route_plain_softmax(logits, E, k, capacity)
+    if score == "softmax" and bias is None and groups == 1 and renormalize and scale == 1.0 and use_native(logits) \
+            and logits.dtype == torch.bfloat16 and E <= 64 and k <= 8 and logits.is_contiguous() and logits.numel():
+        return _RouterFn.apply(logits, E, k, capacity)        # (a thread per token, csrc/moe.cu)
     how = _route_check(logits, E, k, score, bias, groups, top_groups, group_score, renormalize, scale)
     if use_native(logits) and logits.dtype in _DTYPE and E <= _MOST_EXPERTS and k <= _MOST_CHOICES \
             and groups <= _MOST_GROUPS and logits.numel() and logits.shape[0] * k < 2 ** 31 and ordinary(logits):
@@ -285,18 +284,6 @@ def _slots_in_order(flat, E, capacity):
     rank[order] = torch.arange(key.numel(), device=key.device) - (counts.cumsum(0) - counts)[key[order]]
     slot = torch.where(here & (rank < capacity), rank, torch.full_like(rank, -1))
     return slot.to(torch.int32), counts[:E].to(torch.int32)
-
-
-def _route_plain_softmax(logits, E, k, capacity):
-    """Softmax, top-k, renormalised: up to 64 bf16 experts on the kernels of ``csrc/moe.cu``."""
-    if use_native(logits) and logits.dtype == torch.bfloat16 and E <= 64 and k <= 8 and logits.is_contiguous():
-        return _RouterFn.apply(logits, E, k, capacity)
-    probs = torch.softmax(logits[:, :E].float(), dim=-1)
-    topw, topi = probs.topk(k, dim=-1)
-    topw = topw / topw.sum(-1, keepdim=True)
-    ids = topi.to(torch.int32).reshape(-1).contiguous()
-    slot, counts = assign_slots(ids, E, capacity)
-    return topw, probs.sum(0), ids, slot, counts
 
 
 def assign_slots(ids: torch.Tensor, num_experts: int, capacity: int):
