@@ -236,10 +236,10 @@ __device__ __noinline__ int order_in_64_bits(const RouteArgs& a, unsigned mine, 
 
 // The choice of one token from the keys of its experts: lane i gets the i-th expert, -1 where there is none.  `close` is set
 // where values within `near` of one another (near < 0: all values are exact) decide, are not those of experts alike in logit
-// and bias, and are not decided here (`here`: where they can be).
+// and bias, and are not decided here (`here`: where they can be).  Values up to `floor` may stand for any below them.
 template <typename T, int C>
-__device__ __forceinline__ int choose(const RouteArgs& a, unsigned (&key)[C], int first, int left, int near, bool here, bool& close,
-                                      int* values, const T* from) {
+__device__ __forceinline__ int choose(const RouteArgs& a, unsigned (&key)[C], int first, int left, int near, int floor, bool here,
+                                      bool& close, int* values, const T* from) {
   const int lane = threadIdx.x & 31;
   if (a.groups > 1) {
     int b0, b1, step;
@@ -263,9 +263,10 @@ __device__ __forceinline__ int choose(const RouteArgs& a, unsigned (&key)[C], in
     }
     if (near >= 0) {
       const int least = (int)(worst >> 5), most = (int)(__reduce_max_sync(0xffffffffu, group) >> 5);
-      // (of a group with one expert only its value itself would have to be known)
+      // (of a group with one expert only its value itself would have to be known, and of a sum that is among the best
+      // both values: one that may be any below counts for too much)
       close = (most > 0 && least - most <= (a.group_sum ? 2 * near : near)) ||
-              __any_sync(0xffffffffu, g < a.groups && a.group_sum && a.size > 1 && b0 > 0 && b1 == 0);
+              __any_sync(0xffffffffu, g < a.groups && a.group_sum && a.size > 1 && b0 > 0 && b1 <= (in ? floor : 0));
       if (close && here && a.lanes > 0) {
         unsigned sorted[C];
 #pragma unroll
@@ -489,7 +490,7 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
     Scores<C> s;
     s.set(l, a.sigmoid, top_l);
     unsigned key[C];
-    int near = -1;                                            // differences of values up to here say nothing
+    int near = -1, floor = 0;                                 // differences, and values, up to here say nothing
     if (exact) {
 #pragma unroll
       for (int j = 0; j < C; ++j) key[j] = l[j] > -INFINITY ? (ordered(l[j]) & ~511u) | (511 - first - j) : 0u;
@@ -505,7 +506,9 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
       }
       hi = top_of_warp(hi);
       // (values far below the largest, -inf among them, are not told apart: should they decide, they are close)
-      lo = fmaxf(low_of_warp(lo), hi - (a.by_logit ? 64.f : 8.f));
+      const float low = low_of_warp(lo);
+      lo = fmaxf(low, hi - (a.by_logit ? 64.f : 8.f));
+      floor = low < lo;
       const float range = hi - lo, steps = range > 1e-25f ? __fdividef(kSteps, range) : 0.f;
       // scores: sigmoid 4e-7 off at most (its slope times the exponential's error, a division), softmax 4e-6 of the largest,
       // the bias's addition; the cut itself: a step each way
@@ -522,7 +525,7 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
         if ((bad >> j) & 1u) key[j] = kBad | (511 - first - j);
     }
     bool close = false;
-    int chosen = choose<T, C>(a, key, first, left, near, !nan && (a.by_logit || a.sigmoid), close,
+    int chosen = choose<T, C>(a, key, first, left, near, floor, !nan && (a.by_logit || a.sigmoid), close,
                               reinterpret_cast<int*>(s_row[warp]), from);
     if (close) {                                              // (the same on every lane)
       float again[C];

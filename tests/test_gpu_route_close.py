@@ -48,3 +48,22 @@ def test_biases_a_step_apart_on_few_values():
         for score in ("softmax", "sigmoid"):
             check(logits, E, 6, 30, grads=False, score=score, bias=bias)
             check(logits, E, 6, 30, grads=False, score=score, bias=bias, groups=8, top_groups=3, group_score="top2")
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups", [(64, 8), (256, 8), (60, 6), (512, 4), (16, 8)])
+def test_group_sums_of_experts_far_below_the_best(E, groups, score):
+    """Of a group's two best the second may lie far below all others, and still decides."""
+    g = torch.Generator().manual_seed(E)
+    size = E // groups
+    logits = torch.randn(50, E, generator=g)
+    bias = -200.0 - 100.0 * torch.rand(E, generator=g)
+    place = torch.randperm(groups, generator=g)
+    for i, (best, second) in enumerate([(0.5, -100.0), (-0.5, -50.0), (0.25, -75.0), (-9.0, -12.0)]):
+        bias[place[i] * size + torch.randperm(size, generator=g)[:2]] = torch.tensor([best, second])
+    how = dict(score=score, groups=groups, group_score="top2", bias=bias.cuda())
+    for top_groups in (1, 2, 3):
+        check(logits.cuda(), E, 2, 50, grads=False, top_groups=top_groups, **how)
+    masked = logits.clone()
+    masked[torch.rand(50, E, generator=g) < 0.3] = -float("inf")
+    check(masked.cuda(), E, 2, 50, grads=False, top_groups=2, **how)
