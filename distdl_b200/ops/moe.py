@@ -175,19 +175,18 @@ def _choose(logits, E, k, how):
     """The experts ``[tokens, k]`` of :func:`route` (-1: none left), in 64 bits."""
     score, bias, groups, top_groups, group_score, _renormalize, _scale = how
     l = logits[:, :E].detach().double()
-    c = _scores(l.masked_fill(torch.isnan(l), -math.inf), E, score)[0]
+    best = torch.isnan(l) if score == "sigmoid" else torch.isnan(l) | (l == math.inf)     # no numbers: the best
+    c = _scores(l.masked_fill(best, -math.inf), E, score)[0]
     if bias is not None:
         c = c + bias.double()
     elif groups == 1 or group_score == "max":
         c = l                                               # the same order, also where scores are no longer told apart
-    c = c.masked_fill((l == -math.inf) | torch.isnan(c), -math.inf).masked_fill(torch.isnan(l), math.inf)
-    if score == "softmax":
-        c = c.masked_fill(l == math.inf, math.inf)
+    c = c.masked_fill((l == -math.inf) | torch.isnan(c), -math.inf).masked_fill(best, math.inf)
     if top_groups < groups:
-        best = c.reshape(len(c), groups, E // groups).sort(dim=-1, descending=True).values
-        value = best[..., 0]
+        by = c.reshape(len(c), groups, E // groups).sort(dim=-1, descending=True).values
+        value = by[..., 0]
         if group_score == "top2" and E > groups:
-            value = torch.where(best[..., 1] > -math.inf, value + best[..., 1], value)
+            value = torch.where(by[..., 1] > -math.inf, value + by[..., 1], value)
         kept = value.sort(dim=-1, descending=True, stable=True).indices[:, :top_groups]
         live = torch.zeros_like(value, dtype=torch.bool).scatter(1, kept, True)
         c = c.masked_fill(~live.repeat_interleave(E // groups, dim=1), -math.inf)

@@ -55,3 +55,14 @@ def test_ties_and_near_ties(E):
 def test_no_tokens(E):
     w, prob, ids, slot, counts = moe.route(torch.zeros(0, E), E, 3, 9)
     assert w.shape == (0, 3) and ids.numel() == slot.numel() == 0 and (prob == 0).all() and (counts == 0).all()
+
+
+@pytest.mark.parametrize("how", [dict(bias=torch.zeros(8)), dict(bias=torch.zeros(8), groups=2, top_groups=1, group_score="top2"),
+                                 dict(groups=4, top_groups=2, group_score="top2"), dict(scale=1.5)], ids=lambda h: str(len(h)))
+def test_softmax_of_infinity_still_chooses_k_experts(how):
+    logits = torch.tensor([[0.0, 3.0, 1.0, math.inf, 2.0, -1.0, 5.0, 4.0], [0.0, 3.0, 1.0, 2.5, 2.0, -1.0, math.inf, math.inf]])
+    w, _, ids, slot, counts = moe.route(logits, 8, 3, 9, **how)
+    ids = ids.reshape(2, 3)
+    # (half of the experts: the ones beside the infinite)
+    assert ids.tolist() == ([[3, 1, 2], [6, 7, 4]] if how.get("groups") == 2 else [[3, 6, 7], [6, 7, 1]])
+    assert torch.isnan(w).all() and counts.sum() == 6 and (slot >= 0).all()
