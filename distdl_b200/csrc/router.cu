@@ -31,6 +31,7 @@
 
 #include <cuda_fp16.h>
 
+#include <cfloat>
 #include <cstring>
 
 using namespace dd;
@@ -364,6 +365,7 @@ __device__ __noinline__ int choose_in_64_bits(const RouteArgs& a, const float* l
     if (!a.by_logit && !a.sigmoid) c[j] /= z;
     if (a.bias != nullptr && j < left) c[j] += (double)a.bias[first + j];
     if (!(l_in[j] > -INFINITY) || c[j] != c[j]) c[j] = (bad >> j) & 1u ? INFINITY : -INFINITY;
+    else c[j] = fmin(c[j], DBL_MAX);                          // (+inf from a sigmoid or a bias: below what is no number)
   }
   if (a.groups > 1) {
     double b0 = -INFINITY, b1 = -INFINITY;
@@ -527,6 +529,7 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
     bool close = false;
     int chosen = choose<T, C>(a, key, first, left, near, floor, !nan && (a.by_logit || a.sigmoid), close,
                               reinterpret_cast<int*>(s_row[warp]), from);
+    close = close || (nan && a.groups > 1 && a.group_sum);    // (what is no number is the best, whatever is added to it)
     if (close) {                                              // (the same on every lane)
       float again[C];
 #pragma unroll

@@ -181,6 +181,7 @@ def _choose(logits, E, k, how):
         c = c + bias.double()
     elif groups == 1 or group_score == "max":
         c = l                                               # the same order, also where scores are no longer told apart
+    c = c.clamp(max=torch.finfo(torch.float64).max)         # (+inf of a sigmoid or a bias: below what is no number)
     c = c.masked_fill((l == -math.inf) | torch.isnan(c), -math.inf).masked_fill(best, math.inf)
     if top_groups < groups:
         by = c.reshape(len(c), groups, E // groups).sort(dim=-1, descending=True).values

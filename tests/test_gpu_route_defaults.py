@@ -80,3 +80,24 @@ def test_no_tokens():
     for dtype in (BF16, FP32):
         w, prob, ids, slot, counts = moe.route(torch.zeros(0, 8, device="cuda", dtype=dtype), 8, 3, 9)
         assert w.shape == (0, 3) and ids.numel() == slot.numel() == 0 and (prob == 0).all() and (counts == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups", [(24, 1), (64, 8), (256, 8), (60, 6), (512, 16), (10, 5)])
+def test_the_kernels_choose_as_the_path_without_them(E, groups, score, dtype):
+    """Tokens with several logits that are no numbers, and with infinities."""
+    g = torch.Generator().manual_seed(E)
+    logits = torch.randn(200, E, generator=g).to(dtype)
+    for value in (math.nan, math.inf, -math.inf):
+        logits[torch.rand(200, E, generator=g) < 1.5 / E] = value
+    bias = torch.randn(E, generator=g) * 0.1
+    for by in ("max", "top2"):
+        for b in (None, bias):
+            how = dict(score=score, groups=groups, top_groups=(groups + 1) // 2, group_score=by)
+            got = moe.route(logits.cuda(), E, 4, 20, bias=None if b is None else b.cuda(), **how)
+            want = moe.route(logits, E, 4, 20, bias=b, **how)
+            for x, y in zip(got[2:], want[2:]):
+                assert torch.equal(x.cpu(), y)
+            assert torch.equal(torch.isnan(got[0]).cpu(), torch.isnan(want[0]))
+            assert torch.allclose(got[0].cpu(), want[0], rtol=1e-5, atol=1e-30, equal_nan=True)
