@@ -111,6 +111,8 @@ class _RouteFn(torch.autograd.Function):
     def backward(ctx, dw, dprob, _dids, _dslot, _dcounts):
         logits, ids, w = ctx.saved_tensors
         E, k, how = ctx.cfg
+        if dw is None and dprob is None:
+            return None, None, None, None, None
         if torch.is_grad_enabled() or not all([g is None or ordinary_gradient(g) for g in (dw, dprob)]):
             # differentiated itself, or under a function transform: elementary operations, with the experts as they are
             with torch.enable_grad():
@@ -118,8 +120,6 @@ class _RouteFn(torch.autograd.Function):
                 outs, grads = zip(*[(o, g) for o, g in zip(outs, (dw, dprob)) if g is not None])
                 (d,) = torch.autograd.grad(outs, logits, grads, create_graph=True)
             return d, None, None, None, None
-        if dw is None and dprob is None:
-            return None, None, None, None, None
         if dw is not None and (dw.dtype != torch.float32 or not dw.is_contiguous()):
             dw = dw.float().contiguous()
         if dprob is not None and (dprob.dtype != torch.float32 or not dprob.is_contiguous()):
