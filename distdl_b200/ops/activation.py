@@ -145,7 +145,8 @@ def rope_(qkv: torch.Tensor, seq: int, nheads: int, theta: float = 500000.0, off
 
     ``rotary`` (an :class:`~distdl_b200.ops.Rotary`, in the place of ``theta``): other pairings, a part of the head, long
     contexts.  ``positions`` (int64 or int32, on the device of ``qkv``): a position per token, or per place in a sequence.
-    With either of them bf16, fp16 and fp32 heads are turned in place, at any strides with unit stride inside a head;
+    With either of them ``qkv`` itself is turned and returned, on every device: bf16, fp16 and fp32 heads on CUDA by the
+    kernels, at any strides with unit stride inside a head.  It must not be a leaf that requires a gradient;
     :func:`~distdl_b200.ops.rope` leaves its input alone."""
     if rotary is not None or positions is not None:
         from .rotary import Rotary, rope_in_place

@@ -382,14 +382,15 @@ def rope_in_place(qkv, seq, nheads, rotary, offset=0, ranges=None, positions=Non
     _check_heads(read, nheads)
     where = _where(read, rotary, seq, offset, ranges, positions)
     rotary._plan(shape[2])
-    if not _native_ok(read):
-        return _plain_rope(qkv.reshape(shape), nheads, where).reshape(qkv.shape)
-    if not held or _overlaps(read) or (read.stride(2) != 1 and shape[2] > 1):
-        raise ValueError("a tensor that is turned in place must have its heads' components next to one another in memory "
-                         "of their own: use ops.rope")
+    native = _native_ok(read)
+    if not held or _overlaps(read) or (native and read.stride(2) != 1 and shape[2] > 1):
+        raise ValueError("a tensor that is turned in place must have its heads in memory of their own (for the kernels, their "
+                         "components next to one another): use ops.rope")
+    if qkv.requires_grad and torch.is_grad_enabled() and qkv.is_leaf:
+        raise RuntimeError("a leaf that requires a gradient cannot be turned in place: use ops.rope, or torch.no_grad()")
+    if not native:
+        return qkv.copy_(_plain_rope(qkv.reshape(shape), nheads, where).reshape(qkv.shape))
     if qkv.requires_grad and torch.is_grad_enabled():
-        if qkv.is_leaf:
-            raise RuntimeError("a leaf that requires a gradient cannot be turned in place: use ops.rope, or torch.no_grad()")
         return _RopeInPlaceFn.apply(qkv, (shape, nheads, where))
     _call(_ROTATE, read, read, nheads, 0, where)
     torch.autograd.graph.increment_version(qkv)               # (passes over tensors of inference mode)
