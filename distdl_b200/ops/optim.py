@@ -69,6 +69,7 @@ def accumulate_f32_(acc: torch.Tensor, g: torch.Tensor, scale: float = 1.0) -> N
         acc.add_(g.reshape(-1).to(acc.dtype), alpha=scale)
 
 
+_Parameter = torch.nn.Parameter
 _CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -111,6 +112,13 @@ def _flat(tensors):
     return [t for t in tensors if t is not None]
 
 
+def gradients_of(tensors):
+    """The gradients meant by ``tensors`` (one, or an iterable): of a parameter, trained or frozen, its ``.grad``, of which there
+    may be none; anything else as it is."""
+    return _flat([t.grad if (t.requires_grad and t.is_leaf) or (type(t) is not torch.Tensor and isinstance(t, _Parameter)) else t
+                  for t in _flat(tensors)])
+
+
 def _plain_sumsq(tensors):
     return torch.stack([t.detach().double().square().sum() for t in tensors]).sum()
 
@@ -147,12 +155,12 @@ def grad_norm(tensors, squared: bool = False) -> torch.Tensor:
 
 def clip_grad_norm_(tensors, max_norm: float, norm: torch.Tensor = None) -> torch.Tensor:
     """Scales gradients in place by ``min(1, max_norm / (norm + 1e-6))``, ``norm`` being their 2-norm, which is returned (an
-    fp32 scalar on their device; nothing waits for it).  ``tensors``: gradients, or parameters (whose ``.grad`` is meant:
-    leaves that require a gradient), None passed over.  ``norm`` given (an fp32 scalar on their device, say of the gradients
-    of all workers): that norm is taken.  Where the norm is not above ``max_norm`` nothing is written; one that is not a
-    number makes all gradients so.  The tensors must not share memory with one another."""
-    tensors = [t.grad if t.requires_grad and t.is_leaf else t for t in _flat(tensors)]
-    tensors = _flat(tensors)
+    fp32 scalar on their device; nothing waits for it).  ``tensors``: gradients, or parameters (and other leaves that require
+    a gradient), whose ``.grad`` is meant, also where they are frozen; None is passed over.  ``norm`` given (an fp32 scalar
+    on their device, say of the gradients of all workers): that norm is taken.  Where the norm is not above ``max_norm``
+    nothing is written; one that is not a number makes all gradients so.  The tensors must not share memory with one
+    another."""
+    tensors = gradients_of(tensors)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, and a number: {max_norm}")

@@ -6,17 +6,16 @@ import torch
 import torch.distributed as dist
 
 from .. import ops
+from ..ops.optim import gradients_of
 
 
 @torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
-    """Scales the gradients of ``parameters`` (this worker's; gradients themselves are taken too) in place so that the norm
-    of the gradients of ALL workers together is at most ``max_norm``, and returns that norm (an fp32 scalar on the
-    gradients' device).  Every element of a distributed layer's parameters lives on exactly one worker, so that the
-    workers' sums of squares add up.  Collective over all processes; a worker without gradients takes part."""
-    grads = [t.grad if t.requires_grad and t.is_leaf else t
-             for t in ([parameters] if isinstance(parameters, torch.Tensor) else parameters)]
-    grads = [g for g in grads if g is not None]
+    """Scales the gradients of ``parameters`` (this worker's; gradients themselves are taken too, None is passed over) in
+    place so that the norm of the gradients of ALL workers together is at most ``max_norm``, and returns that norm (an fp32
+    scalar on the gradients' device).  Every element of a distributed layer's parameters lives on exactly one worker, so that
+    the workers' sums of squares add up.  Collective over all processes; a worker without gradients takes part."""
+    grads = gradients_of(parameters)
     if not dist.is_initialized() or dist.get_world_size() == 1:
         return ops.clip_grad_norm_(grads, max_norm)
     total = ops.grad_norm(grads, squared=True)
