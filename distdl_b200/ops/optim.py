@@ -70,6 +70,7 @@ def accumulate_f32_(acc: torch.Tensor, g: torch.Tensor, scale: float = 1.0) -> N
 
 
 _Parameter = torch.nn.Parameter
+_TYPES = {torch.Tensor, _Parameter}             # (others may hold their elements elsewhere)
 _CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -100,7 +101,8 @@ def _tensors(tensors):
             if not t.is_floating_point():
                 raise ValueError(f"gradients are floating-point tensors, not {t.dtype}")
         return None
-    if not use_native(tensors[0]) or not ordinary(tensors[0]) or not all([t.is_contiguous() or _dense(t) for t in tensors]):
+    if not use_native(tensors[0]) or not ordinary(tensors[0]) or not _TYPES.issuperset([type(t) for t in tensors]) \
+            or not all([t.is_contiguous() or _dense(t) for t in tensors]):
         return None
     return (array.array("Q", [t.data_ptr() for t in tensors]), array.array("q", [t.numel() for t in tensors]),
             array.array("B", codes))

@@ -26,3 +26,37 @@ def test_frozen_parameters_are_no_gradients(clip, device):
     # gradients as they are
     g = torch.full((4,), 2.0, device=device)
     assert clip(g, 1.0).item() == 4.0 and torch.allclose(g, torch.full_like(g, 0.5))
+
+
+class _Elsewhere(torch.Tensor):
+    """A tensor whose elements are those of another one, doubled."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        if func is torch.ops.aten.copy_.default and isinstance(args[0], cls):
+            args[0].inner.copy_(args[1] / 2)
+            return args[0]
+        return func(*[a.inner * 2 if isinstance(a, cls) else a for a in args], **(kwargs or {}))
+
+
+@pytest.mark.parametrize("place", [0, 1, 2])
+def test_a_subclass_is_not_taken_by_its_address_wherever_it_stands(place, monkeypatch):
+    from distdl_b200.ops import optim
+    tensors = [torch.ones(3), torch.ones(2), torch.ones(4)]
+    inner = tensors[place].clone()
+    tensors[place] = _Elsewhere(inner)
+    n = inner.numel()
+    want = torch.tensor(9.0 - n + 4.0 * n).sqrt()
+    assert torch.allclose(ops.grad_norm(tensors), want)
+    assert torch.allclose(ops.clip_grad_norm_(tensors, 1.0), want) and torch.allclose(inner, torch.ones(n) / want)
+    monkeypatch.setattr(optim, "use_native", lambda t: True)
+    assert optim._tensors(tensors) is None
+    tensors[place] = inner
+    assert optim._tensors(tensors) is not None
