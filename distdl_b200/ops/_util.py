@@ -21,9 +21,13 @@ _batched = torch._C._functorch.is_legacy_batchedtensor
 _tensor_types = (torch.Tensor, torch.nn.Parameter)
 
 
-def ordinary(t: torch.Tensor) -> bool:
+def ordinary(t: torch.Tensor, *others) -> bool:
     """Whether a kernel may stand for elementary operations on ``t`` in a forward pass: a tensor itself, outside dispatch
-    modes, function transforms, forward-mode derivatives and tracing."""
+    modes, function transforms, forward-mode derivatives and tracing.  ``others``: further operands (or None), no subclasses
+    either."""
+    for o in others:
+        if o is not None and type(o) not in _tensor_types:
+            return False
     return type(t) in _tensor_types and not _modes() and not _transforms() and forward_ad._current_level < 0 \
         and not _tracing()
 

@@ -223,7 +223,7 @@ def route(logits: torch.Tensor, num_experts: int, k: int, capacity: int, *, scor
         return _RouterFn.apply(logits, E, k, capacity)        # (a thread per token, csrc/moe.cu)
     how = _route_check(logits, E, k, score, bias, groups, top_groups, group_score, renormalize, scale)
     if use_native(logits) and logits.dtype in _DTYPE and E <= _MOST_EXPERTS and k <= _MOST_CHOICES \
-            and groups <= _MOST_GROUPS and logits.numel() and logits.shape[0] * k < 2 ** 31 and ordinary(logits):
+            and groups <= _MOST_GROUPS and logits.numel() and logits.shape[0] * k < 2 ** 31 and ordinary(logits, how[1]):
         logits = logits if logits.is_contiguous() else logits.contiguous()
         capacity = min(int(capacity), 2 ** 31 - 1)
         if torch.is_grad_enabled() and logits.requires_grad:

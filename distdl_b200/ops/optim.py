@@ -86,7 +86,7 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _tensors(tensors):
+def _tensors(tensors, norm=None):
     """(addresses, sizes, type codes) of the tensors as C arrays, or None where the kernels do not take them (CUDA, bf16 /
     fp16 / fp32, dense)."""
     device = tensors[0].device
@@ -101,8 +101,8 @@ def _tensors(tensors):
             if not t.is_floating_point():
                 raise ValueError(f"gradients are floating-point tensors, not {t.dtype}")
         return None
-    if not use_native(tensors[0]) or not ordinary(tensors[0]) or not _TYPES.issuperset([type(t) for t in tensors]) \
-            or not all([t.is_contiguous() or _dense(t) for t in tensors]):
+    if not use_native(tensors[0]) or not ordinary(tensors[0], norm) \
+            or not _TYPES.issuperset([type(t) for t in tensors]) or not all([t.is_contiguous() or _dense(t) for t in tensors]):
         return None
     return (array.array("Q", [t.data_ptr() for t in tensors]), array.array("q", [t.numel() for t in tensors]),
             array.array("B", codes))
@@ -172,7 +172,7 @@ def clip_grad_norm_(tensors, max_norm: float, norm: torch.Tensor = None) -> torc
         return torch.zeros((), dtype=torch.float32) if norm is None else norm
     if norm is not None and norm.device != tensors[0].device:
         raise ValueError(f"the norm is on {norm.device}, the gradients on {tensors[0].device}")
-    lists = _tensors(tensors)
+    lists = _tensors(tensors, norm)
     if lists is None:
         with torch.no_grad():
             norm = _plain_sumsq(tensors).sqrt().float() if norm is None else norm

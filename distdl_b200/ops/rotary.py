@@ -238,8 +238,8 @@ def _plain_rope(qkv, nheads, where, sign=1.0):
     return torch.cat([y.to(qkv.dtype), qkv[:, nheads:]], dim=1)
 
 
-def _native_ok(qkv):
-    return use_native(qkv) and qkv.dtype in _DTYPE and 1 <= qkv.shape[2] <= 512 and ordinary(qkv)
+def _native_ok(qkv, *others):
+    return use_native(qkv) and qkv.dtype in _DTYPE and 1 <= qkv.shape[2] <= 512 and ordinary(qkv, *others)
 
 
 def _unit(t):
@@ -357,7 +357,7 @@ def rope(qkv: torch.Tensor, seq: int, nheads: int, *, rotary: Rotary, offset: in
         raise ValueError("rope needs a Rotary")
     where = _where(qkv, rotary, seq, offset, ranges, positions)
     rotary._plan(qkv.shape[2])
-    if not _native_ok(qkv):
+    if not _native_ok(qkv, where[1]):
         return _plain_rope(qkv, nheads, where)
     if qkv.requires_grad and torch.is_grad_enabled():
         return _RopeFn.apply(qkv, (nheads, where, 1.0))
@@ -382,7 +382,7 @@ def rope_in_place(qkv, seq, nheads, rotary, offset=0, ranges=None, positions=Non
     _check_heads(read, nheads)
     where = _where(read, rotary, seq, offset, ranges, positions)
     rotary._plan(shape[2])
-    native = _native_ok(read)
+    native = _native_ok(read, where[1])
     if not held or _overlaps(read) or (native and read.stride(2) != 1 and shape[2] > 1):
         raise ValueError("a tensor that is turned in place must have its heads in memory of their own (for the kernels, their "
                          "components next to one another): use ops.rope")
@@ -488,7 +488,7 @@ def _norm_args(qkv, hq, hkv, wq, wk, rotary, seq, offset, ranges, positions):
     where = _where(qkv, rotary, seq, offset, ranges, positions)
     if rotary is not None:
         rotary._plan(qkv.shape[2])
-    native = (_native_ok(qkv) and _weight_ok(wq, qkv) and _weight_ok(wk, qkv)
+    native = (_native_ok(qkv, where[1], wq, wk) and _weight_ok(wq, qkv) and _weight_ok(wk, qkv)
               and (wq is None or wk is None or wq.dtype == wk.dtype))
     # (a weight that is a row already stays the tensor that it is: its accumulator is an attribute of it)
     if wq is not None and (wq.dim() != 1 or not wq.is_contiguous()):

@@ -28,7 +28,7 @@ def test_ranges_are_the_positions_that_they_list(ranges):
 def test_ranges_first_met_in_inference_mode(ranges, monkeypatch):
     """What a gradient keeps of the positions is not what a call in inference mode has made (the launches themselves stubbed)."""
     ranges = tuple((a + 1000, n) for a, n in ranges)           # (met nowhere else)
-    monkeypatch.setattr(rotary_module, "_native_ok", lambda t: True)
+    monkeypatch.setattr(rotary_module, "_native_ok", lambda *t: True)
     monkeypatch.setattr(rotary_module, "_call", lambda *a, **k: None)
     monkeypatch.setattr(rotary_module, "_parts", lambda d: 1)
     r, x = ops.Rotary(), torch.randn(14, 4, 16)
