@@ -148,10 +148,14 @@ class MoEFeedForward(torch.nn.Module):
             full = full.to(p.device) if self.P_root.active else zero_volume_tensor(device=p.device, dtype=p.dtype)
             destination[prefix + name] = self.scatter_experts[name](full)
         if self.router_bias is not None:
-            # the first worker's, on all of them
-            mine = destination.get(prefix + "router_bias") if self.P_root.active else torch.zeros(self.cfg.n_experts)
-            destination[prefix + "router_bias"] = torch.as_tensor(
-                self.P_ep.allreduce_data(mine.detach().cpu().numpy())).to(self.router_bias.device)
+            # the first worker's, on all of them (with whether it has any: a checkpoint of a model without the biases lacks
+            # the key on every worker then, and is refused or passed over as any other missing key)
+            mine, row = destination.pop(prefix + "router_bias", None), np.zeros(self.cfg.n_experts + 1, dtype=np.float32)
+            if self.P_root.active and mine is not None:
+                row = np.append(mine.detach().float().cpu().numpy(), np.float32(1))
+            row = self.P_ep.allreduce_data(row)
+            if row[-1] > 0:
+                destination[prefix + "router_bias"] = torch.as_tensor(row[:-1]).to(self.router_bias.device)
         return destination
 
     def take_routed(self):
