@@ -435,7 +435,20 @@ __device__ __forceinline__ float top_logit(float (&l)[C], bool sigmoid, unsigned
   return top;
 }
 
-// Scores of a token, p = s / sum s (0 in rows without an expert), from the largest logit.
+// e^x for x <= 0, within 2^-21 however far below zero: x log2 e as a product and what its rounding leaves (Dekker's two-product by
+// fma, and the rest of the constant), the second by its first-order term.  (__expf forms the product alone, which is off by
+// |x| 2^-24; 16384 tokens of 256 experts 22.6 -> 23.6 us.)
+__device__ __forceinline__ float exp_of(float x) {
+  constexpr double kLog2e = 1.4426950408889634;
+  constexpr float kHigh = (float)kLog2e, kRest = (float)(kLog2e - (double)kHigh), kLn2 = 0.6931471805599453f;
+  x = fmaxf(x, -200.f);                                       // (0 from -104 on; -inf has no remainder)
+  const float t = x * kHigh, rest = fmaf(x, kRest, fmaf(x, kHigh, -t));
+  const float e = exp2f(t);
+  return fmaf(e, rest * kLn2, e);
+}
+
+// Scores of a token, p = s / sum s (0 in rows without an expert), from the largest logit.  Sigmoids take the fast exponential: a
+// score is off by 2^-22 + (1 - s) |l| 2^-23 of itself, so that only scores that count for nothing beside others lose bits.
 template <int C>
 struct Scores {
   float inv;                // p = part * inv
@@ -447,7 +460,7 @@ struct Scores {
     if (!sigmoid) {
       const float shift = none ? 0.f : top;
 #pragma unroll
-      for (int j = 0; j < C; ++j) part[j] = __expf(l[j] - shift);
+      for (int j = 0; j < C; ++j) part[j] = exp_of(l[j] - shift);
     } else if (top >= 0.f) {
 #pragma unroll
       for (int j = 0; j < C; ++j) part[j] = __fdividef(1.f, 1.f + __expf(-l[j]));   // (e^88: 0, as e^-88)
@@ -546,7 +559,7 @@ __global__ void __launch_bounds__(kWarps * 32, C <= 8 ? 3 : 2) route_kernel(cons
         const float shift = a.renormalize ? fminf(top, 0.f) : 0.f, e = __expf(-fabsf(lc));
         v = __fdividef(lc > 0.f ? 1.f : shift == 0.f ? e : __expf(lc - shift), 1.f + e);
       } else {
-        v = __expf(lc - top);
+        v = exp_of(lc - top);
       }
       if (chosen < 0) v = 0.f;
       if (a.renormalize) v = __fdividef(v, warp_sum(v));
