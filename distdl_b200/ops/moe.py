@@ -327,7 +327,7 @@ def _gather(src, ids, slot, w, tokens, k):
     rows = src[ids.long().clamp(min=0), slot.long().clamp(min=0)].reshape(tokens, k, d).float()
     if w is not None:
         rows = rows * w.reshape(tokens, k, 1)
-    return (rows * keep).sum(1).to(src.dtype)
+    return rows.masked_fill(~keep, 0.0).sum(1).to(src.dtype)
 
 
 def _pair_dot(a, b, ids, slot, k):
@@ -340,7 +340,7 @@ def _pair_dot(a, b, ids, slot, k):
         return out
     rows = b[ids.long().clamp(min=0), slot.long().clamp(min=0)].float()
     av = a[torch.arange(n, device=a.device) // k].float()
-    return (rows * av).sum(-1) * (slot >= 0)
+    return (rows * av).sum(-1).masked_fill(slot < 0, 0.0)
 
 
 class DispatchFn(torch.autograd.Function):
