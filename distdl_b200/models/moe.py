@@ -111,11 +111,12 @@ class MoEFeedForward(torch.nn.Module):
         self.aux_loss = None
         self.last_dropped = None
         self.router_bias = None
-        self._routed = None             # pairs per expert since the last take_routed()
         if cfg.router_bias:
             # the same on all workers: moved by the counts of all of them (Decoder.balance_routers)
             del self.router_bias
             self.register_buffer("router_bias", torch.zeros(E, dtype=torch.float32, device=dev))
+            # pairs per expert since the last take_routed(), added up in place: in a captured step, too
+            self.register_buffer("_routed", torch.zeros(E, dtype=torch.int64, device=dev), persistent=False)
         self.collect_state = collect
         if collect:
             # serial layout: all experts along dimension 0, on the first worker only
@@ -161,8 +162,11 @@ class MoEFeedForward(torch.nn.Module):
     def take_routed(self):
         """Pairs that this worker has routed to every expert in training since the last call, as a numpy array; starts
         over.  (A block that recomputes its forward pass counts it twice, all experts alike.)"""
-        counts, self._routed = self._routed, None
-        return np.zeros(self.cfg.n_experts, dtype=np.int64) if counts is None else counts.cpu().numpy().astype(np.int64)
+        if self.router_bias is None:
+            return np.zeros(self.cfg.n_experts, dtype=np.int64)
+        counts = self._routed.cpu().numpy().copy()
+        self._routed.zero_()
+        return counts
 
     def forward(self, x):
         cfg = self.cfg
@@ -178,7 +182,7 @@ class MoEFeedForward(torch.nn.Module):
             top_groups=cfg.router_top_groups, group_score=cfg.router_group_score, renormalize=cfg.router_renormalize,
             scale=cfg.router_scale)
         if self.router_bias is not None and self.training:
-            self._routed = counts.long() if self._routed is None else self._routed + counts
+            self._routed += counts
         # load-balancing auxiliary loss (fraction routed x mean router probability)
         frac = counts.float() / float(T * k)
         self.aux_loss = E * (frac.detach() * (prob_sum / float(T))).sum()
