@@ -29,6 +29,8 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC,-fvisibility=hidden,-fopenmp",
     "--expt-relaxed-constexpr",
 ]
+# of single files: gradients below 2^-126 are numbers like others (fast math takes them for 0)
+FILE_FLAGS = {"grad_norm.cu": ["--ftz=false"]}
 
 
 def _nvcc() -> str:
@@ -56,12 +58,12 @@ def _compile_one(src: str, verbose: bool, hdr: str, force: bool, debug: bool = F
     obj = os.path.join(OBJ_DIR + ("_debug" if debug else ""), src.rsplit(".", 1)[0] + ".o")
     stamp = obj + ".stamp"
     with open(os.path.join(CSRC, src), "rb") as fh:
-        digest = hashlib.sha256(fh.read() + hdr.encode()).hexdigest()
+        digest = hashlib.sha256(fh.read() + (hdr + " ".join(FILE_FLAGS.get(src, []))).encode()).hexdigest()
     if not force and os.path.exists(obj) and os.path.exists(stamp):
         with open(stamp) as fh:
             if fh.read().strip() == digest:
                 return obj
-    cmd = [_nvcc(), *NVCC_FLAGS, *(["-DDD_BOUNDS_CHECK"] if debug else []), "-I", CSRC, "-c", os.path.join(CSRC, src),
+    cmd = [_nvcc(), *NVCC_FLAGS, *FILE_FLAGS.get(src, []), *(["-DDD_BOUNDS_CHECK"] if debug else []), "-I", CSRC, "-c", os.path.join(CSRC, src),
            "-o", obj]
     if src.endswith(".cpp"):
         cmd.insert(1, "-x")
