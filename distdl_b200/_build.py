@@ -63,8 +63,8 @@ def _compile_one(src: str, verbose: bool, hdr: str, force: bool, debug: bool = F
         with open(stamp) as fh:
             if fh.read().strip() == digest:
                 return obj
-    cmd = [_nvcc(), *NVCC_FLAGS, *FILE_FLAGS.get(src, []), *(["-DDD_BOUNDS_CHECK"] if debug else []), "-I", CSRC, "-c", os.path.join(CSRC, src),
-           "-o", obj]
+    cmd = [_nvcc(), *NVCC_FLAGS, *FILE_FLAGS.get(src, []), *(["-DDD_BOUNDS_CHECK"] if debug else []), "-I", CSRC,
+           "-c", os.path.join(CSRC, src), "-o", obj]
     if src.endswith(".cpp"):
         cmd.insert(1, "-x")
         cmd.insert(2, "cu")
