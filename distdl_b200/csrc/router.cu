@@ -383,7 +383,7 @@ __device__ __noinline__ int choose_in_64_bits(const RouteArgs& a, const float* l
       __syncwarp();
     }
     const int g = best_of_groups<double>(a, values, -INFINITY, b0, b1, step);
-    const double value = a.group_sum && b1 > -INFINITY ? b0 + b1 : b0;
+    const double value = a.group_sum && b1 > -INFINITY && b0 < INFINITY ? fmin(b0 + b1, DBL_MAX) : b0;
     const bool in = among_best(a, value, g, step);
     clear_others<double, C>(a, c, -INFINITY, in, first, left, step);
     __syncwarp();

@@ -179,7 +179,7 @@ def _choose(logits, E, k, how):
     c = _scores(l.masked_fill(best, -math.inf), E, score)[0]
     if bias is not None:
         c = c + bias.double()
-    elif groups == 1 or group_score == "max":
+    elif group_score == "max" or top_groups == groups or groups == E:
         c = l                                               # the same order, also where scores are no longer told apart
     c = c.clamp(max=torch.finfo(torch.float64).max)         # (+inf of a sigmoid or a bias: below what is no number)
     c = c.masked_fill((l == -math.inf) | torch.isnan(c), -math.inf).masked_fill(best, math.inf)
@@ -187,7 +187,8 @@ def _choose(logits, E, k, how):
         by = c.reshape(len(c), groups, E // groups).sort(dim=-1, descending=True).values
         value = by[..., 0]
         if group_score == "top2" and E > groups:
-            value = torch.where(by[..., 1] > -math.inf, value + by[..., 1], value)
+            value = torch.where((by[..., 1] > -math.inf) & (value < math.inf),
+                                (value + by[..., 1]).clamp(max=torch.finfo(torch.float64).max), value)
         kept = value.sort(dim=-1, descending=True, stable=True).indices[:, :top_groups]
         live = torch.zeros_like(value, dtype=torch.bool).scatter(1, kept, True)
         c = c.masked_fill(~live.repeat_interleave(E // groups, dim=1), -math.inf)
