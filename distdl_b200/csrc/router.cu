@@ -15,13 +15,14 @@
 //
 // The choice is that of exact arithmetic.  Experts are compared as integers: 23 bits of value over 9 bits that favour the
 // lower number.  16-bit logits that decide themselves (no bias, no sums of scores) fit into them; everything else is cut to
-// steps of 2^-23 of the token's range, and where two neighbours of the order are closer than their errors (and not alike in
-// logit and bias) those that matter are decided in 64 bits: some tokens in a thousand.  So neither the order of sums nor the fast
+// steps of 2^-23 of the token's range, and where one of the chosen and another expert are closer than their errors (and not
+// alike in logit and bias), or a sum of two holds a value below the range, those that matter are decided in 64 bits: some tokens
+// in a thousand.  So neither the order of sums nor the fast
 // exponential shows in the experts.
 //
 // A warp works on a token, its lanes on C consecutive experts each, which they sort; the k best are then the largest of the
 // lanes' first ones, k times, one warp-wide integer maximum each.  Above some thousand tokens instructions that follow from one
-// another bound it, 510 (softmax, no bias) to 820 (sigmoid, bias, 8 groups) per token of 256 experts: 16384 tokens 22 to 29 us
+// another bound it, 580 (softmax, no bias) to 840 (sigmoid, bias, 8 groups) per token of 256 experts: 16384 tokens 23 to 30 us
 // with the slots (with the experts unsorted and the winner's place looked for by ballot and shuffle 1 130 to 1 920, 40 to 66
 // us); below, a latency.  Slots follow in a second kernel (route_slot_kernel): a pair's
 // slot is its rank in pair order among the pairs of its expert, so nothing depends on how CTAs are scheduled; sums of p are

@@ -16,7 +16,8 @@ class DistributedQKNormRope(Module):
     and gathered on use, and their gradients are summed over them.  Positions as for ``ops.rope``: ``offset``, ``ranges`` or
     ``positions``.
 
-    A new tensor while gradients are recorded; otherwise ``qkv`` itself, changed in place, is returned."""
+    A new tensor while gradients are recorded; otherwise ``qkv`` itself, changed in place, is returned.  ``q_norm`` and
+    ``k_norm`` hold the weights and are not called themselves: hooks belong on this layer."""
 
     def __init__(self, P_x, head_dim, rotary=None, eps=1e-6, collect_state=False, device=None, dtype=None,
                  scale_backward=None, auto_clear_buffer=True):
