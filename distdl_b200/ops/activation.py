@@ -80,13 +80,13 @@ def _host_table(seq, head_dim, theta):
 
 def _kept_table(key, make, device):
     """The table of ``key``, copied from the host when it is first asked for: the copy has ended when this returns, so that
-    every stream may read it.  Under a dispatch mode (fake tensors, say) tables are made for the call alone."""
-    if _modes():
-        return make().to(device).contiguous()
+    every stream may read it.  Fake tensors get a fake one, which is not kept."""
     t = _rope_cache.get(key)
-    if t is None:
+    if t is None or (_modes() and torch._guards.detect_fake_mode() is not None):
         with torch.inference_mode(False):
-            t = _rope_cache[key] = make().to(device).contiguous()
+            t = make().to(device).contiguous()
+        if type(t) is torch.Tensor:
+            _rope_cache[key] = t
     return t
 
 

@@ -66,6 +66,17 @@ def test_tables_first_made_under_fake_tensors_or_in_inference_mode(place):
             ops.rope_(torch.randn(14, 4, 16), 7, 3, theta=theta, **place)
 
 
+def test_tables_are_kept_under_modes_whose_tensors_are_none_of_their_own():
+    from torch.utils.flop_counter import FlopCounterMode
+
+    from distdl_b200.ops.activation import rope_table, rope_table_ranges
+    with FlopCounterMode(display=False):
+        a, b = rope_table(7, 16, 703.0, "cpu"), rope_table_ranges(((1, 3), (9, 2)), 16, 703.0, "cpu")
+    assert rope_table(7, 16, 703.0, "cpu") is a and rope_table_ranges(((1, 3), (9, 2)), 16, 703.0, "cpu") is b
+    with FlopCounterMode(display=False):
+        assert rope_table(7, 16, 703.0, "cpu") is a
+
+
 def test_ranges_that_are_refused():
     x, r = torch.randn(14, 4, 16), ops.Rotary()
     for ranges, tokens in ((((0, 6),), 14), (((0, 8), (3, -1)), 14), (((0, 7),), 13), ((), 14)):
