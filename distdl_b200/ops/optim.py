@@ -108,6 +108,20 @@ def _tensors(tensors, norm=None):
             array.array("B", codes))
 
 
+def _parts(tensors, norm=None):
+    """(tensors that the kernels take, their :func:`_tensors` or None, the others)."""
+    lists = _tensors(tensors, norm)
+    if lists is not None:
+        return tensors, lists, []
+    taken = [t.dtype in _CODES and type(t) in _TYPES and _dense(t) for t in tensors]
+    if any(taken) and not all(taken):
+        mine = [t for t, own in zip(tensors, taken) if own]
+        lists = _tensors(mine, norm)
+        if lists is not None:
+            return mine, lists, [t for t, own in zip(tensors, taken) if not own]
+    return [], None, tensors
+
+
 def _flat(tensors):
     if isinstance(tensors, torch.Tensor):
         tensors = [tensors]
@@ -142,13 +156,16 @@ def _grad_norm(tensors, lists, norm, squared, max_norm, given, clip):
 def grad_norm(tensors, squared: bool = False) -> torch.Tensor:
     """The 2-norm of all elements of ``tensors`` (one tensor, or an iterable; None is passed over) as an fp32 scalar on their
     device, or with ``squared`` the sum of squares in fp64 (to be added over workers).  Squares and sums are formed in 64
-    bits, in an order that does not change from run to run.  bf16, fp16 and fp32, mixed as they come, run on the kernels."""
+    bits, in an order that does not change from run to run.  bf16, fp16 and fp32, mixed as they come, run on the kernels;
+    fp64, subclasses and views with holes among them by torch's operators."""
     tensors = _flat(tensors)
     if not tensors:
         return torch.zeros((), dtype=torch.float64 if squared else torch.float32)
-    lists = _tensors(tensors)
-    if lists is None:
-        total = _plain_sumsq(tensors)
+    mine, lists, others = _parts(tensors)
+    if others:
+        total = _plain_sumsq(others)
+        if mine:
+            total = total + grad_norm(mine, squared=True)
         return total if squared else total.sqrt().float()
     out = torch.empty((), dtype=torch.float64 if squared else torch.float32, device=tensors[0].device)
     _grad_norm(tensors, lists, None if squared else out, out if squared else None, 0.0, False, False)
@@ -172,17 +189,18 @@ def clip_grad_norm_(tensors, max_norm: float, norm: torch.Tensor = None) -> torc
         return torch.zeros((), dtype=torch.float32) if norm is None else norm
     if norm is not None and norm.device != tensors[0].device:
         raise ValueError(f"the norm is on {norm.device}, the gradients on {tensors[0].device}")
-    lists = _tensors(tensors, norm)
-    if lists is None:
+    mine, lists, others = _parts(tensors, norm)
+    if others and norm is None:
+        norm = grad_norm(tensors)
+    if mine:
+        given = norm is not None
+        if not given:
+            norm = torch.empty((), dtype=torch.float32, device=mine[0].device)
+        _grad_norm(mine, lists, norm, None, max_norm, given, True)
+        torch.autograd.graph.increment_version(mine)          # (passes over tensors of inference mode)
+    if others:
         with torch.no_grad():
-            norm = _plain_sumsq(tensors).sqrt().float() if norm is None else norm
             scale = (max_norm / (norm + 1e-6)).clamp(max=1.0).reshape(())
-            for t in tensors:
+            for t in others:
                 t.copy_(t * scale if t.dtype == torch.float64 else t.float() * scale)
-        return norm
-    given = norm is not None
-    if not given:
-        norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
-    _grad_norm(tensors, lists, norm, None, max_norm, given, True)
-    torch.autograd.graph.increment_version(tensors)           # (passes over tensors of inference mode)
     return norm
